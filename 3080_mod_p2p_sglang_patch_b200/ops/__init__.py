@@ -16,6 +16,7 @@ import torch
 
 from .._ext import cuda_ext
 from ..utils import launches
+from .fp8_pages import Fp8Pages, fp8_cache  # noqa: F401
 
 
 class _Workspace:
@@ -259,15 +260,38 @@ def rope_cos_sin(max_pos: int, head_dim: int, theta: float, device, scaling=None
     return torch.cat([ang.cos(), ang.sin()], dim=1).to(torch.float32).to(device)
 
 
+def _is_fp8(k_cache, v_cache) -> bool:
+    """Whether a (k, v) cache pair is in 8 bits; both or neither."""
+    k8 = isinstance(k_cache, Fp8Pages)
+    if k8 != isinstance(v_cache, Fp8Pages):
+        raise TypeError("k_cache and v_cache must both be Fp8Pages, or neither")
+    return k8
+
+
 def rope_and_cache(qkv, positions, cos_sin, nq, nkv, slots=None, k_cache=None, v_cache=None, q_out=None, page=16,
                    q_norm=None, k_norm=None, eps=0.0):
     """Rotate q/k (neox), write rotated q to q_out [T, nq, 128] and k/v to the
     paged cache at ``slots`` (int64 block*page+offset). ``q_norm`` /
     ``k_norm`` (bf16 [128]): Qwen3's per-head RMSNorm of q and k (epsilon
-    ``eps``) before the rotation, in the same launch."""
+    ``eps``) before the rotation, in the same launch.
+
+    With ``Fp8Pages`` caches, k (rotated, not rounded in between) and v are
+    rounded into them as they are written: each byte is the one that the exact
+    row's definition gives. Slots that are negative or past the cache are not
+    written; of tokens that name the same slot the last one is stored; a
+    position outside the table takes its nearest row."""
     T = qkv.shape[0]
     if q_out is None:
         q_out = torch.empty((T, nq, 128), dtype=qkv.dtype, device=qkv.device)
+    if _is_fp8(k_cache, v_cache) and slots is not None:
+        if page != 16:
+            raise ValueError("8-bit caches have pages of 16 tokens")
+        cuda_ext().rope_and_cache_kv8(qkv, positions, cos_sin, slots, q_out, k_cache.values, k_cache.exps,
+                                      v_cache.values, v_cache.exps, nq, nkv, q_norm, k_norm, float(eps))
+        launches.add(1)
+        return q_out
+    if slots is None:
+        k_cache = v_cache = None
     cuda_ext().rope_and_cache(qkv, positions, cos_sin, slots, q_out, k_cache, v_cache, nq, nkv, page, q_norm, k_norm,
                               float(eps))
     launches.add(1)
@@ -289,7 +313,7 @@ def qkv_rope_and_cache(x, w, positions, cos_sin, nq, nkv, slots=None, k_cache=No
     which round the same way)."""
     C = cuda_ext()
     T = x.shape[0]
-    if T > C.GEMV_MAX_ROWS or not _GEMV_ON:
+    if T > C.GEMV_MAX_ROWS or not _GEMV_ON or _is_fp8(k_cache, v_cache):
         return None
     q_out = torch.empty((T, nq, 128), dtype=torch.bfloat16, device=x.device)
     if not C.gemv_rope(x, w, positions, cos_sin, slots, q_out, k_cache, v_cache, nq, nkv, page):
@@ -364,20 +388,104 @@ def prefill_splits(n_tiles: int, nq: int, max_kv: int, sms: int = 148) -> int:
     return int(max(1, min(want, max_kv // 512, 16)))
 
 
-def prefill_attention(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, scale=None, out=None, splits=1):
+@dataclasses.dataclass
+class PagePlan:
+    """Where ``read_pages`` puts the pages of a ragged batch: ``table`` int32
+    [requests, pages], the output page of each request's page, and ``pages``,
+    how many the output has."""
+    table: torch.Tensor
+    pages: int
+
+
+def page_plan(kv_lens, columns: int) -> PagePlan:
+    """The plan (on the CPU) that packs the pages of requests of ``kv_lens``
+    tokens one after another; ``columns`` is the block table's width. Without a
+    plan every request gets ``columns`` pages of scratch."""
+    counts = torch.tensor([max(0, min(columns, -(-int(n) // 16))) for n in kv_lens], dtype=torch.int32)
+    i = torch.arange(columns, dtype=torch.int32)[None, :]
+    start = (counts.cumsum(0, dtype=torch.int32) - counts)[:, None]
+    return PagePlan(torch.where(i < counts[:, None], start + i, torch.full_like(i, -1)).contiguous(),
+                    int(counts.sum()))
+
+
+def read_pages(k_cache, v_cache, block_table, kv_len, out_table=None, k_out=None, v_out=None):
+    """Pages of an 8-bit cache back to bf16 (exact): (k, v) [pages, kv heads,
+    16, 128]. Page i of request r (block ``block_table[r, i]``) goes to page
+    ``out_table[r, i]`` of the outputs, by default ``r * columns + i``; the
+    entries used must differ. Pages behind ``kv_len[r]`` tokens, and entries
+    outside the outputs, are left as they were; rows behind the length in a
+    request's last page are zeros, as are pages whose block is not in the
+    cache. Returned new outputs (none given) are zeros where nothing is
+    written."""
+    if not _is_fp8(k_cache, v_cache):
+        raise TypeError("read_pages reads 8-bit caches (ops.Fp8Pages)")
+    if (k_out is None) != (v_out is None):
+        raise ValueError("k_out and v_out go together")
+    if k_out is None:
+        if out_table is not None:
+            raise ValueError("out_table names pages of k_out and v_out: give them too")
+        shape = (block_table.shape[0] * block_table.shape[1],) + tuple(k_cache.shape[1:])
+        k_out = torch.zeros(shape, dtype=torch.bfloat16, device=k_cache.device)
+        v_out = torch.zeros_like(k_out)
+    cuda_ext().read_pages_kv8(k_cache.values, k_cache.exps, v_cache.values, v_cache.exps, block_table, kv_len,
+                              out_table, k_out, v_out)
+    launches.add(1)
+    return k_out, v_out
+
+
+_PAGE_IDS = {}  # device -> [0, 1, 2, ...] in growing lengths: the block table of scratch pages in order
+
+
+def _page_ids(n, device):
+    if torch.cuda.is_current_stream_capturing():
+        return torch.arange(n, dtype=torch.int32, device=device)
+    ids = _PAGE_IDS.setdefault(device, [])
+    if not ids or ids[-1].numel() < n:
+        # copied from the host before this returns, so any stream may read it;
+        # shorter ones stay alive for the launches that have them
+        ids.append(torch.arange(max(n, 4096, 2 * ids[-1].numel() if ids else 0), dtype=torch.int32).to(device))
+    return ids[-1][:n]
+
+
+def prefill_attention(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, scale=None, out=None, splits=1,
+                      plan=None):
     """Causal chunked-prefill attention over the paged cache, tcgen05/TMEM
     kernel; ``tiles`` from ``prefill_tiles(q_lens)`` (128-row tiles).
     ``splits`` > 1 splits each query tile's keys across CTAs (see
-    ``prefill_splits``); the partials are merged by a combine kernel."""
+    ``prefill_splits``); the partials are merged by a combine kernel.
+
+    ``Fp8Pages`` caches are read back to bf16 scratch pages first
+    (``read_pages``; placed by ``plan``, a ``page_plan`` on the device)."""
     if out is None:
         out = torch.empty_like(q)
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    if _is_fp8(k_cache, v_cache):
+        return _prefill_fp8(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, scale, out, splits, plan)
     po = pl = None
     if splits > 1:
         T, nq, _ = q.shape
         po, pl = workspace(q.device).prefill(T * nq * splits * 128, T * nq * splits)
     cuda_ext().prefill_attention_tc(q, k_cache, v_cache, out, cu_q, kv_len, block_table, tiles, scale,
                                     workspace(q.device).err, splits, po, pl)
+    launches.add(2 if splits > 1 else 1)
+    return out
+
+
+def _prefill_fp8(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, scale, out, splits, plan):
+    # Scratch comes from the caching allocator call by call, not from the shared
+    # workspace: two captured graphs (or two streams) never meet in it.
+    R, cols = block_table.shape
+    pages = R * cols if plan is None else plan.pages
+    table = _page_ids(pages, q.device).view(R, cols) if plan is None else plan.table
+    kv = torch.empty((2, max(1, pages)) + tuple(k_cache.shape[1:]), dtype=torch.bfloat16, device=q.device)
+    read_pages(k_cache, v_cache, block_table, kv_len, out_table=table, k_out=kv[0], v_out=kv[1])
+    po = pl = None
+    if splits > 1:
+        part = torch.empty(q.numel() // 128 * splits * 129, dtype=torch.float32, device=q.device)
+        po, pl = part[:q.numel() * splits], part[q.numel() * splits:]
+    with torch.cuda.device(q.device):
+        cuda_ext().prefill_attention_tc(q, kv[0], kv[1], out, cu_q, kv_len, table, tiles, scale,
+                                        workspace(q.device).err, splits, po, pl)
     launches.add(2 if splits > 1 else 1)
     return out
 
@@ -404,10 +512,24 @@ def decode_splits(batch: int, nkv: int, max_len: int, sms: int = 148) -> int:
 
 
 def decode_attention(q, k_cache, v_cache, kv_len, block_table, scale=None, splits=1, out=None):
+    """Attention of one new token per request: q [B, nq, 128] over the paged
+    cache, ``kv_len[b]`` keys each (0: zeros), split-KV over ``splits``.
+
+    Over ``Fp8Pages`` caches the kernel divides the work by itself
+    (``splits`` is not used): lengths are clamped to the block table, and
+    keys of blocks outside the cache do not count."""
     if out is None:
         out = torch.empty_like(q)
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     B, nq, _ = q.shape
+    if _is_fp8(k_cache, v_cache):
+        nkv, cols = k_cache.shape[1], block_table.shape[1]
+        s = int(max(1, min(2368 // max(1, B * nkv), cols // 8, 64)))
+        part = torch.empty(B * nq * s * 129, dtype=torch.float32, device=q.device)
+        cuda_ext().decode_attention_kv8(q, k_cache.values, k_cache.exps, v_cache.values, v_cache.exps, out, kv_len,
+                                        block_table, scale, s, part[:B * nq * s * 128], part[B * nq * s * 128:])
+        launches.add(2)
+        return out
     po = pl = cnt = None
     if splits > 1:
         ws = workspace(q.device)

@@ -13,6 +13,7 @@ extension, and it is not a serving path.
 import torch
 
 from . import reference as ref
+from .fp8_pages import Fp8Pages, quantize_rows
 
 BF16 = torch.bfloat16
 
@@ -56,11 +57,15 @@ def rope_and_cache(qkv, positions, cos_sin, nq, nkv, slots=None, k_cache=None, v
     """Rotate q/k of the fused [T, (nq + 2 nkv) D] projection (neox halves),
     store k/v at the paged ``slots`` (block * page + offset); returns q.
     ``q_norm`` / ``k_norm``: per-head RMSNorm of q and k first (Qwen3), kept
-    in fp32 into the rotation."""
+    in fp32 into the rotation. ``Fp8Pages`` caches take rows rounded once, k's
+    from fp64."""
     T = qkv.shape[0]
     D = cos_sin.shape[1]
     q = qkv[:, :nq * D].view(T, nq, D)
     k = qkv[:, nq * D:(nq + nkv) * D].view(T, nkv, D)
+    fp8 = isinstance(k_cache, Fp8Pages)
+    if fp8:
+        k = k.double()
     if q_norm is not None:
         q, k = ref.rmsnorm(q, q_norm, eps), ref.rmsnorm(k, k_norm, eps)
     v = qkv[:, (nq + nkv) * D:(nq + 2 * nkv) * D].view(T, nkv, D)
@@ -68,6 +73,12 @@ def rope_and_cache(qkv, positions, cos_sin, nq, nkv, slots=None, k_cache=None, v
     if slots is not None:
         s = slots.long()
         blk, off = s // page, s % page
+        if fp8:
+            for c, rows in ((k_cache, ref.rope(k, positions, cos_sin)), (v_cache, v.float())):
+                values, exps = quantize_rows(rows)
+                c.values.view(torch.uint8)[blk, :, off, :] = values.view(torch.uint8)
+                c.exps[blk, :, off] = exps
+            return _emit(qr, qkv.dtype, q_out)
         k_cache[blk, :, off, :] = ref.rope(k, positions, cos_sin).to(k_cache.dtype)
         v_cache[blk, :, off, :] = v.to(v_cache.dtype)
     return _emit(qr, qkv.dtype, q_out)

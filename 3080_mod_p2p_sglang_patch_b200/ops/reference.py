@@ -1,9 +1,16 @@
 """Plain PyTorch (fp32) references of every kernel, for numerics tests and the
-cuBLAS/NCCL baseline model path. Shapes/semantics match ``ops``."""
+cuBLAS/NCCL baseline model path. Shapes/semantics match ``ops``. ``rmsnorm``
+and ``rope`` stay in fp64 when given fp64."""
 import math
 
 import torch
 import torch.nn.functional as F
+
+from .fp8_pages import Fp8Pages, dequantize_rows
+
+
+def _wide(x):
+    return x if x.dtype == torch.float64 else x.float()
 
 
 def gemm(a, w, residual=None):
@@ -14,7 +21,7 @@ def gemm(a, w, residual=None):
 
 
 def rmsnorm(x, w, eps):
-    xf = x.float()
+    xf = _wide(x)
     return xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps) * w.float()
 
 
@@ -28,7 +35,7 @@ def rope(x, positions, cos_sin):
     D = x.shape[-1]
     cs = cos_sin[positions.long()]  # [T, D]
     c, s = cs[:, : D // 2].unsqueeze(1), cs[:, D // 2:].unsqueeze(1)
-    x1, x2 = x.float()[..., : D // 2], x.float()[..., D // 2:]
+    x1, x2 = _wide(x)[..., : D // 2], _wide(x)[..., D // 2:]
     return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1)
 
 
@@ -39,9 +46,13 @@ def silu_mul(x):
 
 
 def gather_kv(cache, block_table_row, length, page=16):
-    """[length, nkv, D] from a paged cache [blocks, nkv, page, D]."""
+    """[length, nkv, D] from a paged cache [blocks, nkv, page, D] (bf16, or
+    ``Fp8Pages``: then fp32, exact)."""
     idx = torch.arange(length, device=cache.device)
     blk = block_table_row.long()[idx // page]
+    if isinstance(cache, Fp8Pages):  # indexed as bytes: not every build indexes float8
+        values = cache.values.view(torch.uint8)[blk, :, idx % page, :].view(cache.values.dtype)
+        return dequantize_rows(values, cache.exps[blk, :, idx % page])
     return cache[blk, :, idx % page, :]
 
 

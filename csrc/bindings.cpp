@@ -5,7 +5,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cstring>
+#include <initializer_list>
+#include <utility>
 
 #include "kernels.h"
 #include "symm/symm.h"
@@ -512,6 +515,163 @@ void decode_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_ca
                           pl, (float)scale, cur_stream(), cnt);
 }
 
+// ---------------------------------------------------------------- 8-bit KV cache
+// Types, shapes and alignment are checked before the device, which comes last
+// (check_devices): a wrong call says what is wrong with it on any machine.
+void check_dense(const torch::Tensor& t, const char* name, torch::ScalarType type) {
+  TORCH_CHECK(t.scalar_type() == type, name, " must be ", type, ", is ", t.scalar_type());
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 || t.numel() == 0, name,
+              " must be 16-byte aligned");
+}
+void check_devices(std::initializer_list<std::pair<const char*, const torch::Tensor*>> ts) {
+  const torch::Tensor& first = *ts.begin()->second;
+  for (const auto& [name, t] : ts) {
+    if (t == nullptr) continue;
+    TORCH_CHECK(t->is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(t->device() == first.device(), name, " must be on ", first.device(), " like ", ts.begin()->first,
+                ", is on ", t->device());
+  }
+}
+
+// The e4m3 pages and exponents of one of K / V.
+void check_pages8(const torch::Tensor& v, const torch::Tensor& e, const char* name) {
+  TORCH_CHECK(v.scalar_type() == torch::kFloat8_e4m3fn && v.dim() == 4 && v.size(0) > 0 && v.size(1) > 0 &&
+                  v.size(2) == 16 && v.size(3) == 128,
+              name, " values must be float8_e4m3fn [blocks, nkv, 16, 128] with at least one block");
+  check_dense(v, name, torch::kFloat8_e4m3fn);
+  TORCH_CHECK(e.scalar_type() == torch::kUInt8 && e.dim() == 3 && e.size(0) == v.size(0) && e.size(1) == v.size(1) &&
+                  e.size(2) == 16,
+              name, " exps must be uint8 [blocks, nkv, 16]");
+  TORCH_CHECK(e.stride(2) == 1 && e.stride(0) % 16 == 0 && e.stride(1) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(e.data_ptr()) % 16 == 0,
+              name, " exps must be 16-byte aligned, with unit stride in a page and multiples of 16 between pages");
+  TORCH_CHECK(v.size(0) < (int64_t)1 << 27, name, ": too many blocks");
+}
+
+Kv8Cache kv8_cache(const torch::Tensor& kv, const torch::Tensor& ke, const torch::Tensor& vv, const torch::Tensor& ve,
+                   int64_t nkv) {
+  check_pages8(kv, ke, "k_cache");
+  check_pages8(vv, ve, "v_cache");
+  TORCH_CHECK(kv.size(1) == nkv, "the cache must have nkv = " + std::to_string(nkv) + " heads, has " + std::to_string(kv.size(1)));
+  TORCH_CHECK(kv.sizes() == vv.sizes(), "k_cache and v_cache must have the same shape");
+  Kv8Cache c;
+  c.kv = static_cast<uint8_t*>(kv.data_ptr());
+  c.vv = static_cast<uint8_t*>(vv.data_ptr());
+  c.ke = static_cast<uint8_t*>(ke.data_ptr());
+  c.ve = static_cast<uint8_t*>(ve.data_ptr());
+  c.ke_sb = ke.stride(0);
+  c.ke_sh = ke.stride(1);
+  c.ve_sb = ve.stride(0);
+  c.ve_sh = ve.stride(1);
+  c.blocks = kv.size(0);
+  return c;
+}
+
+// int32 [requests, pages] whose rows are contiguous (the row stride is free).
+void check_table(const torch::Tensor& t, const char* name, int64_t rows) {
+  TORCH_CHECK(t.scalar_type() == torch::kInt32 && t.dim() == 2 && t.size(0) == rows &&
+                  (t.size(1) <= 1 || t.stride(1) == 1),
+              name, " must be int32 [requests, pages] with contiguous rows");
+}
+void check_lens(const torch::Tensor& t) {
+  TORCH_CHECK(t.scalar_type() == torch::kInt32 && t.dim() == 1 && t.is_contiguous(),
+              "kv_len must be contiguous int32 [requests]");
+}
+
+void rope_and_cache_kv8(torch::Tensor qkv, torch::Tensor positions, torch::Tensor cos_sin, torch::Tensor slots,
+                        torch::Tensor q_out, torch::Tensor kv, torch::Tensor ke, torch::Tensor vv, torch::Tensor ve,
+                        int64_t nq, int64_t nkv, c10::optional<torch::Tensor> q_norm,
+                        c10::optional<torch::Tensor> k_norm, double eps) {
+  check_dense(qkv, "qkv", torch::kBFloat16);
+  TORCH_CHECK(nq > 0 && nkv > 0 && qkv.dim() == 2 && qkv.size(1) == (nq + 2 * nkv) * 128,
+              "qkv must be [T, (nq + 2 nkv) * 128]");
+  const Kv8Cache c = kv8_cache(kv, ke, vv, ve, nkv);
+  const int64_t T = qkv.size(0);
+  check_dense(q_out, "q_out", torch::kBFloat16);
+  TORCH_CHECK(q_out.numel() == T * nq * 128, "q_out must be [T, nq, 128]");
+  TORCH_CHECK(positions.scalar_type() == torch::kInt32 && positions.numel() == T && positions.is_contiguous(),
+              "positions must be contiguous int32 [T]");
+  TORCH_CHECK(slots.scalar_type() == torch::kInt64 && slots.numel() == T && slots.is_contiguous(),
+              "slots must be contiguous int64 [T]");
+  check_dense(cos_sin, "cos_sin", torch::kFloat32);
+  TORCH_CHECK(cos_sin.dim() == 2 && cos_sin.size(1) == 128 && cos_sin.size(0) > 0 &&
+                  cos_sin.size(0) < (int64_t)1 << 31,
+              "cos_sin must be fp32 [P, 128]");
+  TORCH_CHECK(T * (nq + 2 * nkv) < (int64_t)1 << 31, "rope: too many rows");
+  TORCH_CHECK(q_norm.has_value() == k_norm.has_value(), "q_norm and k_norm go together");
+  if (q_norm.has_value()) {
+    check_dense(*q_norm, "q_norm", torch::kBFloat16);
+    check_dense(*k_norm, "k_norm", torch::kBFloat16);
+    TORCH_CHECK(q_norm->numel() == 128 && k_norm->numel() == 128, "q_norm / k_norm must be [128]");
+  }
+  check_devices({{"qkv", &qkv}, {"positions", &positions}, {"cos_sin", &cos_sin}, {"slots", &slots},
+                 {"q_out", &q_out}, {"k_cache", &kv}, {"k_cache exps", &ke}, {"v_cache", &vv}, {"v_cache exps", &ve},
+                 {"q_norm", q_norm ? &*q_norm : nullptr}, {"k_norm", k_norm ? &*k_norm : nullptr}});
+  const at::cuda::CUDAGuard guard(qkv.device());
+  rope_and_cache_kv8_launch(qkv.data_ptr(), positions.data_ptr<int>(), cos_sin.data_ptr<float>(), cos_sin.size(0),
+                            slots.data_ptr<int64_t>(), q_out.data_ptr(), c, T, (int)nq, (int)nkv, cur_stream(),
+                            q_norm ? q_norm->data_ptr() : nullptr, k_norm ? k_norm->data_ptr() : nullptr, eps);
+}
+
+void read_pages_kv8(torch::Tensor kv, torch::Tensor ke, torch::Tensor vv, torch::Tensor ve, torch::Tensor block_table,
+                    torch::Tensor kv_len, c10::optional<torch::Tensor> out_table, torch::Tensor k_out,
+                    torch::Tensor v_out) {
+  check_pages8(kv, ke, "k_cache");
+  const int64_t nkv = kv.size(1);
+  const Kv8Cache c = kv8_cache(kv, ke, vv, ve, nkv);
+  check_lens(kv_len);
+  const int64_t R = kv_len.numel();
+  check_table(block_table, "block_table", R);
+  const int64_t mb = block_table.size(1);
+  check_dense(k_out, "k_out", torch::kBFloat16);
+  check_dense(v_out, "v_out", torch::kBFloat16);
+  TORCH_CHECK(k_out.dim() == 4 && k_out.size(1) == nkv && k_out.size(2) == 16 && k_out.size(3) == 128 &&
+                  v_out.sizes() == k_out.sizes(),
+              "k_out and v_out must be [pages, nkv, 16, 128]");
+  if (out_table.has_value()) {
+    check_table(*out_table, "out_table", R);
+    TORCH_CHECK(out_table->size(1) >= mb, "out_table must have a column for every column of block_table");
+  } else {
+    TORCH_CHECK(k_out.size(0) >= R * mb, "k_out and v_out must hold " + std::to_string(R * mb) + " pages (requests * columns)");
+  }
+  TORCH_CHECK(R * mb * nkv < (int64_t)1 << 31 && k_out.size(0) < (int64_t)1 << 31, "read_pages: too many pages");
+  check_devices({{"k_cache", &kv}, {"k_cache exps", &ke}, {"v_cache", &vv}, {"v_cache exps", &ve},
+                 {"block_table", &block_table}, {"kv_len", &kv_len}, {"out_table", out_table ? &*out_table : nullptr},
+                 {"k_out", &k_out}, {"v_out", &v_out}});
+  const at::cuda::CUDAGuard guard(kv.device());
+  read_pages_kv8_launch(c, (int)nkv, block_table.data_ptr<int>(), block_table.stride(0),
+                        out_table ? out_table->data_ptr<int>() : nullptr, out_table ? out_table->stride(0) : 0,
+                        kv_len.data_ptr<int>(), (int)R, (int)mb, k_out.data_ptr(), v_out.data_ptr(), k_out.size(0),
+                        cur_stream());
+}
+
+void decode_attention_kv8(torch::Tensor q, torch::Tensor kv, torch::Tensor ke, torch::Tensor vv, torch::Tensor ve,
+                          torch::Tensor out, torch::Tensor kv_len, torch::Tensor block_table, double scale,
+                          int64_t splits, torch::Tensor part_o, torch::Tensor part_lse) {
+  check_dense(q, "q", torch::kBFloat16);
+  TORCH_CHECK(q.dim() == 3 && q.size(2) == 128, "q must be [B, nq, 128]");
+  check_dense(out, "out", torch::kBFloat16);
+  TORCH_CHECK(out.sizes() == q.sizes(), "out must have q's shape");
+  check_pages8(kv, ke, "k_cache");
+  const int64_t B = q.size(0), nq = q.size(1), nkv = kv.size(1);
+  const Kv8Cache c = kv8_cache(kv, ke, vv, ve, nkv);
+  TORCH_CHECK(nq > 0 && nq % nkv == 0 && nq / nkv <= 16, "q heads must be 1 to 16 per kv head, a whole number");
+  check_lens(kv_len);
+  TORCH_CHECK(kv_len.numel() == B, "kv_len must be int32 [B]");
+  check_table(block_table, "block_table", B);
+  TORCH_CHECK(B * nkv * std::max<int64_t>(1, block_table.size(1)) < (int64_t)1 << 31, "decode: too many pages");
+  check_devices({{"q", &q}, {"k_cache", &kv}, {"k_cache exps", &ke}, {"v_cache", &vv}, {"v_cache exps", &ve},
+                 {"out", &out}, {"kv_len", &kv_len}, {"block_table", &block_table}, {"scratch", &part_o},
+                 {"scratch", &part_lse}});
+  TORCH_CHECK(part_o.numel() >= B * nq * splits * 128 && part_lse.numel() >= B * nq * splits,
+              "decode: scratch too small");
+  const at::cuda::CUDAGuard guard(q.device());
+  decode_attention_kv8_launch(q.data_ptr(), c, out.data_ptr(), kv_len.data_ptr<int>(), block_table.data_ptr<int>(),
+                              block_table.stride(0), (int)block_table.size(1), (int)B, (int)nq, (int)nkv, (int)splits,
+                              part_o.data_ptr<float>(), part_lse.data_ptr<float>(), (float)scale, cur_stream());
+}
+
 }  // namespace
 }  // namespace mbx
 
@@ -653,4 +813,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_attention", &decode_attention, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("out"),
         py::arg("kv_len"), py::arg("block_table"), py::arg("part_o"), py::arg("part_lse"), py::arg("splits"),
         py::arg("scale"), py::arg("counters") = c10::nullopt);
+  m.def("rope_and_cache_kv8", &rope_and_cache_kv8);
+  m.def("read_pages_kv8", &read_pages_kv8);
+  m.def("decode_attention_kv8", &decode_attention_kv8);
 }

@@ -182,4 +182,35 @@ void decode_attention_launch(const void* q, const void* kc, const void* vc, void
                              const int* block_table, int max_blocks, int B, int nq, int nkv, int splits,
                              float* part_o, float* part_lse, float scale, cudaStream_t s, int* counters = nullptr);
 
+// ---- 8-bit KV cache (attn/kv8.cu) ---------------------------------------------
+// Keys and values as e4m3 rows [blocks, nkv, 16, 128] with one exponent byte
+// per row [blocks, nkv, 16] (block and head strides in bytes, multiples of 16):
+// a row stands for values * 2^(exponent byte - 127).
+struct Kv8Cache {
+  uint8_t *kv, *vv;
+  uint8_t *ke, *ve;
+  int64_t ke_sb, ke_sh, ve_sb, ve_sh;
+  int64_t blocks;
+};
+// rope_and_cache_launch with the rotated k and the v rounded into the cache.
+// Negative slots and slots past the cache are not written; of two tokens with
+// the same slot the later one is stored. Positions are clamped to the table.
+void rope_and_cache_kv8_launch(const void* qkv, const int* pos, const float* cos_sin, int64_t max_pos,
+                               const int64_t* slots, void* q_out, const Kv8Cache& c, int64_t T, int nq, int nkv,
+                               cudaStream_t s, const void* q_norm = nullptr, const void* k_norm = nullptr,
+                               double eps = 0.0);
+// Pages of a ragged batch to bf16: page i of request r to page
+// out_table[r, i] (nullptr: r * max_blocks + i) of k_out / v_out [out_pages,
+// nkv, 16, 128]. Pages behind kv_len[r] and out entries outside [0, out_pages)
+// are skipped; rows behind the length and pages whose block is not in the
+// cache are written as zeros.
+void read_pages_kv8_launch(const Kv8Cache& c, int nkv, const int* block_table, int64_t bt_stride, const int* out_table,
+                           int64_t ot_stride, const int* kv_len, int R, int max_blocks, void* k_out, void* v_out,
+                           int64_t out_pages, cudaStream_t s);
+// decode_attention_launch over the 8-bit cache; lengths are clamped to
+// max_blocks pages, keys of blocks outside the cache do not count.
+void decode_attention_kv8_launch(const void* q, const Kv8Cache& c, void* o, const int* kv_len, const int* block_table,
+                                 int64_t bt_stride, int max_blocks, int B, int nq, int nkv, int splits, float* part_o,
+                                 float* part_lse, float scale, cudaStream_t s);
+
 }  // namespace mbx

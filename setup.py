@@ -2,7 +2,8 @@
 
 * ``_cpu``: host-only C++ runtime (CPU mailbox allreduce engine, FD exchange).
 * ``_C``:   CUDA for sm_100a only (symmetric memory, allreduce kernels,
-            tcgen05 GEMM, attention, elementwise ops, AWQ int4 GEMV/dequant).
+            tcgen05 GEMM, attention, elementwise ops, AWQ int4 GEMV/dequant,
+            the 8-bit KV cache).
 
 Usage: ``python setup.py build_ext --inplace`` (``__graft_entry__.build`` does
 this). The arch is passed explicitly as ``-gencode arch=compute_100a,
@@ -48,6 +49,7 @@ ext_modules = [
             src("attn", "attention.cu"),
             src("attn", "decode_noalloc.cu"),
             src("attn", "fmha_tc.cu"),
+            src("attn", "kv8.cu"),
             src("quant", "awq.cu"),
         ],
         include_dirs=[os.path.join(ROOT, "csrc")],

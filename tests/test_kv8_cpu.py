@@ -1,0 +1,221 @@
+"""The 8-bit KV cache's format, its PyTorch statement and its entry points'
+refusals (no GPU): a wrong call is refused before anything is launched."""
+import glob
+import os
+
+import pytest
+import torch
+
+from conftest import PKG, ROOT, sub
+
+D, PAGE = 128, 16
+
+
+def _built():
+    return bool(glob.glob(os.path.join(ROOT, PKG, "_C.*.so")))
+
+
+needs_ext = pytest.mark.skipif(not _built(), reason="_C is not built in this tree")
+
+
+def _brute(row):
+    """Exponent and values of one fp64 row by search over every e4m3 number."""
+    b = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    b = b[torch.isfinite(b)].unique()
+    top = max(abs(x) for x in row)
+    e = -117
+    while top > 448 * 2.0 ** e:
+        e += 1
+    out = []
+    for x in row:
+        d = (b * 2.0 ** e - x).abs()
+        near = b[d == d.min()]
+        if near.numel() > 1:  # a tie: the one whose last fraction bit is 0
+            near = near[[int(v.to(torch.float8_e4m3fn).view(torch.uint8)) % 2 == 0 for v in near.float()]]
+        out.append(float(near[0]) * 2.0 ** e)
+    return e, out
+
+
+def test_rows_are_the_nearest_e4m3_numbers_at_the_smallest_exponent():
+    f8 = sub("ops.fp8_pages")
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(24, D, generator=g, dtype=torch.float64) * torch.exp2(
+        torch.randint(-40, 40, (24, 1), generator=g).double())
+    x[0] = 0
+    x[1, :4] = torch.tensor([448.0, -432.0, 2.0 ** -9, 2.0 ** -10])          # top exactly 448: exponent 0; ties
+    x[1, 4:] = 0
+    x[2, 0] = 448.0 * (1 + 2.0 ** -40)                                       # just above: exponent 1
+    x[2, 1:] = 1.0
+    x[3] = x[3].sign() * 2.0 ** -133                                         # bf16's smallest: held at 2^-117
+    x[4, :3] = torch.tensor([400.0, 17 + 2.0 ** -30, 17 - 2.0 ** -30], dtype=x.dtype)  # next to a border, in 64 bits
+    x[4, 3:] = 17.0                                                          # the border itself: to even (16)
+    values, exps = f8.quantize_rows(x)
+    got = f8.dequantize_rows(values, exps).double()
+    for i in range(x.shape[0]):
+        e, want = _brute(x[i].tolist())
+        assert int(exps[i]) == e + 127, i
+        assert got[i].tolist() == want, i
+    assert int(exps[0]) == 10 and int(exps[1]) == 127 and int(exps[2]) == 128
+    assert got[4, 1:4].tolist() == [18.0, 16.0, 16.0]
+    # a stored row is exact in bf16
+    assert torch.equal(got.to(torch.bfloat16).double(), got)
+
+
+def test_elements_that_are_not_finite_become_nan_and_leave_the_rest_alone():
+    f8 = sub("ops.fp8_pages")
+    x = torch.linspace(-3, 3, D).repeat(2, 1)
+    y = x.clone()
+    y[1, 5], y[1, 9], y[1, 10] = float("inf"), float("nan"), float("-inf")
+    a, b = (f8.dequantize_rows(*f8.quantize_rows(t)) for t in (x, y))
+    bad = ~torch.isfinite(y)
+    assert torch.isnan(b[bad]).all() and torch.equal(b[~bad], a[~bad])
+
+
+def test_cache_constructor_layout():
+    ops = sub("ops")
+    k, v = ops.fp8_cache(3, 2, "cpu")
+    assert k.shape == (3, 2, PAGE, D) and v.values.dtype == torch.float8_e4m3fn
+    assert k.exps.shape == (3, 2, PAGE) and k.exps.stride() == (64, 32, 1)
+    assert v.exps.data_ptr() - k.exps.data_ptr() == PAGE
+    assert k.dequantize().abs().sum() == 0 and k.device.type == "cpu"
+
+
+def test_page_plan_packs_pages():
+    ops = sub("ops")
+    p = ops.page_plan([33, 0, 16, 200], 4)
+    assert p.pages == 3 + 0 + 1 + 4
+    assert p.table.tolist() == [[0, 1, 2, -1], [-1] * 4, [3, -1, -1, -1], [4, 5, 6, 7]]
+
+
+def test_oracle_writes_and_reads_the_format():
+    """The oracle's cache write and paged attention on an 8-bit cache."""
+    ops, oracle, ref, f8 = sub("ops"), sub("ops.oracle"), sub("ops.reference"), sub("ops.fp8_pages")
+    torch.manual_seed(0)
+    T, nq, nkv = 21, 4, 2
+    cs = ops.rope_cos_sin(64, D, 10000.0, "cpu")
+    qkv = torch.randn(T, (nq + 2 * nkv) * D).to(torch.bfloat16)
+    pos = torch.arange(T, dtype=torch.int32)
+    bt = torch.tensor([[2, 0]], dtype=torch.int32)
+    slots = bt[0].long()[pos.long() // PAGE] * PAGE + pos.long() % PAGE
+    w = (1 + 0.1 * torch.randn(D)).to(torch.bfloat16)
+    for norm in ({}, dict(q_norm=w, k_norm=w, eps=1e-5)):
+        k8, v8 = ops.fp8_cache(3, nkv, "cpu")
+        q = oracle.rope_and_cache(qkv, pos, cs, nq, nkv, slots, k8, v8, **norm)
+        k = qkv[:, nq * D:(nq + nkv) * D].view(T, nkv, D).double()
+        if norm:
+            k = ref.rmsnorm(k, w, 1e-5)
+        want, _ = f8.quantize_rows(ref.rope(k, pos, cs))
+        got = k8.values.view(torch.uint8)[slots // PAGE, :, slots % PAGE]
+        assert torch.equal(got, want.view(torch.uint8))
+        kk, vv = ref.gather_kv(k8, bt[0], T), ref.gather_kv(v8, bt[0], T)
+        # e4m3 keeps 4 significant bits: half a step is 2^-4 of the value
+        v = qkv[:, (nq + nkv) * D:].view(T, nkv, D).float()
+        top = v.abs().amax(-1, keepdim=True)
+        assert ((vv - v).abs() <= v.abs() * 2.0 ** -4 + top * 2.0 ** -17).all()
+        out = oracle.paged_attention(q, k8, v8, [T], [T], bt)
+        assert torch.equal(out, ref.attention(q, kk, vv, causal_offset=0).to(q.dtype))
+
+
+def _args(ops, T=3, nq=4, nkv=2, blocks=3):
+    k, v = ops.fp8_cache(blocks, nkv, "cpu")
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    return dict(
+        rope=dict(qkv=bf(T, (nq + 2 * nkv) * D), positions=i32(T), cos_sin=torch.zeros(8, D), nq=nq, nkv=nkv,
+                  slots=torch.zeros(T, dtype=torch.int64), k_cache=k, v_cache=v),
+        read=dict(k_cache=k, v_cache=v, block_table=i32(T, 2), kv_len=i32(T)),
+        decode=dict(q=bf(T, nq, D), k_cache=k, v_cache=v, kv_len=i32(T), block_table=i32(T, 2)))
+
+
+def _pages(ops, **kw):
+    k, _ = ops.fp8_cache(kw.pop("blocks", 3), kw.pop("nkv", 2), "cpu")
+    return ops.Fp8Pages(kw.get("values", k.values), kw.get("exps", k.exps))
+
+
+REFUSED = [
+    ("rope", dict(page=32), "16 tokens"),
+    ("rope", dict(qkv="float"), "qkv must be"),
+    ("rope", dict(nq=3), "qkv must be"),
+    ("rope", dict(nkv=0), "qkv must be"),
+    ("rope", dict(positions="long"), "positions must be"),
+    ("rope", dict(slots="int"), "slots must be"),
+    ("rope", dict(cos_sin=torch.zeros(0, D)), "cos_sin must be"),
+    ("rope", dict(cos_sin=torch.zeros(8, 64)), "cos_sin must be"),
+    ("rope", dict(q_norm=torch.zeros(D, dtype=torch.bfloat16)), "go together"),
+    ("rope", dict(q_out=torch.zeros(1, dtype=torch.bfloat16)), "q_out must be"),
+    ("read", dict(kv_len="long"), "kv_len must be"),
+    ("read", dict(block_table=torch.zeros(2, 2, dtype=torch.int32)), "block_table must be"),
+    ("read", dict(k_out=torch.zeros(5, 2, PAGE, D, dtype=torch.bfloat16),
+                  v_out=torch.zeros(5, 2, PAGE, D, dtype=torch.bfloat16)), "must hold"),
+    ("read", dict(k_out=torch.zeros(6, 2, PAGE, D, dtype=torch.bfloat16),
+                  v_out=torch.zeros(6, 2, PAGE, D)), "v_out must be"),
+    ("read", dict(k_out=torch.zeros(6, 2, PAGE, D, dtype=torch.bfloat16),
+                  v_out=torch.zeros(6, 2, PAGE, D, dtype=torch.bfloat16),
+                  out_table=torch.zeros(3, 1, dtype=torch.int32)), "out_table must have"),
+    ("decode", dict(q=torch.zeros(3, 4, 64, dtype=torch.bfloat16)), "q must be"),
+    ("decode", dict(q=torch.zeros(3, 5, D, dtype=torch.bfloat16)), "q heads"),
+    ("decode", dict(q=torch.zeros(3, 34, D, dtype=torch.bfloat16)), "q heads"),
+    ("decode", dict(q=torch.zeros(3, 8, D, dtype=torch.bfloat16)[:, ::2]), "contiguous"),
+    ("decode", dict(kv_len=torch.zeros(2, dtype=torch.int32)), "kv_len must be"),
+    ("decode", dict(block_table=torch.zeros(3, 4, dtype=torch.int32)[:, ::2]), "block_table must be"),
+    ("decode", dict(out=torch.zeros(3, 4, D)), "out must be"),
+]
+
+
+def _call(ops, which, a):
+    return dict(rope=ops.rope_and_cache, read=ops.read_pages, decode=ops.decode_attention)[which](**a)
+
+
+@needs_ext
+@pytest.mark.parametrize("which,change,message", REFUSED)
+def test_refusals(which, change, message):
+    ops = sub("ops")
+    a = _args(ops)[which]
+    for name, v in change.items():
+        a[name] = getattr(a[name], v)() if isinstance(v, str) else v
+    with pytest.raises((RuntimeError, ValueError), match=message):
+        _call(ops, which, a)
+
+
+@needs_ext
+@pytest.mark.parametrize("which", ["rope", "read", "decode"])
+def test_refusals_of_the_cache(which):
+    ops = sub("ops")
+    k, v = ops.fp8_cache(3, 2, "cpu")
+    for bad, message in ((ops.Fp8Pages(k.values.view(torch.uint8), k.exps), "float8_e4m3fn"),
+                         (ops.Fp8Pages(k.values[:, :, :8], k.exps), "float8_e4m3fn"),
+                         (ops.Fp8Pages(k.values[:0], k.exps[:0]), "at least one block"),
+                         (ops.Fp8Pages(k.values[:2], k.exps), "exps must be"),
+                         (ops.Fp8Pages(k.values, k.exps.float()), "exps must be"),
+                         (ops.Fp8Pages(k.values, torch.zeros(3, 2, 24, dtype=torch.uint8)[..., :16]), "exps must be"),
+                         (ops.Fp8Pages(k.values.transpose(0, 1), k.exps), "k_cache")):
+        a = _args(ops)[which]
+        a["k_cache"] = bad
+        with pytest.raises(RuntimeError, match=message):
+            _call(ops, which, a)
+    a = _args(ops)[which]
+    a["v_cache"] = _pages(ops, blocks=4)
+    with pytest.raises(RuntimeError, match="same shape"):
+        _call(ops, which, a)
+    a["v_cache"] = torch.zeros(3, 2, PAGE, D, dtype=torch.bfloat16)
+    with pytest.raises(TypeError, match="both be Fp8Pages"):
+        _call(ops, which, a)
+    # right in every respect but the device
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        _call(ops, which, _args(ops)[which])
+
+
+@needs_ext
+def test_refusals_of_head_counts_and_outputs():
+    ops = sub("ops")
+    a = _args(ops)["rope"]
+    a["k_cache"], a["v_cache"] = ops.fp8_cache(3, 1, "cpu")
+    with pytest.raises(RuntimeError, match="nkv = 2"):
+        ops.rope_and_cache(**a)
+    a = _args(ops)["read"]
+    with pytest.raises(ValueError, match="go together"):
+        ops.read_pages(**a, k_out=torch.zeros(6, 2, PAGE, D, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="give them too"):
+        ops.read_pages(**a, out_table=torch.zeros(3, 2, dtype=torch.int32))
+    with pytest.raises(TypeError, match="8-bit caches"):
+        ops.read_pages(torch.zeros(1), torch.zeros(1), a["block_table"], a["kv_len"])

@@ -1,0 +1,628 @@
+"""The 8-bit KV cache on the GPU against its definition in 64 bits: writing
+(byte for byte), reading back (exact), decode and prefill attention.
+
+Tolerances of attention, from the roundings alone (u16 = 2^-11, half a step of
+f16; ub = 2^-8, half a step of bf16), with A = sum_j p_j |v_j| / sum_j p_j:
+the weights' f16 rounding moves the output by at most u16 A, what underflows in
+f16 by n 2^-25 of the largest |v| / 2^8, and scores that are off by d (relative
+weights off by about d) by 2 d A. d: the fp32 sum of 128 exact products, its
+scaling and 2^x, at most 2^-17 of sum |q||k| * scale in log2 units plus 2^-21.
+Then the output's own rounding, ub |o|."""
+import pytest
+import torch
+
+from conftest import sub
+
+pytestmark = pytest.mark.gpu
+
+PAGE, D = 16, 128
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _bytes_of(pages):
+    return pages.values.view(torch.uint8)
+
+
+def _fill(pages, values, exps):
+    _bytes_of(pages).copy_(values.view(torch.uint8))
+    pages.exps.copy_(exps)
+
+
+def _cache(lens, nkv, seed=0, columns=None, spread=0, extra=3):
+    """A cache whose requests' rows are random and whose other rows are NaN
+    bytes with exponent 255; (k, v, kv_len, block_table)."""
+    ops, f8 = sub("ops"), sub("ops.fp8_pages")
+    g = _gen(seed)
+    counts = [-(-n // PAGE) for n in lens]
+    blocks = sum(counts) + extra
+    perm = torch.randperm(blocks, device="cuda", generator=g).to(torch.int32)
+    cols = columns or max(max(counts), 1)
+    table = torch.full((len(lens), cols), -1, dtype=torch.int32, device="cuda")
+    live = torch.zeros(blocks, PAGE, dtype=torch.bool, device="cuda")
+    at = 0
+    for r, n in enumerate(lens):
+        mine = perm[at:at + counts[r]]
+        table[r, :counts[r]] = mine
+        at += counts[r]
+        live[mine.long()] = torch.arange(counts[r] * PAGE, device="cuda").view(-1, PAGE) < n
+    cache = ops.fp8_cache(blocks, nkv, "cuda")
+    for i, c in enumerate(cache):
+        x = torch.randn(blocks, nkv, PAGE, D, device="cuda", generator=g)
+        if i == 0:
+            x[..., ::13] *= 3
+        if spread:  # rows of very different magnitude
+            x *= torch.exp2(torch.randint(-spread, spread + 1, (blocks, nkv, PAGE, 1), device="cuda",
+                                          generator=g).float())
+        v, e = f8.quantize_rows(x)
+        v = torch.where(live[:, None, :, None], v.view(torch.uint8), 0x7F)
+        _fill(c, v, torch.where(live[:, None, :], e, 255))
+    return cache[0], cache[1], torch.tensor(lens, dtype=torch.int32, device="cuda"), table
+
+
+def _row(pages, table_row, n):
+    """[n, nkv, 128] fp64 of a request."""
+    ref = sub("ops.reference")
+    if n == 0:
+        return torch.zeros(0, pages.shape[1], D, dtype=torch.float64, device="cuda")
+    return ref.gather_kv(pages, table_row, n).double()
+
+
+def _attention(q, k, v, scale, last=None):
+    """fp64 (output, tolerance) of q [rows, nq, 128] over k, v [n, nkv, 128];
+    row i sees keys 0..last[i]."""
+    G = q.shape[1] // k.shape[1]
+    q, k, v = q.double(), k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
+    n = k.shape[0]
+    if n == 0:
+        return torch.zeros_like(q), torch.zeros_like(q)
+    s = torch.einsum("qhd,khd->hqk", q, k) * scale
+    hidden = torch.zeros(q.shape[0], n, dtype=torch.bool, device=q.device)
+    if last is not None:
+        hidden = torch.arange(n, device=q.device)[None] > last[:, None]
+    p = torch.softmax(s.masked_fill(hidden, -torch.inf), -1)
+    o = torch.einsum("hqk,khd->qhd", p, v)
+    A = torch.einsum("hqk,khd->qhd", p, v.abs())
+    mag = torch.einsum("qhd,khd->hqk", q.abs(), k.abs()).masked_fill(hidden, 0).amax(-1).T[..., None] * abs(scale)
+    d = mag * 1.4427 * 2.0 ** -17 + 2.0 ** -21
+    tol = o.abs() * 2.0 ** -8 + A * (2.0 ** -11 + 2 * d) * 1.01 + n * 2.0 ** -33 * v.abs().amax() + 1e-30
+    return o, tol
+
+
+def _check_decode(out, q, k8, v8, table, lens, scale=D ** -0.5):
+    for b, n in enumerate(lens):
+        want, tol = _attention(q[b:b + 1], _row(k8, table[b], n), _row(v8, table[b], n), scale)
+        err = (out[b:b + 1].double() - want).abs()
+        assert (err <= tol).all(), f"request {b} of {n} keys: off by {(err / tol).max().item():.2f} of the tolerance"
+
+
+# ---------------------------------------------------------------- append
+def _append_case(T, nq, nkv, norm, seed, scale=1.0):
+    ops = sub("ops")
+    g = _gen(seed)
+    qkv = (torch.randn(T, (nq + 2 * nkv) * D, device="cuda", generator=g) * scale).to(torch.bfloat16)
+    pos = torch.randint(0, 4000, (T,), device="cuda", generator=g, dtype=torch.int32)
+    cs = ops.rope_cos_sin(4096, D, 500000.0, "cuda")
+    blocks = -(-T // PAGE) + 4
+    slots = torch.randperm(blocks * PAGE, device="cuda", generator=g)[:T]
+    kw = {}
+    if norm:
+        kw = dict(q_norm=(1 + 0.3 * torch.randn(D, device="cuda", generator=g)).to(torch.bfloat16),
+                  k_norm=(1 + 0.3 * torch.randn(D, device="cuda", generator=g)).to(torch.bfloat16), eps=1e-6)
+    return qkv, pos, cs, slots, blocks, kw
+
+
+def _append_want(qkv, pos, cs, nq, nkv, kw):
+    """fp64 q, k (rotated) and v, and the stored bytes of k and v."""
+    ref, f8 = sub("ops.reference"), sub("ops.fp8_pages")
+    T = qkv.shape[0]
+    x = qkv.double().view(T, nq + 2 * nkv, D)
+    q, k, v = x[:, :nq], x[:, nq:nq + nkv], x[:, nq + nkv:]
+    if kw:
+        q, k = ref.rmsnorm(q, kw["q_norm"], kw["eps"]), ref.rmsnorm(k, kw["k_norm"], kw["eps"])
+    q, k = ref.rope(q, pos, cs), ref.rope(k, pos, cs)
+    return q, f8.quantize_rows(k), f8.quantize_rows(v)
+
+
+def _check_append(q, k8, v8, qkv, pos, cs, slots, nq, nkv, kw):
+    want_q, (kv, ke), (vv, ve) = _append_want(qkv, pos, cs, nq, nkv, kw)
+    blk, off = slots // PAGE, slots % PAGE
+    for pages, v, e in ((k8, kv, ke), (v8, vv, ve)):
+        assert torch.equal(pages.exps[blk, :, off], e)
+        assert torch.equal(_bytes_of(pages)[blk, :, off], v.view(torch.uint8))
+    # q in fp32: two products and a sum, with the norm's 128-term sum, rsqrt and two products before it
+    mag = want_q.abs() + want_q.roll(D // 2, -1).abs()
+    tol = want_q.abs() * 2.0 ** -8 + mag * 2.0 ** -18
+    assert ((q.double() - want_q).abs() <= tol * 1.01 + 1e-30).all()
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("T,nq,nkv", [(1, 32, 8), (1, 1, 1), (2, 4, 1), (17, 8, 1), (33, 6, 2), (64, 32, 8),
+                                      (129, 64, 8), (1000, 8, 1), (515, 7, 7)])
+def test_append_writes_the_definition(T, nq, nkv, norm):
+    ops = sub("ops")
+    qkv, pos, cs, slots, blocks, kw = _append_case(T, nq, nkv, norm, T)
+    k8, v8 = ops.fp8_cache(blocks, nkv, "cuda")
+    for p in (k8, v8):
+        _bytes_of(p).fill_(0x55)
+        p.exps.fill_(77)
+    q = ops.rope_and_cache(qkv, pos, cs, nq, nkv, slots, k8, v8, **kw)
+    _check_append(q, k8, v8, qkv, pos, cs, slots, nq, nkv, kw)
+    # no other row changed
+    rest = torch.ones(blocks * PAGE, dtype=torch.bool, device="cuda")
+    rest[slots] = False
+    for p in (k8, v8):
+        assert (_bytes_of(p).transpose(1, 2).reshape(-1, nkv, D)[rest] == 0x55).all()
+        assert (p.exps.transpose(1, 2).reshape(-1, nkv)[rest] == 77).all()
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-38, 1e-30, 1e30])
+def test_append_extreme_magnitudes(scale):
+    ops = sub("ops")
+    T, nq, nkv = 9, 4, 2
+    qkv, pos, cs, slots, blocks, kw = _append_case(T, nq, nkv, False, 3, scale)
+    k8, v8 = ops.fp8_cache(blocks, nkv, "cuda")
+    ops.rope_and_cache(qkv, pos, cs, nq, nkv, slots, k8, v8)
+    _, (kv, ke), (vv, ve) = _append_want(qkv, pos, cs, nq, nkv, kw)
+    blk, off = slots // PAGE, slots % PAGE
+    for pages, v, e in ((k8, kv, ke), (v8, vv, ve)):
+        assert torch.equal(pages.exps[blk, :, off], e)
+        assert torch.equal(_bytes_of(pages)[blk, :, off].view(torch.float8_e4m3fn).float(), v.float())
+
+
+def test_append_borders_and_elements_that_are_not_finite():
+    """Rows on and next to rounding borders (position 0: no rotation), and
+    rows with NaN and infinities."""
+    ops, f8 = sub("ops"), sub("ops.fp8_pages")
+    nq, nkv, T = 1, 1, 6
+    cs = ops.rope_cos_sin(4, D, 10000.0, "cuda")
+    x = torch.zeros(T, 3, D, device="cuda")
+    ties = torch.tensor([448.0, 17.0, 19.0, 21.0, -17.0, -19.0, 1.0625, 1.1875, 2.0 ** -10, 3 * 2.0 ** -10], device="cuda")
+    x[0, 1:, :10] = ties
+    x[1, 1:, :10] = -ties * 2.0 ** 5
+    x[2, 1:] = 448.0
+    x[3, 1:] = 450.0          # just past: the next exponent
+    x[4, 1:] = torch.linspace(-2, 2, D, device="cuda")
+    x[4, 1:, 3], x[4, 1:, 70] = float("nan"), float("inf")
+    x[5, 1:] = float("-inf")
+    qkv = x.reshape(T, -1).to(torch.bfloat16)
+    pos = torch.zeros(T, dtype=torch.int32, device="cuda")
+    slots = torch.arange(T, device="cuda") + 5
+    k8, v8 = ops.fp8_cache(2, 1, "cuda")
+    ops.rope_and_cache(qkv, pos, cs, nq, nkv, slots, k8, v8)
+    v, e = f8.quantize_rows(qkv.view(T, 3, D)[:, 2:].float())
+    got = _bytes_of(v8)[slots // PAGE, :, slots % PAGE].view(torch.float8_e4m3fn).float()
+    assert torch.equal(v8.exps[slots // PAGE, :, slots % PAGE], e)
+    assert torch.equal(got.nan_to_num(nan=1e9), v.float().nan_to_num(nan=1e9))
+    # k: cos 1, sin 0 keeps finite rows; 0 * inf makes the partner NaN as well
+    assert torch.equal(k8.exps[slots // PAGE, :, slots % PAGE][:4], e[:4])
+    gk = _bytes_of(k8)[slots // PAGE, :, slots % PAGE].view(torch.float8_e4m3fn).float()
+    assert torch.equal(gk[:4], v.float()[:4])
+    assert torch.isnan(gk[4, 0, [3, 6, 67, 70]]).all() and torch.isnan(gk[4]).sum() == 4
+    assert torch.isnan(gk[5]).all()
+
+
+@pytest.mark.parametrize("T", [5, 300])
+def test_append_skips_slots_outside_and_keeps_the_last_of_equal_ones(T):
+    ops = sub("ops")
+    nq, nkv = 4, 2
+    qkv, pos, cs, slots, blocks, kw = _append_case(T, nq, nkv, False, 9)
+    slots[1] = -1
+    slots[2] = blocks * PAGE
+    slots[0] = slots[T - 1]           # the last token keeps it
+    if T > 100:
+        slots[40:90:7] = slots[97]    # several tokens, one slot; 97 is the last
+    k8, v8 = ops.fp8_cache(blocks, nkv, "cuda")
+    k0, v0 = k8.values.view(torch.uint8).clone(), v8.exps.clone()
+    q = ops.rope_and_cache(qkv, pos, cs, nq, nkv, slots, k8, v8)
+    last = {int(s): t for t, s in enumerate(slots.tolist()) if 0 <= s < blocks * PAGE}
+    keep = torch.tensor(sorted(last.values()), device="cuda")
+    want_q, (kv, ke), (vv, ve) = _append_want(qkv, pos, cs, nq, nkv, kw)
+    blk, off = slots[keep] // PAGE, slots[keep] % PAGE
+    for pages, v, e in ((k8, kv, ke), (v8, vv, ve)):
+        assert torch.equal(_bytes_of(pages)[blk, :, off], v.view(torch.uint8)[keep])
+        assert torch.equal(pages.exps[blk, :, off], e[keep])
+        mask = torch.ones(blocks, PAGE, dtype=torch.bool, device="cuda")
+        mask[blk, off] = False
+        assert (_bytes_of(pages).transpose(1, 2)[mask] == 0).all()
+    assert ((q.double() - want_q).abs() <= want_q.abs() * 2.0 ** -8 + 2e-5).all()
+
+
+def test_append_positions_outside_the_table_take_its_ends():
+    ops = sub("ops")
+    nq, nkv, T = 4, 2, 4
+    qkv, pos, cs, slots, blocks, kw = _append_case(T, nq, nkv, False, 2)
+    cs = cs[:100].contiguous()
+    bad = torch.tensor([-5, 100, 2 ** 31 - 1, 50], dtype=torch.int32, device="cuda")
+    k8, v8 = ops.fp8_cache(blocks, nkv, "cuda")
+    q = ops.rope_and_cache(qkv, bad, cs, nq, nkv, slots, k8, v8)
+    _check_append(q, k8, v8, qkv, bad.clamp(0, 99), cs, slots, nq, nkv, kw)
+
+
+def test_append_nothing():
+    ops = sub("ops")
+    k8, v8 = ops.fp8_cache(1, 1, "cuda")
+    cs = ops.rope_cos_sin(4, D, 10000.0, "cuda")
+    q = ops.rope_and_cache(torch.zeros(0, 3 * D, device="cuda", dtype=torch.bfloat16),
+                           torch.zeros(0, device="cuda", dtype=torch.int32), cs, 1, 1,
+                           torch.zeros(0, device="cuda", dtype=torch.int64), k8, v8)
+    assert q.shape == (0, 1, D)
+
+
+# ---------------------------------------------------------------- read
+@pytest.mark.parametrize("lens,nkv", [([1], 1), ([16], 2), ([17, 0, 31, 32, 33], 3), ([777], 8),
+                                      ([5, 300, 0, 64, 1029, 1], 8)])
+def test_read_pages(lens, nkv):
+    ops = sub("ops")
+    k8, v8, kvl, table = _cache(lens, nkv, seed=len(lens), spread=30)
+    R, cols = table.shape
+    fresh = ops.read_pages(k8, v8, table, kvl)
+    given = [torch.full((R * cols + 2, nkv, PAGE, D), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    ops.read_pages(k8, v8, table, kvl, k_out=given[0], v_out=given[1])
+    for pages, a, b in ((k8, fresh[0], given[0]), (v8, fresh[1], given[1])):
+        for r, n in enumerate(lens):
+            used = -(-n // PAGE)
+            for out, rest in ((a, 0.0), (b, 7.0)):
+                mine = out[r * cols:(r + 1) * cols]
+                rows = mine.transpose(1, 2).reshape(-1, nkv, D)
+                assert torch.equal(rows[:n].double(), _row(pages, table[r], n))
+                assert (rows[n:used * PAGE] == 0).all() and (rows[used * PAGE:] == rest).all()
+        assert (b[R * cols:] == 7.0).all()
+
+
+def test_read_pages_by_plan_strided_tables_and_bad_pages():
+    ops = sub("ops")
+    lens, nkv = [40, 0, 7, 100], 2
+    k8, v8, kvl, table = _cache(lens, nkv, seed=4, columns=7)
+    wide = torch.full((4, 12), 10 ** 9, dtype=torch.int32, device="cuda")
+    wide[:, 2:9] = table
+    view = wide[:, 2:9]
+    plan = ops.page_plan(lens, 7)
+    out = [torch.zeros(plan.pages, nkv, PAGE, D, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    ops.read_pages(k8, v8, view, kvl, out_table=plan.table.cuda(), k_out=out[0], v_out=out[1])
+    dense = ops.read_pages(k8, v8, table, kvl)
+    at = 0
+    for r, n in enumerate(lens):
+        for i in range(-(-n // PAGE)):
+            assert torch.equal(out[0][at], dense[0][r * 7 + i]) and torch.equal(out[1][at], dense[1][r * 7 + i])
+            at += 1
+    # blocks outside the cache read as zeros; output entries outside the output are skipped
+    bad = table.clone()
+    bad[0, 1], bad[3, 0] = -7, k8.shape[0]
+    t = plan.table.cuda()
+    t[2, 0], t[3, 1] = plan.pages, -3
+    out = [torch.full((plan.pages, nkv, PAGE, D), 3.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    ops.read_pages(k8, v8, bad, kvl, out_table=t, k_out=out[0], v_out=out[1])
+    assert (out[0][1] == 0).all() and (out[1][4] == 0).all()                # request 0 page 1, request 3 page 0
+    assert (out[0][3] == 3.0).all() and (out[1][5] == 3.0).all()            # the skipped ones
+    assert torch.equal(out[0][0], dense[0][0]) and torch.equal(out[1][6], dense[1][3 * 7 + 2])
+    # a length past the table reads the table's pages only
+    over = torch.full_like(kvl, 10 ** 6)
+    k, _ = ops.read_pages(k8, v8, table[3:], over[3:])
+    assert torch.equal(k[:6, :, :4], dense[0][21:27, :, :4])
+    # nothing to read
+    assert ops.read_pages(k8, v8, table[:0], kvl[:0])[0].shape[0] == 0
+    assert ops.read_pages(k8, v8, table[:, :0], kvl)[0].shape[0] == 0
+
+
+# ---------------------------------------------------------------- decode
+LENS = [1, 0, 2, 15, 16, 17, 31, 33, 100, 500, 777, 2049]
+
+
+@pytest.mark.parametrize("nq,nkv", [(1, 1), (3, 1), (4, 1), (7, 1), (8, 1), (9, 1), (16, 1), (32, 8), (64, 8),
+                                    (6, 2), (48, 3)])
+def test_decode_heads_and_lengths(nq, nkv):
+    ops = sub("ops")
+    k8, v8, kvl, table = _cache(LENS, nkv, seed=nq)
+    q = torch.randn(len(LENS), nq, D, device="cuda", generator=_gen(nq)).to(torch.bfloat16)
+    out = ops.decode_attention(q, k8, v8, kvl, table)
+    _check_decode(out, q, k8, v8, table, LENS)
+    assert (out[1] == 0).all()
+    # call after call the same bits, whatever the other requests' lengths
+    for _ in range(3):
+        assert torch.equal(ops.decode_attention(q, k8, v8, kvl, table), out)
+
+
+@pytest.mark.parametrize("lens", [[1], [16], [4096], [9000], [4096, 3], [33000, 0, 1, 20000]])
+def test_decode_few_long_requests(lens):
+    ops = sub("ops")
+    for nq, nkv in ((32, 8), (8, 1), (16, 1)):
+        k8, v8, kvl, table = _cache(lens, nkv, seed=lens[0])
+        q = torch.randn(len(lens), nq, D, device="cuda", generator=_gen(1)).to(torch.bfloat16)
+        out = ops.decode_attention(q, k8, v8, kvl, table)
+        _check_decode(out, q, k8, v8, table, lens)
+
+
+@pytest.mark.parametrize("B,nq,nkv", [(70, 8, 2), (300, 4, 4), (1100, 2, 1)])
+def test_decode_many_requests(B, nq, nkv):
+    ops = sub("ops")
+    lens = [(r * 37) % 130 for r in range(B)]
+    k8, v8, kvl, table = _cache(lens, nkv, seed=B)
+    q = torch.randn(B, nq, D, device="cuda", generator=_gen(2)).to(torch.bfloat16)
+    out = ops.decode_attention(q, k8, v8, kvl, table)
+    _check_decode(out, q, k8, v8, table, lens)
+
+
+@pytest.mark.parametrize("spread,qscale,scale", [(12, 1.0, None), (0, 30.0, None), (0, 1e-20, 1e20), (0, 1e20, 1e-20),
+                                                 (6, 1.0, -0.3), (0, 1.0, 0.0), (40, 1.0, 1e-9)])
+def test_decode_magnitudes(spread, qscale, scale):
+    """Rows whose scales differ by up to 2^80, sharp and flat softmaxes, the
+    weight of one row against many, negative and zero scales."""
+    ops = sub("ops")
+    lens, nq, nkv = [1, 40, 700, 3000], 16, 2
+    k8, v8, kvl, table = _cache(lens, nkv, seed=17, spread=spread)
+    if spread:  # k rows of one magnitude, so that the softmax is not one key's
+        k8 = _cache(lens, nkv, seed=17)[0]
+    q = (torch.randn(4, nq, D, device="cuda", generator=_gen(3)) * qscale).to(torch.bfloat16)
+    out = ops.decode_attention(q, k8, v8, kvl, table, scale=scale)
+    _check_decode(out, q, k8, v8, table, lens, scale if scale is not None else D ** -0.5)
+
+
+def test_decode_scores_that_rise_along_the_cache():
+    """The running maximum moves on every page; an early key of weight zero."""
+    ops, f8 = sub("ops"), sub("ops.fp8_pages")
+    n, nkv, nq = 1500, 1, 8
+    k8, v8, kvl, table = _cache([n], nkv, seed=5)
+    x = torch.zeros(-(-n // PAGE) * PAGE, nkv, D, device="cuda")
+    x[:, 0, 0] = torch.arange(x.shape[0], device="cuda") * 0.25
+    x[:, 0, 1:] = 0.1 * torch.randn(x.shape[0], D - 1, device="cuda", generator=_gen(5))
+    v, e = f8.quantize_rows(x.view(-1, PAGE, nkv, D).transpose(1, 2))
+    _bytes_of(k8)[table[0].long()] = v.view(torch.uint8)
+    k8.exps[table[0].long()] = e
+    for sign in (1.0, -1.0):
+        q = torch.randn(1, nq, D, device="cuda", generator=_gen(6)).to(torch.bfloat16)
+        q[..., 0] = 8.0 * sign
+        out = ops.decode_attention(q, k8, v8, kvl, table)
+        _check_decode(out, q, k8, v8, table, [n])
+
+
+def test_decode_non_finite_inputs_stay_in_their_rows():
+    ops = sub("ops")
+    lens, nq, nkv = [50, 50, 50, 600], 8, 2
+    k8, v8, kvl, table = _cache(lens, nkv, seed=8)
+    q = torch.randn(4, nq, D, device="cuda", generator=_gen(8)).to(torch.bfloat16)
+    want = ops.decode_attention(q, k8, v8, kvl, table)
+    q[0, 1, 5] = float("nan")
+    q[1, 2, 9] = float("inf")
+    _bytes_of(v8)[table[2, 1].long(), 1, 3, 7] = 0x7F    # one element of one row: heads 4..7, dim 7
+    _bytes_of(k8)[table[3, 20].long(), 0, 2, 0] = 0x7F   # one key: heads 0..3
+    out = ops.decode_attention(q, k8, v8, kvl, table)
+    bad = torch.zeros(4, nq, D, dtype=torch.bool, device="cuda")
+    bad[0, 1] = bad[1, 2] = True
+    bad[2, 4:, 7] = True
+    bad[3, :4] = True
+    assert torch.isnan(out[bad]).all()
+    assert torch.equal(out[~bad], want[~bad])
+
+
+def test_decode_tables_lengths_and_pages_outside():
+    ops = sub("ops")
+    lens, nq, nkv = [100, 40, 33], 8, 2
+    k8, v8, kvl, table = _cache(lens, nkv, seed=11, columns=8)
+    q = torch.randn(3, nq, D, device="cuda", generator=_gen(4)).to(torch.bfloat16)
+    out = ops.decode_attention(q, k8, v8, kvl, table)
+    wide = torch.full((3, 20), 10 ** 9, dtype=torch.int32, device="cuda")
+    wide[:, 5:13] = table
+    assert torch.equal(ops.decode_attention(q, k8, v8, kvl, wide[:, 5:13]), out)
+    # lengths behind the table end at it; negative ones are empty
+    over = torch.tensor([10 ** 9, 40, -5], dtype=torch.int32, device="cuda")
+    full = table[:, :6]
+    got = ops.decode_attention(q, k8, v8, over, full)
+    _check_decode(got[:2], q[:2], k8, v8, full, [96, 40])
+    assert (got[2] == 0).all()
+    # blocks outside the cache: their keys do not count
+    bad = table.clone()
+    bad[0, 2], bad[1, 0], bad[1, 1], bad[1, 2] = -1, k8.shape[0], 2 ** 31 - 1, -2 ** 31
+    got = ops.decode_attention(q, k8, v8, kvl, bad)
+    k = torch.cat([_row(k8, table[0], 100)[:32], _row(k8, table[0], 100)[48:]])
+    v = torch.cat([_row(v8, table[0], 100)[:32], _row(v8, table[0], 100)[48:]])
+    want, tol = _attention(q[:1], k, v, D ** -0.5)
+    assert ((got[:1].double() - want).abs() <= tol).all()
+    assert (got[1] == 0).all() and torch.equal(got[2], out[2])
+    # no requests, no columns
+    assert ops.decode_attention(q[:0], k8, v8, kvl[:0], table[:0]).shape == (0, nq, D)
+    assert (ops.decode_attention(q, k8, v8, kvl, table[:, :0]) == 0).all()
+    # rows of an output given are all that is written
+    o = torch.full((5, nq, D), 9.0, dtype=torch.bfloat16, device="cuda")
+    assert ops.decode_attention(q, k8, v8, kvl, table, out=o[1:4]).data_ptr() == o[1].data_ptr()
+    assert torch.equal(o[1:4], out) and (o[0] == 9).all() and (o[4] == 9).all()
+
+
+def test_decode_shared_pages():
+    """Two requests that share a prefix's pages, and one page named twice."""
+    ops = sub("ops")
+    k8, v8, kvl, table = _cache([80, 80], 2, seed=13)
+    table[1, :3] = table[0, :3]
+    table[1, 4] = table[1, 3]
+    q = torch.randn(2, 8, D, device="cuda", generator=_gen(4)).to(torch.bfloat16)
+    out = ops.decode_attention(q, k8, v8, kvl, table)
+    _check_decode(out, q, k8, v8, table, [80, 80])
+
+
+def test_decode_far_offsets():
+    """Pages whose bytes lie past 2^31 and 2^32 of the cache's start."""
+    ops = sub("ops")
+    nkv, nq, n = 8, 32, 200
+    k8, v8, kvl, table = _cache([n], nkv, seed=21)
+    blocks = (5 << 30) // (nkv * PAGE * D)
+    big = [ops.Fp8Pages(torch.empty(blocks, nkv, PAGE, D, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn),
+                        torch.empty(blocks, nkv, PAGE, dtype=torch.uint8, device="cuda")) for _ in range(2)]
+    far = torch.linspace(3, blocks - 1, table.shape[1], device="cuda").long().flip(0)
+    for a, b in zip(big, (k8, v8)):
+        _bytes_of(a)[far] = _bytes_of(b)[table[0].long()]
+        a.exps[far] = b.exps[table[0].long()]
+    q = torch.randn(1, nq, D, device="cuda", generator=_gen(4)).to(torch.bfloat16)
+    t = far.to(torch.int32)[None]
+    out = ops.decode_attention(q, *big, kvl, t)
+    assert torch.equal(out, ops.decode_attention(q, k8, v8, kvl, table))
+    k, v = ops.read_pages(*big, t, kvl)
+    want = ops.read_pages(k8, v8, table, kvl)
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+    # a row written at the far end
+    cs = ops.rope_cos_sin(8, D, 10000.0, "cuda")
+    qkv = torch.randn(1, (nq + 2 * nkv) * D, device="cuda", generator=_gen(1)).to(torch.bfloat16)
+    pos = torch.tensor([3], dtype=torch.int32, device="cuda")
+    slot = torch.tensor([blocks * PAGE - 2], device="cuda")
+    ops.rope_and_cache(qkv, pos, cs, nq, nkv, slot, *big)
+    _, (kb, ke), (vb, ve) = _append_want(qkv, pos, cs, nq, nkv, {})
+    assert torch.equal(_bytes_of(big[0])[-1, :, -2], kb[0].view(torch.uint8))
+    assert torch.equal(_bytes_of(big[1])[-1, :, -2], vb[0].view(torch.uint8)) and torch.equal(big[1].exps[-1, :, -2], ve[0])
+
+
+def test_separate_exponent_tensors():
+    """Exponents in tensors of their own, and with padding between heads."""
+    ops = sub("ops")
+    k8, v8, kvl, table = _cache([70, 5], 2, seed=2)
+    q = torch.randn(2, 4, D, device="cuda", generator=_gen(4)).to(torch.bfloat16)
+    out = ops.decode_attention(q, k8, v8, kvl, table)
+    pad = torch.empty(k8.shape[0], 2, 48, dtype=torch.uint8, device="cuda")
+    pad[..., 16:32] = k8.exps
+    a, b = ops.Fp8Pages(k8.values, pad[..., 16:32]), ops.Fp8Pages(v8.values, v8.exps.contiguous())
+    assert torch.equal(ops.decode_attention(q, a, b, kvl, table), out)
+    assert torch.equal(ops.read_pages(a, b, table, kvl)[0], ops.read_pages(k8, v8, table, kvl)[0])
+
+
+# ---------------------------------------------------------------- prefill
+def _check_prefill(out, q, k8, v8, table, q_lens, kv_lens):
+    """The tcgen05 kernel rounds its weights (at most 2^8) to bf16: ub A
+    instead of u16 A; the keys and values it reads are the cache's exactly."""
+    row = 0
+    for r, (ql, n) in enumerate(zip(q_lens, kv_lens)):
+        last = torch.arange(n - ql, n, device="cuda")
+        k, v = _row(k8, table[r], n), _row(v8, table[r], n)
+        want, tol = _attention(q[row:row + ql], k, v, D ** -0.5, last)
+        A, _ = _attention(q[row:row + ql], k, v.abs(), D ** -0.5, last)
+        err = (out[row:row + ql].double() - want).abs()
+        assert (err <= tol + A * 2.0 ** -8 * 1.01).all(), f"request {r}: {(err / (tol + A * 2.0 ** -8)).max().item()}"
+        row += ql
+
+
+@pytest.mark.parametrize("nq,nkv", [(32, 8), (8, 1), (3, 1)])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("planned", [False, True])
+def test_prefill_over_the_cache(nq, nkv, splits, planned):
+    ops = sub("ops")
+    kv_lens, q_lens = [100, 264, 1, 777, 16], [100, 64, 1, 257, 3]
+    k8, v8, kvl, table = _cache(kv_lens, nkv, seed=nq)
+    q = torch.randn(sum(q_lens), nq, D, device="cuda", generator=_gen(1)).to(torch.bfloat16)
+    cu = torch.tensor([0] + q_lens, device="cuda").cumsum(0).to(torch.int32)
+    plan = ops.page_plan(kv_lens, table.shape[1]) if planned else None
+    if planned:
+        plan.table = plan.table.cuda()
+    out = ops.prefill_attention(q, k8, v8, cu, kvl, table, ops.prefill_tiles(q_lens).cuda(), splits=splits, plan=plan)
+    torch.cuda.synchronize()
+    assert ops.gemm_error() == 0
+    _check_prefill(out, q, k8, v8, table, q_lens, kv_lens)
+
+
+# ---------------------------------------------------------------- together
+def test_append_then_attend():
+    """A prompt in two chunks, then tokens one by one, as a model's layer
+    makes the calls; every attention against the definition."""
+    ops = sub("ops")
+    nq, nkv = 8, 2
+    k8, v8 = ops.fp8_cache(40, nkv, "cuda")
+    for p in (k8, v8):
+        _bytes_of(p).fill_(0x7F)
+        p.exps.fill_(255)
+    table = torch.randperm(40, device="cuda", generator=_gen(0))[:20].to(torch.int32).view(2, 10)
+    cs = ops.rope_cos_sin(256, D, 500000.0, "cuda")
+    lens = [0, 0]
+    for step, new in enumerate([[70, 33], [31, 64], [1, 1], [1, 1], [1, 1]]):
+        T = sum(new)
+        pos = torch.cat([torch.arange(a, a + b, device="cuda") for a, b in zip(lens, new)])
+        row = torch.tensor([0] * new[0] + [1] * new[1], device="cuda")
+        slots = table.long()[row, pos // PAGE] * PAGE + pos % PAGE
+        lens = [a + b for a, b in zip(lens, new)]
+        qkv = torch.randn(T, (nq + 2 * nkv) * D, device="cuda", generator=_gen(step)).to(torch.bfloat16)
+        kvl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        q = ops.rope_and_cache(qkv, pos.to(torch.int32), cs, nq, nkv, slots, k8, v8)
+        _check_append(q, k8, v8, qkv, pos.to(torch.int32), cs, slots, nq, nkv, {})
+        if new == [1, 1]:
+            out = ops.decode_attention(q, k8, v8, kvl, table)
+            _check_decode(out, q, k8, v8, table, lens)
+        else:
+            cu = torch.tensor([0] + new, device="cuda").cumsum(0).to(torch.int32)
+            out = ops.prefill_attention(q, k8, v8, cu, kvl, table, ops.prefill_tiles(new).cuda())
+            _check_prefill(out, q, k8, v8, table, new, lens)
+
+
+def _layer(ops, s):
+    q = ops.rope_and_cache(s["qkv"], s["pos"], s["cs"], s["nq"], s["nkv"], s["slots"], s["k8"], s["v8"])
+    d = ops.decode_attention(q, s["k8"], s["v8"], s["kvl"], s["table"])
+    p = ops.prefill_attention(q, s["k8"], s["v8"], s["cu"], s["kvl"], s["table"], s["tiles"], splits=2)
+    return q, d, p
+
+
+def _layer_state(ops, seed, lens, nq=8, nkv=2):
+    k8, v8, kvl, table = _cache(lens, nkv, seed=seed)
+    B = len(lens)
+    last = kvl.long() - 1
+    return dict(nq=nq, nkv=nkv, k8=k8, v8=v8, kvl=kvl, table=table, cs=ops.rope_cos_sin(max(lens), D, 1e4, "cuda"),
+                pos=last.to(torch.int32), slots=table.long().gather(1, (last // PAGE)[:, None])[:, 0] * PAGE + last % PAGE,
+                qkv=torch.randn(B, (nq + 2 * nkv) * D, device="cuda", generator=_gen(seed)).to(torch.bfloat16),
+                cu=torch.arange(B + 1, dtype=torch.int32, device="cuda"), tiles=ops.prefill_tiles([1] * B).cuda())
+
+
+def test_two_captured_graphs_and_eager_calls_at_once():
+    """Two graphs captured on one stream, replayed on two at the same time
+    with eager calls on a third: nothing they use is shared."""
+    ops = sub("ops")
+    states = [_layer_state(ops, 1, [3000, 17, 900]), _layer_state(ops, 2, [5000, 1, 250, 4000]),
+              _layer_state(ops, 3, [2500] * 5)]
+    want = [_layer(ops, s) for s in states]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    for s in states[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append(_layer(ops, s))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for round_ in range(20):
+        for o in outs:
+            for t in o:
+                t.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(streams[0]):
+            graphs[0].replay()
+        with torch.cuda.stream(streams[1]):
+            graphs[1].replay()
+        with torch.cuda.stream(streams[2]):
+            eager = _layer(ops, states[2])
+        torch.cuda.synchronize()
+        for got, w in zip(outs + [eager], want):
+            for a, b in zip(got, w):
+                assert torch.equal(a, b), f"round {round_}"
+    # new inputs in the same buffers
+    fresh = _layer_state(ops, 7, [3000, 17, 900])
+    for name in ("qkv", "kvl", "table", "pos", "slots"):
+        states[0][name].copy_(fresh[name])
+    for name in ("k8", "v8"):
+        _fill(states[0][name], fresh[name].values, fresh[name].exps)
+    graphs[0].replay()
+    w = _layer(ops, fresh)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs[0], w))
+
+
+@pytest.mark.skipif(not torch.cuda.is_available() or torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_second_device_while_the_first_is_current():
+    ops = sub("ops")
+    s = _layer_state(ops, 1, [300, 17])
+    want = _layer(ops, s)
+    other = {}
+    for k, v in s.items():
+        if isinstance(v, torch.Tensor):
+            v = v.to("cuda:1")
+        elif isinstance(v, ops.Fp8Pages):
+            v = ops.Fp8Pages(v.values.to("cuda:1"), v.exps.contiguous().to("cuda:1"))
+        other[k] = v
+    got = _layer(ops, other)
+    torch.cuda.synchronize("cuda:1")
+    assert all(torch.equal(a, b.to("cuda:0")) for a, b in zip(want, got))
+    with pytest.raises(RuntimeError, match="must be on"):
+        ops.decode_attention(want[0], other["k8"], other["v8"], s["kvl"], s["table"])
