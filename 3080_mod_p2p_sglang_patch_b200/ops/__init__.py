@@ -518,18 +518,14 @@ def decode_attention(q, k_cache, v_cache, kv_len, block_table, scale=None, split
     Over ``Fp8Pages`` caches the kernel divides the work by itself
     (``splits`` is not used): lengths are clamped to the block table, and
     keys of blocks outside the cache do not count."""
+    scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    if _is_fp8(k_cache, v_cache):
+        launches.add(1)
+        return cuda_ext().decode_attention_kv8(q, k_cache.values, k_cache.exps, v_cache.values, v_cache.exps, out,
+                                               kv_len, block_table, scale)
     if out is None:
         out = torch.empty_like(q)
-    scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     B, nq, _ = q.shape
-    if _is_fp8(k_cache, v_cache):
-        nkv, cols = k_cache.shape[1], block_table.shape[1]
-        s = int(max(1, min(2368 // max(1, B * nkv), cols // 8, 64)))
-        part = torch.empty(B * nq * s * 129, dtype=torch.float32, device=q.device)
-        cuda_ext().decode_attention_kv8(q, k_cache.values, k_cache.exps, v_cache.values, v_cache.exps, out, kv_len,
-                                        block_table, scale, s, part[:B * nq * s * 128], part[B * nq * s * 128:])
-        launches.add(2)
-        return out
     po = pl = cnt = None
     if splits > 1:
         ws = workspace(q.device)

@@ -259,12 +259,12 @@ struct Kv8DecodeArgs {
   const uint8_t *kv, *vv, *ke, *ve;
   int64_t ke_sb, ke_sh, ve_sb, ve_sh;
   __nv_bfloat16* o;        // [B, nq, D]
-  float* part_o;           // [B, nq, splits, D]
-  float* part_lse;         // [B, nq, splits]
+  float* part;             // partial results of segments that span CTAs [grid][2][heads][D], then their (m, l)
+  int* counters;           // [grid] arrivals, zero between launches
   const int* kv_len;       // [B]
   const int* block_table;  // [B, max_blocks], row stride bt_s
   int64_t bt_s;
-  int max_blocks, num_blocks, nq, nkv, splits;
+  int B, max_blocks, num_blocks, nq, nkv;
   float scale_log2;
 };
 
@@ -434,49 +434,372 @@ struct HeadState {
   }
 };
 
-// One warp per (split, kv head, request), pages straight from global memory.
+// ---- the work's division
+// The pages of all (request, kv head) pairs form one list, pairs one after
+// another; every warp of the grid takes an equal run of it, whatever the
+// lengths are (they live on the device, so a captured graph adapts too). A
+// pair's pages inside one warp's run are a segment of that warp:
+//   * a pair that lies in one warp's run is finished by the warp alone;
+//   * otherwise each warp leaves a partial state (m, l, O) in shared memory, and
+//     the CTA folds its warps' partials, in order, into the output or, for a
+//     pair that reaches into other CTAs, into one partial in global memory; the
+//     last of those CTAs to arrive folds these in CTA order.
+// All orders are fixed, so results do not depend on timing. At most one pair
+// enters a CTA's run and one leaves it, hence two global partials per CTA.
+constexpr int kWarps = 8;
+constexpr int kStageBytes = 2 * PAGE * D + 64;  // K, V, 2 x 16 exponents
+constexpr int kRow = D + 4;                     // floats per head of a partial in shared memory (bank spread)
+
 template <int NT>
-__global__ void __launch_bounds__(32) decode_kv8_kernel(Kv8DecodeArgs a) {
-  pdl_wait();
-  const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-  const int lane = threadIdx.x, g = lane >> 2, t = lane & 3;
-  const int G = a.nq / a.nkv;
-  const int L = min(max(a.kv_len[b], 0), a.max_blocks * PAGE);
-  const int pages = (L + PAGE - 1) / PAGE;
-  const int per = (pages + a.splits - 1) / a.splits;
-  HeadState<NT> st;
-  st.begin(a.q + ((int64_t)b * a.nq + kvh * G) * D, G, a.scale_log2, lane);
-  for (int p = split * per; p < min(pages, split * per + per); ++p) {
-    const int blk = a.block_table[b * a.bt_s + p];
-    if (blk < 0 || blk >= a.num_blocks) continue;
-    const int64_t base = ((int64_t)blk * a.nkv + kvh) * PAGE * D;
-    uint4 k[4], v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      k[i] = ld_v4(a.kv + base + (g + 8 * (i >> 1)) * D + (t + 4 * (i & 1)) * 16);
-      v[i] = ld_v4(a.vv + base + (2 * t + (i & 1) + 8 * (i >> 1)) * D + g * 16);
-    }
-    const uint8_t* kep = a.ke + blk * a.ke_sb + kvh * a.ke_sh;
-    const uint8_t* vep = a.ve + blk * a.ve_sb + kvh * a.ve_sh;
-    const int ke[2] = {kep[g], kep[g + 8]}, ve[2] = {vep[g], vep[g + 8]};
-    st.page(k, v, ke, ve, min(PAGE, L - p * PAGE), lane);
+constexpr int kStages = NT == 1 ? 5 : 4;
+
+template <int NT>
+struct DecodeSmem {
+  static constexpr int kHeads = 8 * NT;
+  static constexpr int kRing = 0;
+  static constexpr int kSlot = kWarps * kStages<NT> * kStageBytes;        // [kWarps] partials: kHeads x kRow floats
+  static constexpr int kSlotBytes = kHeads * kRow * 4;
+  static constexpr int kMl = kSlot + kWarps * kSlotBytes;                 // float2 [2][kWarps][kHeads]
+  static constexpr int kTotal = kMl + 2 * kWarps * kHeads * 8;
+  static_assert(kStages<NT> * kStageBytes >= kSlotBytes, "the second partial of a warp lies in its ring");
+};
+
+MBX_DEVICE uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+MBX_DEVICE void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+MBX_DEVICE void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+MBX_DEVICE void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+MBX_DEVICE void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// What a warp's first (it began before the warp's run) and last (it goes on
+// behind it) segments left for the merge.
+struct SegMeta {
+  int valid;   // there is a partial
+  int ends;    // first segment only: the pair's pages end in this warp's run
+  int b, kvh;
+  int begin;   // list index of the pair's first page
+  int pages;
+};
+
+// One merge of partials of one head by one warp: lane l owns dims 4l..4l+3.
+struct Fold {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  MBX_DEVICE void add(float pm, float pl, const float4& po) {
+    const float nm = fmaxf(m, pm);
+    const float a = nm == -INFINITY ? 0.f : ex2(m - nm), b = nm == -INFINITY ? 0.f : ex2(pm - nm);
+    m = nm;
+    l = l * a + pl * b;
+    o.x = o.x * a + po.x * b;
+    o.y = o.y * a + po.y * b;
+    o.z = o.z * a + po.z * b;
+    o.w = o.w * a + po.w * b;
   }
-  st.end();
+  MBX_DEVICE void store(__nv_bfloat16* dst, int lane) const {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x * inv, o.y * inv);
+    const __nv_bfloat162 hi = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+    uint2 w;
+    w.x = *reinterpret_cast<const uint32_t*>(&lo);
+    w.y = *reinterpret_cast<const uint32_t*>(&hi);
+    *reinterpret_cast<uint2*>(dst + lane * 4) = w;
+  }
+};
+
+MBX_DEVICE int block_sum(int v, int* red) {
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int s = 0;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int head = n * 8 + 2 * t + c;
-      if (head >= G) continue;
-      const int64_t row = ((int64_t)b * a.nq + kvh * G + head) * a.splits + split;
-      const float l = st.l[n][c];
-      const float inv = l == 0.f ? 0.f : pow2(max(st.vr, -118) - 8) / l;
+  for (int i = 0; i < kWarps; ++i) s += red[i];
+  return s;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArgs a) {
+  using S = DecodeSmem<NT>;
+  constexpr int kSt = kStages<NT>;
+  pdl_wait();
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int red[kWarps];
+  __shared__ int start_b[kWarps], start_off[kWarps];
+  __shared__ SegMeta meta[2][kWarps];
+  __shared__ int s_last[2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int G = a.nq / a.nkv;
+  auto pages_of = [&](int b) {
+    return (min(max(a.kv_len[b], 0), a.max_blocks * PAGE) + PAGE - 1) / PAGE;
+  };
+  // ---- this warp's run [u0, u1) of the page list, and where it starts
+  if (threadIdx.x < 2 * kWarps) meta[threadIdx.x / kWarps][threadIdx.x % kWarps].valid = 0;
+  const int first = (int)threadIdx.x < a.B ? pages_of(threadIdx.x) : 0;
+  int sum = first;
+  for (int b = threadIdx.x + blockDim.x; b < a.B; b += blockDim.x) sum += pages_of(b);
+  const int total = block_sum(sum, red) * a.nkv;
+  const int n_warps = gridDim.x * kWarps;
+  const int run = max(1, (total + n_warps - 1) / n_warps);
+  const int cta_u0 = blockIdx.x * kWarps * run;
+  for (int b0 = 0, carry = 0; b0 < a.B; b0 += blockDim.x) {
+    const int b = b0 + threadIdx.x;
+    const int n = b0 == 0 ? first : (b < a.B ? pages_of(b) : 0);
+    int inc = n;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        *reinterpret_cast<float2*>(a.part_o + row * D + g * 16 + 2 * i) =
-            make_float2(st.o[n][i][c] * inv, st.o[n][i][2 + c] * inv);
-      if (g == 0) a.part_lse[row] = l == 0.f ? -INFINITY : st.m[n][c] + log2f(l);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
     }
+    __syncthreads();
+    if (lane == 31) red[warp] = inc;
+    __syncthreads();
+    int before = carry;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) before += red[i];
+      carry += red[i];
+    }
+    const int64_t lo = (int64_t)(before + inc - n) * a.nkv, hi = lo + (int64_t)n * a.nkv;
+    if (n > 0 && lo < (int64_t)cta_u0 + kWarps * run && hi > cta_u0)
+      for (int w = 0; w < kWarps; ++w) {
+        const int64_t u = (int64_t)cta_u0 + w * run;
+        if (u >= lo && u < hi) {
+          start_b[w] = b;
+          start_off[w] = (int)(u - lo);
+        }
+      }
+    // requests without keys: zeros, by the CTAs in turn
+    if (b < a.B && n == 0 && b % gridDim.x == blockIdx.x) {
+      uint4* dst = reinterpret_cast<uint4*>(a.o + (int64_t)b * a.nq * D);
+      for (int i = 0; i < a.nq * D / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  __syncthreads();
+
+  const int64_t u0 = (int64_t)cta_u0 + warp * run;
+  const int n_mine = u0 >= total ? 0 : (int)min((int64_t)run, total - u0);
+  const uint32_t ring = smem_addr(smem + S::kRing) + warp * kSt * kStageBytes;
+  if (n_mine > 0) {
+    // cursors into the list: the pages being fetched and the ones being used
+    struct Cursor {
+      int b, kvh, p, pages;
+    };
+    Cursor in, use;
+    in.b = start_b[warp];
+    in.pages = pages_of(in.b);
+    in.kvh = start_off[warp] / in.pages;
+    in.p = start_off[warp] % in.pages;
+    use = in;
+    auto next_pair = [&](Cursor& c) {
+      c.p = 0;
+      if (++c.kvh < a.nkv) return;
+      c.kvh = 0;
+      do {
+        ++c.b;
+        c.pages = pages_of(c.b);
+      } while (c.pages == 0);
+    };
+    int win = -1;       // first page of the table window that the lanes hold
+    int id = -1;
+    uint32_t bad = 0;   // stages whose page is not in the cache
+    auto fetch = [&](int st) {
+      if (in.p == in.pages) {
+        next_pair(in);
+        win = -1;
+      }
+      if (win < 0 || in.p >= win + 32) {
+        win = in.p;
+        id = in.p + lane < in.pages ? a.block_table[in.b * a.bt_s + in.p + lane] : -1;
+      }
+      const int blk = __shfl_sync(0xffffffffu, id, in.p - win);
+      const uint32_t dst = ring + st * kStageBytes;
+      if (blk >= 0 && blk < a.num_blocks) {
+        bad &= ~(1u << st);
+        const int64_t base = ((int64_t)blk * a.nkv + in.kvh) * PAGE * D;
+        const uint8_t* k = a.kv + base + g * D + t * 16;
+        const uint8_t* v = a.vv + base + 2 * t * D + g * 16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          cp_async16(dst + i * 512 + lane * 16, k + (i >> 1) * 8 * D + (i & 1) * 64);
+          cp_async16(dst + 2048 + i * 512 + lane * 16, v + ((i & 1) + 8 * (i >> 1)) * D);
+        }
+        if (lane < 8) {
+          const uint8_t* e = lane < 4 ? a.ke + blk * a.ke_sb + in.kvh * a.ke_sh + lane * 4
+                                      : a.ve + blk * a.ve_sb + in.kvh * a.ve_sh + (lane - 4) * 4;
+          cp_async4(dst + 4096 + lane * 4, e);
+        }
+      } else {
+        bad |= 1u << st;
+      }
+      ++in.p;
+    };
+#pragma unroll
+    for (int i = 0; i < kSt - 1; ++i) {
+      if (i < n_mine) fetch(i);
+      cp_async_commit();
+    }
+    HeadState<NT> st;
+    bool fresh = true;
+    int seg_p0 = use.p;  // the segment's first page
+    int L = 0;
+    int stage = 0;
+    for (int i = 0; i < n_mine; ++i) {
+      if (i + kSt - 1 < n_mine) fetch(stage == 0 ? kSt - 1 : stage - 1);
+      cp_async_commit();
+      if (fresh) {
+        st.begin(a.q + ((int64_t)use.b * a.nq + use.kvh * G) * D, G, a.scale_log2, lane);
+        L = min(a.kv_len[use.b], a.max_blocks * PAGE);
+        seg_p0 = use.p;
+        fresh = false;
+      }
+      cp_async_wait<kSt - 1>();
+      __syncwarp();
+      const uint8_t* src = smem + S::kRing + (warp * kSt + stage) * kStageBytes;
+      uint4 k[4], v[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        k[c] = *reinterpret_cast<const uint4*>(src + c * 512 + lane * 16);
+        v[c] = *reinterpret_cast<const uint4*>(src + 2048 + c * 512 + lane * 16);
+      }
+      const uint8_t* e = src + 4096;
+      const int ke[2] = {e[g], e[g + 8]}, ve[2] = {e[16 + g], e[24 + g]};
+      if (!((bad >> stage) & 1)) st.page(k, v, ke, ve, min(PAGE, L - use.p * PAGE), lane);
+      stage = stage + 1 == kSt ? 0 : stage + 1;
+      ++use.p;
+      const bool ends = use.p == use.pages;
+      if (!ends && i + 1 < n_mine) continue;
+      // ---- the segment is done
+      st.end();
+      const float vs = pow2(max(st.vr, -118) - 8);
+      if (seg_p0 == 0 && ends) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int head = n * 8 + 2 * t + c;
+            if (head >= G) continue;
+            const float inv = st.l[n][c] == 0.f ? 0.f : vs / st.l[n][c];
+            float f[16];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              f[2 * j] = st.o[n][j][c] * inv;
+              f[2 * j + 1] = st.o[n][j][2 + c] * inv;
+            }
+            __nv_bfloat16* dst = a.o + ((int64_t)use.b * a.nq + use.kvh * G + head) * D + g * 16;
+            *reinterpret_cast<uint4*>(dst) = pack_from<__nv_bfloat16>(f);
+            *reinterpret_cast<uint4*>(dst + 8) = pack_from<__nv_bfloat16>(f + 8);
+          }
+      } else {
+        // began earlier: slot 0; begins here and goes on (the warp's last
+        // segment, its ring is free): slot 1
+        const int slot = seg_p0 == 0 ? 1 : 0;
+        float* po = reinterpret_cast<float*>(slot == 0 ? smem + S::kSlot + warp * S::kSlotBytes
+                                                       : smem + S::kRing + warp * kSt * kStageBytes);
+        float2* ml = reinterpret_cast<float2*>(smem + S::kMl) + (slot * kWarps + warp) * S::kHeads;
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int head = n * 8 + 2 * t + c;
+            if (head >= G) continue;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<float2*>(po + head * kRow + g * 16 + 2 * j) =
+                  make_float2(st.o[n][j][c] * vs, st.o[n][j][2 + c] * vs);
+            if (g == 0) ml[head] = make_float2(st.m[n][c], st.l[n][c]);
+          }
+        if (lane == 0) {
+          SegMeta& sm = meta[slot][warp];
+          sm.valid = 1;
+          sm.ends = ends;
+          sm.b = use.b;
+          sm.kvh = use.kvh;
+          sm.begin = (int)(u0 + i + 1) - use.p;
+          sm.pages = use.pages;
+        }
+      }
+      if (ends && i + 1 < n_mine) next_pair(use);
+      fresh = true;
+    }
+  }
+  __syncthreads();
+
+  // ---- fold the warps' partials: chain a = -1 entered the CTA's run, chain a
+  // in 0..kWarps-1 begins in warp a's
+  const float2* ml = reinterpret_cast<const float2*>(smem + S::kMl);
+  auto piece = [&](int slot, int w, int head) {
+    const uint8_t* p = slot == 0 ? smem + S::kSlot + w * S::kSlotBytes : smem + S::kRing + w * kSt * kStageBytes;
+    return *reinterpret_cast<const float4*>(p + (head * kRow + lane * 4) * 4);
+  };
+  float2* part_ml = reinterpret_cast<float2*>(a.part + (int64_t)gridDim.x * 2 * S::kHeads * D);
+  const int span = kWarps * run;  // pages per CTA
+  int out_chain[2] = {-2, -2};    // chains that reach into other CTAs, by global slot (0: entered, 1: begins here)
+  for (int c = -1; c < kWarps; ++c) {
+    const SegMeta& sm = c < 0 ? meta[0][0] : meta[1][c];
+    if (!sm.valid) continue;
+    int last = c;  // the chain's last warp in this CTA
+    bool ended = false;
+    while (!ended && last + 1 < kWarps && meta[0][last + 1].valid) ended = meta[0][++last].ends;
+    const bool whole = c >= 0 && ended;
+    if (!whole) out_chain[c < 0 ? 0 : 1] = c;
+    for (int head = warp; head < G; head += kWarps) {
+      Fold f;
+      if (c >= 0) f.add(ml[(kWarps + c) * S::kHeads + head].x, ml[(kWarps + c) * S::kHeads + head].y, piece(1, c, head));
+      for (int w = c + 1; w <= last; ++w) {
+        const float2 x = ml[w * S::kHeads + head];
+        f.add(x.x, x.y, piece(0, w, head));
+      }
+      if (whole) {
+        f.store(a.o + ((int64_t)sm.b * a.nq + sm.kvh * G + head) * D, lane);
+      } else {
+        const int64_t at = ((int64_t)blockIdx.x * 2 + (c < 0 ? 0 : 1)) * S::kHeads + head;
+        *reinterpret_cast<float4*>(a.part + at * D + lane * 4) = f.o;
+        if (lane == 0) part_ml[at] = make_float2(f.m, f.l);
+      }
+    }
+  }
+  if (out_chain[0] == -2 && out_chain[1] == -2) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    int last = -1;
+    const int c = out_chain[threadIdx.x];
+    if (c != -2) {
+      const SegMeta& sm = c < 0 ? meta[0][0] : meta[1][c];
+      const int c0 = sm.begin / span, c1 = (sm.begin + sm.pages - 1) / span;
+      if (atomicAdd(a.counters + c0, 1) == c1 - c0) {
+        a.counters[c0] = 0;  // for the next launch
+        last = c0;
+      }
+    }
+    s_last[threadIdx.x] = last;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int slot = 0; slot < 2; ++slot) {
+    if (s_last[slot] < 0) continue;
+    __threadfence();
+    const SegMeta& sm = out_chain[slot] < 0 ? meta[0][0] : meta[1][out_chain[slot]];
+    const int c0 = s_last[slot], c1 = (sm.begin + sm.pages - 1) / span;
+    for (int head = warp; head < G; head += kWarps) {
+      Fold f;
+#pragma unroll 4
+      for (int c = c0; c <= c1; ++c) {
+        const int64_t at = ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * S::kHeads + head;
+        const float2 x = __ldcg(part_ml + at);
+        f.add(x.x, x.y, __ldcg(reinterpret_cast<const float4*>(a.part + at * D) + lane));
+      }
+      f.store(a.o + ((int64_t)sm.b * a.nq + sm.kvh * G + head) * D, lane);
+    }
+  }
 }
 
 }  // namespace
@@ -523,19 +846,34 @@ void read_pages_kv8_launch(const Kv8Cache& c, int nkv, const int* block_table, i
   MBX_CUDA_CHECK(cudaGetLastError());
 }
 
+int decode_kv8_grid(int B, int nkv, int max_blocks) {
+  int dev = 0, sms = 0;
+  MBX_CUDA_CHECK(cudaGetDevice(&dev));
+  MBX_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  const int64_t pages = (int64_t)B * nkv * max_blocks;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(sms, (pages + kWarps - 1) / kWarps));
+}
+
+size_t decode_kv8_part_floats(int grid) { return (size_t)grid * 2 * 16 * (D + 2); }
+
 void decode_attention_kv8_launch(const void* q, const Kv8Cache& c, void* o, const int* kv_len, const int* block_table,
-                                 int64_t bt_stride, int max_blocks, int B, int nq, int nkv, int splits, float* part_o,
-                                 float* part_lse, float scale, cudaStream_t s) {
+                                 int64_t bt_stride, int max_blocks, int B, int nq, int nkv, int grid, float* part,
+                                 int* counters, float scale, cudaStream_t s) {
   if (B == 0) return;
   if (nq % nkv != 0 || nq / nkv > 16) throw std::runtime_error("decode: group size must be <= 16");
   Kv8DecodeArgs a{static_cast<const __nv_bfloat16*>(q), c.kv, c.vv, c.ke, c.ve, c.ke_sb, c.ke_sh, c.ve_sb, c.ve_sh,
-                  static_cast<__nv_bfloat16*>(o), part_o, part_lse, kv_len, block_table, bt_stride, max_blocks,
-                  (int)c.blocks, nq, nkv, splits, scale * 1.4426950408889634f};
-  const dim3 grid(splits, nkv, B);
-  if (nq / nkv <= 8) launch_k(decode_kv8_kernel<1>, grid, dim3(32), 0, s, a);
-  else launch_k(decode_kv8_kernel<2>, grid, dim3(32), 0, s, a);
+                  static_cast<__nv_bfloat16*>(o), part, counters, kv_len, block_table, bt_stride, B, max_blocks,
+                  (int)c.blocks, nq, nkv, scale * 1.4426950408889634f};
+  if (nq / nkv <= 8) {
+    static SmemLimit limit;
+    limit.ensure((const void*)decode_kv8_kernel<1>, DecodeSmem<1>::kTotal);
+    launch_k(decode_kv8_kernel<1>, dim3(grid), dim3(kWarps * 32), DecodeSmem<1>::kTotal, s, a);
+  } else {
+    static SmemLimit limit;
+    limit.ensure((const void*)decode_kv8_kernel<2>, DecodeSmem<2>::kTotal);
+    launch_k(decode_kv8_kernel<2>, dim3(grid), dim3(kWarps * 32), DecodeSmem<2>::kTotal, s, a);
+  }
   MBX_CUDA_CHECK(cudaGetLastError());
-  attn_combine_launch(part_o, part_lse, (int64_t)B * nq, splits, o, s);
 }
 
 }  // namespace mbx

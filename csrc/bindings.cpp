@@ -8,6 +8,9 @@
 #include <algorithm>
 #include <cstring>
 #include <initializer_list>
+#include <map>
+#include <mutex>
+#include <tuple>
 #include <utility>
 
 #include "kernels.h"
@@ -646,13 +649,45 @@ void read_pages_kv8(torch::Tensor kv, torch::Tensor ke, torch::Tensor vv, torch:
                         cur_stream());
 }
 
-void decode_attention_kv8(torch::Tensor q, torch::Tensor kv, torch::Tensor ke, torch::Tensor vv, torch::Tensor ve,
-                          torch::Tensor out, torch::Tensor kv_len, torch::Tensor block_table, double scale,
-                          int64_t splits, torch::Tensor part_o, torch::Tensor part_lse) {
+// Scratch of decode_attention_kv8: partial results, and arrival counters that
+// every launch finds and leaves at zero. One per stream, since launches on
+// different streams may run at the same time, and one per graph capture, whose
+// replays may run at the same time as anything else: its counters are zeroed
+// by a node at the head of the graph, and its memory is the graph's own.
+struct DecodeKv8Ws {
+  torch::Tensor part, counters;
+  unsigned long long capture = 0;
+};
+DecodeKv8Ws decode_kv8_ws(const torch::Tensor& q, cudaStream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const cudaError_t err = cudaStreamGetCaptureInfo(stream, &status, &id);
+  TORCH_CHECK(err == cudaSuccess, "cudaStreamGetCaptureInfo: ", cudaGetErrorString(err));
+  const bool capturing = status == cudaStreamCaptureStatusActive;
+  // never destroyed: the process may end after the CUDA context
+  static auto* mu = new std::mutex;
+  static auto* all = new std::map<std::tuple<int, cudaStream_t, bool>, DecodeKv8Ws>;
+  std::lock_guard<std::mutex> lock(*mu);
+  DecodeKv8Ws& ws = (*all)[{q.device().index(), stream, capturing}];
+  if (!ws.part.defined() || (capturing && ws.capture != id)) {
+    const int grid = decode_kv8_grid(1 << 15, 1, 1 << 15);  // the largest
+    const auto opt = torch::TensorOptions().device(q.device());
+    ws.part = torch::empty({(int64_t)decode_kv8_part_floats(grid)}, opt.dtype(torch::kFloat32));
+    ws.counters = torch::zeros({grid}, opt.dtype(torch::kInt32));
+    ws.capture = id;
+  }
+  return ws;
+}
+
+torch::Tensor decode_attention_kv8(torch::Tensor q, torch::Tensor kv, torch::Tensor ke, torch::Tensor vv,
+                                   torch::Tensor ve, c10::optional<torch::Tensor> out_opt, torch::Tensor kv_len,
+                                   torch::Tensor block_table, double scale) {
   check_dense(q, "q", torch::kBFloat16);
   TORCH_CHECK(q.dim() == 3 && q.size(2) == 128, "q must be [B, nq, 128]");
-  check_dense(out, "out", torch::kBFloat16);
-  TORCH_CHECK(out.sizes() == q.sizes(), "out must have q's shape");
+  if (out_opt.has_value()) {
+    check_dense(*out_opt, "out", torch::kBFloat16);
+    TORCH_CHECK(out_opt->sizes() == q.sizes(), "out must have q's shape");
+  }
   check_pages8(kv, ke, "k_cache");
   const int64_t B = q.size(0), nq = q.size(1), nkv = kv.size(1);
   const Kv8Cache c = kv8_cache(kv, ke, vv, ve, nkv);
@@ -660,16 +695,19 @@ void decode_attention_kv8(torch::Tensor q, torch::Tensor kv, torch::Tensor ke, t
   check_lens(kv_len);
   TORCH_CHECK(kv_len.numel() == B, "kv_len must be int32 [B]");
   check_table(block_table, "block_table", B);
-  TORCH_CHECK(B * nkv * std::max<int64_t>(1, block_table.size(1)) < (int64_t)1 << 31, "decode: too many pages");
+  TORCH_CHECK(B * nkv * std::max<int64_t>(1, block_table.size(1)) < (int64_t)1 << 30, "decode: too many pages");
   check_devices({{"q", &q}, {"k_cache", &kv}, {"k_cache exps", &ke}, {"v_cache", &vv}, {"v_cache exps", &ve},
-                 {"out", &out}, {"kv_len", &kv_len}, {"block_table", &block_table}, {"scratch", &part_o},
-                 {"scratch", &part_lse}});
-  TORCH_CHECK(part_o.numel() >= B * nq * splits * 128 && part_lse.numel() >= B * nq * splits,
-              "decode: scratch too small");
+                 {"out", out_opt ? &*out_opt : nullptr}, {"kv_len", &kv_len}, {"block_table", &block_table}});
   const at::cuda::CUDAGuard guard(q.device());
+  torch::Tensor out = out_opt ? *out_opt : torch::empty_like(q);
+  if (B == 0) return out;
+  const cudaStream_t stream = cur_stream();
+  const DecodeKv8Ws ws = decode_kv8_ws(q, stream);
   decode_attention_kv8_launch(q.data_ptr(), c, out.data_ptr(), kv_len.data_ptr<int>(), block_table.data_ptr<int>(),
-                              block_table.stride(0), (int)block_table.size(1), (int)B, (int)nq, (int)nkv, (int)splits,
-                              part_o.data_ptr<float>(), part_lse.data_ptr<float>(), (float)scale, cur_stream());
+                              block_table.stride(0), (int)block_table.size(1), (int)B, (int)nq, (int)nkv,
+                              decode_kv8_grid((int)B, (int)nkv, (int)block_table.size(1)), ws.part.data_ptr<float>(),
+                              ws.counters.data_ptr<int>(), (float)scale, stream);
+  return out;
 }
 
 }  // namespace

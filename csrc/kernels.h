@@ -208,9 +208,14 @@ void read_pages_kv8_launch(const Kv8Cache& c, int nkv, const int* block_table, i
                            int64_t ot_stride, const int* kv_len, int R, int max_blocks, void* k_out, void* v_out,
                            int64_t out_pages, cudaStream_t s);
 // decode_attention_launch over the 8-bit cache; lengths are clamped to
-// max_blocks pages, keys of blocks outside the cache do not count.
+// max_blocks pages, keys of blocks outside the cache do not count. `grid` from
+// decode_kv8_grid (for the current device); part holds
+// decode_kv8_part_floats(grid) floats, counters grid zeros, which the launch
+// leaves zero. Launches that may run at the same time need their own.
+int decode_kv8_grid(int B, int nkv, int max_blocks);
+size_t decode_kv8_part_floats(int grid);
 void decode_attention_kv8_launch(const void* q, const Kv8Cache& c, void* o, const int* kv_len, const int* block_table,
-                                 int64_t bt_stride, int max_blocks, int B, int nq, int nkv, int splits, float* part_o,
-                                 float* part_lse, float scale, cudaStream_t s);
+                                 int64_t bt_stride, int max_blocks, int B, int nq, int nkv, int grid, float* part,
+                                 int* counters, float scale, cudaStream_t s);
 
 }  // namespace mbx
