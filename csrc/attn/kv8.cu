@@ -259,7 +259,8 @@ struct Kv8DecodeArgs {
   const uint8_t *kv, *vv, *ke, *ve;
   int64_t ke_sb, ke_sh, ve_sb, ve_sh;
   __nv_bfloat16* o;        // [B, nq, D]
-  float* part;             // partial results of segments that span CTAs [grid][2][heads][D], then their (m, l)
+  float* part;             // partials of pairs that span CTAs [grid][2][heads][D], their (m, l), partials that wait
+                           // for the CTA's merge [grid][warps][heads][kRow]
   int* counters;           // [grid] arrivals, zero between launches
   const int* kv_len;       // [B]
   const int* block_table;  // [B, max_blocks], row stride bt_s
@@ -269,6 +270,19 @@ struct Kv8DecodeArgs {
 };
 
 constexpr int kNoExp = -1000;  // value exponent of a masked key, and vr before the first page
+
+// Where a fetched page's 16-byte chunks lie in shared memory. The reader of a
+// K chunk (row r, chunk c) is lane (g, t) = (r % 8, c % 4), of a V chunk lane
+// (c, r % 8 / 2), one of its four chunks each; the exclusive ors spread the
+// writes (8 chunks of a row at once) and the reads over all banks.
+MBX_DEVICE uint32_t k_place(int row, int ch) {
+  const int slot = (row >> 3) * 2 + (ch >> 2);
+  return slot * 512 + ((((row & 7) * 4 + (ch & 3)) ^ ((ch >> 2) << 2)) << 4);
+}
+MBX_DEVICE uint32_t v_place(int row, int ch) {
+  const int slot = (row >> 3) * 2 + (row & 1), t = (row & 7) >> 1;
+  return slot * 512 + ((t * 8 + (ch ^ (2 * t))) << 4);
+}
 
 // One warp's running state over the pages of one (request, kv head); NT tiles
 // of 8 query heads. Of tile n, lane (g, t) holds heads 8n + 2t and 8n + 2t + 1
@@ -325,45 +339,59 @@ struct HeadState {
     }
   }
 
-  // k[0..1]: row g, chunks t and t + 4; k[2..3]: row g + 8. v[i]: chunk g of
-  // keys 2t, 2t + 1, 2t + 8, 2t + 9. ke, ve: exponent bytes of keys g, g + 8.
-  // Only the page's first `live` keys count.
-  MBX_DEVICE void page(const uint4 (&k)[4], uint4 (&v)[4], const int (&ke)[2], const int (&ve)[2], int live,
-                       int lane) {
+  // P pages at once (independent chains of tensor-core work), as fetched into
+  // shared memory: K (k_place), V (v_place), then the exponents of the 16 keys
+  // and of the 16 values. A lane takes K rows g and g + 8, chunks t and t + 4,
+  // and chunk g of V's rows 2t, 2t + 1, 2t + 8, 2t + 9. Only a page's first
+  // live[p] keys count.
+  template <int P>
+  MBX_DEVICE void pages(const uint8_t* const (&src)[2], const int (&live)[2], int lane) {
     const int g = lane >> 2, t = lane & 3;
-    float s[NT][4];
+    float s[P][NT][4];
+    uint4 k[P][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-    const uint32_t kw[4][4] = {{k[0].x, k[0].y, k[0].z, k[0].w},
-                               {k[1].x, k[1].y, k[1].z, k[1].w},
-                               {k[2].x, k[2].y, k[2].z, k[2].w},
-                               {k[3].x, k[3].y, k[3].z, k[3].w}};
+    for (int p = 0; p < P; ++p)
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-      const uint32_t r0 = kw[ks >> 2][ks & 3], r8 = kw[2 + (ks >> 2)][ks & 3];
-      const uint32_t af[4] = {f16x2_of(r0, 0), f16x2_of(r8, 0), f16x2_of(r0, 1), f16x2_of(r8, 1)};
+      for (int c = 0; c < 4; ++c) k[p][c] = *reinterpret_cast<const uint4*>(src[p] + k_place(g + 8 * (c >> 1), t + 4 * (c & 1)));
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_f16(s[n], af, qf[n][ks][0], qf[n][ks][1]);
-    }
-    const bool on[2] = {g < live, g + 8 < live};
-    int vx[2];
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[p][n][0] = s[p][n][1] = s[p][n][2] = s[p][n][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const uint4 &w0 = k[p][ks >> 2], &w8 = k[p][2 + (ks >> 2)];
+        const uint32_t r0 = (ks & 3) == 0 ? w0.x : (ks & 3) == 1 ? w0.y : (ks & 3) == 2 ? w0.z : w0.w;
+        const uint32_t r8 = (ks & 3) == 0 ? w8.x : (ks & 3) == 1 ? w8.y : (ks & 3) == 2 ? w8.z : w8.w;
+        const uint32_t af[4] = {f16x2_of(r0, 0), f16x2_of(r8, 0), f16x2_of(r0, 1), f16x2_of(r8, 1)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16(s[p][n], af, qf[n][ks][0], qf[n][ks][1]);
+      }
+    int vx[P][2];
     bool grow = false;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      vx[r] = on[r] ? ve[r] - 127 : kNoExp;
-      grow |= vx[r] > vr + 3;
-      const float kf = __uint_as_float((uint32_t)ke[r] << 23);
+    for (int p = 0; p < P; ++p)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int r = 0; r < 2; ++r) {
+        const uint8_t* e = src[p] + 4096 + g + 8 * r;
+        const bool on = g + 8 * r < live[p];
+        vx[p][r] = on ? (int)e[16] - 127 : kNoExp;
+        grow |= vx[p][r] > vr + 3;
+        const float kf = __uint_as_float((uint32_t)e[0] << 23);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float x = on[r] ? s[n][2 * r + c] * (kf * qs[n][c]) : -INFINITY;
-          s[n][2 * r + c] = x;
-          grow |= x > m[n][c] + 4.f;
-        }
-    }
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float x = on ? s[p][n][2 * r + c] * (kf * qs[n][c]) : -INFINITY;
+            s[p][n][2 * r + c] = x;
+            grow |= x > m[n][c] + 4.f;
+          }
+      }
     if (__any_sync(0xffffffffu, grow)) {
-      int nv = max(vr, max(vx[0], vx[1]));
+      int nv = vr;
+#pragma unroll
+      for (int p = 0; p < P; ++p) nv = max(nv, max(vx[p][0], vx[p][1]));
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) nv = max(nv, __shfl_xor_sync(0xffffffffu, nv, off));
       const float vc = ex2((float)(vr - nv));
@@ -373,7 +401,9 @@ struct HeadState {
         float corr[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float nm = fmaxf(m[n][c], fmaxf(s[n][c], s[n][2 + c]));
+          float nm = m[n][c];
+#pragma unroll
+          for (int p = 0; p < P; ++p) nm = fmaxf(nm, fmaxf(s[p][n][c], s[p][n][2 + c]));
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, off));
           corr[c] = nm == -INFINITY ? 1.f : ex2(m[n][c] - nm);
@@ -389,38 +419,47 @@ struct HeadState {
         }
       }
     }
-    uint32_t pf[NT][2];
-    const float vf[2] = {pow2(max(vx[0] - vr + 8, -126)), pow2(max(vx[1] - vr + 8, -126))};
+    uint32_t pf[P][NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float w[2];
+        const float vf = pow2(max(vx[p][r] - vr + 8, -126));
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float p = ex2(s[n][2 * r + c] - (m[n][c] == -INFINITY ? 0.f : m[n][c]));
-          l[n][c] += p;
-          w[c] = p * vf[r];
+        for (int n = 0; n < NT; ++n) {
+          float w[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float x = ex2(s[p][n][2 * r + c] - (m[n][c] == -INFINITY ? 0.f : m[n][c]));
+            l[n][c] += x;
+            w[c] = x * vf;
+          }
+          pf[p][n][r] = transpose8x8(pack_f16(w[0], w[1]));
         }
-        pf[n][r] = transpose8x8(pack_f16(w[0], w[1]));
       }
-    if (live < PAGE) {  // rows behind the length may hold anything: 0 * NaN would not be 0
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (2 * t + (i & 1) + 8 * (i >> 1) >= live) v[i] = make_uint4(0, 0, 0, 0);
-    }
-    const uint32_t vw[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w},
-                               {v[1].x, v[1].y, v[1].z, v[1].w},
-                               {v[2].x, v[2].y, v[2].z, v[2].w},
-                               {v[3].x, v[3].y, v[3].z, v[3].w}};
+    for (int p = 0; p < P; ++p) {
+      uint4 v[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
-      const uint32_t a01 = __byte_perm(vw[0][i >> 1], vw[1][i >> 1], sel);
-      const uint32_t a89 = __byte_perm(vw[2][i >> 1], vw[3][i >> 1], sel);
-      const uint32_t af[4] = {f16x2_of(a01, 0), f16x2_of(a01, 1), f16x2_of(a89, 0), f16x2_of(a89, 1)};
+      for (int c = 0; c < 4; ++c) v[c] = *reinterpret_cast<const uint4*>(src[p] + 2048 + v_place(2 * t + (c & 1) + 8 * (c >> 1), g));
+      if (live[p] < PAGE) {  // rows behind the length may hold anything: 0 * NaN would not be 0
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_f16(o[n][i], af, pf[n][0], pf[n][1]);
+        for (int i = 0; i < 4; ++i)
+          if (2 * t + (i & 1) + 8 * (i >> 1) >= live[p]) v[i] = make_uint4(0, 0, 0, 0);
+      }
+      const uint32_t vw[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w},
+                                 {v[1].x, v[1].y, v[1].z, v[1].w},
+                                 {v[2].x, v[2].y, v[2].z, v[2].w},
+                                 {v[3].x, v[3].y, v[3].z, v[3].w}};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
+        const uint32_t a01 = __byte_perm(vw[0][i >> 1], vw[1][i >> 1], sel);
+        const uint32_t a89 = __byte_perm(vw[2][i >> 1], vw[3][i >> 1], sel);
+        const uint32_t af[4] = {f16x2_of(a01, 0), f16x2_of(a01, 1), f16x2_of(a89, 0), f16x2_of(a89, 1)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16(o[n][i], af, pf[p][n][0], pf[p][n][1]);
+      }
     }
   }
 
@@ -446,22 +485,21 @@ struct HeadState {
 //     last of those CTAs to arrive folds these in CTA order.
 // All orders are fixed, so results do not depend on timing. At most one pair
 // enters a CTA's run and one leaves it, hence two global partials per CTA.
-constexpr int kWarps = 8;
+template <int NT>
+constexpr int kWarps = NT == 1 ? 16 : 8;
 constexpr int kStageBytes = 2 * PAGE * D + 64;  // K, V, 2 x 16 exponents
 constexpr int kRow = D + 4;                     // floats per head of a partial in shared memory (bank spread)
 
 template <int NT>
-constexpr int kStages = NT == 1 ? 5 : 4;
+constexpr int kStages = NT == 1 ? 3 : 6;
 
 template <int NT>
 struct DecodeSmem {
   static constexpr int kHeads = 8 * NT;
-  static constexpr int kRing = 0;
-  static constexpr int kSlot = kWarps * kStages<NT> * kStageBytes;        // [kWarps] partials: kHeads x kRow floats
-  static constexpr int kSlotBytes = kHeads * kRow * 4;
-  static constexpr int kMl = kSlot + kWarps * kSlotBytes;                 // float2 [2][kWarps][kHeads]
-  static constexpr int kTotal = kMl + 2 * kWarps * kHeads * 8;
-  static_assert(kStages<NT> * kStageBytes >= kSlotBytes, "the second partial of a warp lies in its ring");
+  static constexpr int kWarpBytes = kStages<NT> * kStageBytes;  // a warp's ring, then its last segment's partial
+  static constexpr int kMl = kWarps<NT> * kWarpBytes;           // float2 [2][kWarps][kHeads]
+  static constexpr int kTotal = kMl + 2 * kWarps<NT> * kHeads * 8;
+  static_assert(kWarpBytes >= kHeads * kRow * 4, "a partial fits in the ring");
 };
 
 MBX_DEVICE uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -482,6 +520,7 @@ MBX_DEVICE void cp_async_wait() {
 struct SegMeta {
   int valid;   // there is a partial
   int ends;    // first segment only: the pair's pages end in this warp's run
+  int far;     // first segment only: its state is in global memory
   int b, kvh;
   int begin;   // list index of the pair's first page
   int pages;
@@ -512,6 +551,7 @@ struct Fold {
   }
 };
 
+template <int W>
 MBX_DEVICE int block_sum(int v, int* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -520,34 +560,38 @@ MBX_DEVICE int block_sum(int v, int* red) {
   __syncthreads();
   int s = 0;
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) s += red[i];
+  for (int i = 0; i < W; ++i) s += red[i];
   return s;
 }
 
 template <int NT>
-__global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArgs a) {
+__global__ void __launch_bounds__(kWarps<NT> * 32, 1) decode_kv8_kernel(Kv8DecodeArgs a) {
   using S = DecodeSmem<NT>;
-  constexpr int kSt = kStages<NT>;
+  constexpr int kSt = kStages<NT>, kW = kWarps<NT>;
   pdl_wait();
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int red[kWarps];
-  __shared__ int start_b[kWarps], start_off[kWarps];
-  __shared__ SegMeta meta[2][kWarps];
+  __shared__ int red[kW];
+  __shared__ int start_b[kW], start_off[kW];
+  __shared__ SegMeta meta[2][kW];
   __shared__ int s_last[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = a.nq / a.nkv;
   auto pages_of = [&](int b) {
     return (min(max(a.kv_len[b], 0), a.max_blocks * PAGE) + PAGE - 1) / PAGE;
   };
+  // partials that wait for the CTA's merge while their warp works on
+  auto near_part = [&](int w) {
+    return a.part + (int64_t)gridDim.x * 2 * S::kHeads * (D + 2) + ((int64_t)blockIdx.x * kW + w) * S::kHeads * kRow;
+  };
   // ---- this warp's run [u0, u1) of the page list, and where it starts
-  if (threadIdx.x < 2 * kWarps) meta[threadIdx.x / kWarps][threadIdx.x % kWarps].valid = 0;
+  if (threadIdx.x < 2 * kW) meta[threadIdx.x / kW][threadIdx.x % kW].valid = 0;
   const int first = (int)threadIdx.x < a.B ? pages_of(threadIdx.x) : 0;
   int sum = first;
   for (int b = threadIdx.x + blockDim.x; b < a.B; b += blockDim.x) sum += pages_of(b);
-  const int total = block_sum(sum, red) * a.nkv;
-  const int n_warps = gridDim.x * kWarps;
+  const int total = block_sum<kW>(sum, red) * a.nkv;
+  const int n_warps = gridDim.x * kW;
   const int run = max(1, (total + n_warps - 1) / n_warps);
-  const int cta_u0 = blockIdx.x * kWarps * run;
+  const int cta_u0 = blockIdx.x * kW * run;
   for (int b0 = 0, carry = 0; b0 < a.B; b0 += blockDim.x) {
     const int b = b0 + threadIdx.x;
     const int n = b0 == 0 ? first : (b < a.B ? pages_of(b) : 0);
@@ -562,13 +606,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
     __syncthreads();
     int before = carry;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
+    for (int i = 0; i < kW; ++i) {
       if (i < warp) before += red[i];
       carry += red[i];
     }
     const int64_t lo = (int64_t)(before + inc - n) * a.nkv, hi = lo + (int64_t)n * a.nkv;
-    if (n > 0 && lo < (int64_t)cta_u0 + kWarps * run && hi > cta_u0)
-      for (int w = 0; w < kWarps; ++w) {
+    if (n > 0 && lo < (int64_t)cta_u0 + kW * run && hi > cta_u0)
+      for (int w = 0; w < kW; ++w) {
         const int64_t u = (int64_t)cta_u0 + w * run;
         if (u >= lo && u < hi) {
           start_b[w] = b;
@@ -585,7 +629,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
 
   const int64_t u0 = (int64_t)cta_u0 + warp * run;
   const int n_mine = u0 >= total ? 0 : (int)min((int64_t)run, total - u0);
-  const uint32_t ring = smem_addr(smem + S::kRing) + warp * kSt * kStageBytes;
+  const uint32_t ring = smem_addr(smem) + warp * S::kWarpBytes;
   if (n_mine > 0) {
     // cursors into the list: the pages being fetched and the ones being used
     struct Cursor {
@@ -606,6 +650,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
         c.pages = pages_of(c.b);
       } while (c.pages == 0);
     };
+    // Each copy instruction reads 512 contiguous bytes (four rows, lane l the
+    // l-th 16) and places them where pages() reads them.
+    uint32_t k_dst[2], v_dst[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = i * 4 + (lane >> 3), ch = lane & 7;
+      k_dst[i] = k_place(row, ch);
+      v_dst[i] = 2048 + v_place(row, ch);
+    }
     int win = -1;       // first page of the table window that the lanes hold
     int id = -1;
     uint32_t bad = 0;   // stages whose page is not in the cache
@@ -623,12 +676,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
       if (blk >= 0 && blk < a.num_blocks) {
         bad &= ~(1u << st);
         const int64_t base = ((int64_t)blk * a.nkv + in.kvh) * PAGE * D;
-        const uint8_t* k = a.kv + base + g * D + t * 16;
-        const uint8_t* v = a.vv + base + 2 * t * D + g * 16;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          cp_async16(dst + i * 512 + lane * 16, k + (i >> 1) * 8 * D + (i & 1) * 64);
-          cp_async16(dst + 2048 + i * 512 + lane * 16, v + ((i & 1) + 8 * (i >> 1)) * D);
+          cp_async16(dst + k_dst[i & 1] + (i >> 1) * 1024, a.kv + base + i * 512 + lane * 16);
+          cp_async16(dst + v_dst[i & 1] + (i >> 1) * 1024, a.vv + base + i * 512 + lane * 16);
         }
         if (lane < 8) {
           const uint8_t* e = lane < 4 ? a.ke + blk * a.ke_sb + in.kvh * a.ke_sh + lane * 4
@@ -640,8 +691,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
       }
       ++in.p;
     };
+    // groups 0..kSt-1: the first pages; then one group per page used, in order
 #pragma unroll
-    for (int i = 0; i < kSt - 1; ++i) {
+    for (int i = 0; i < kSt; ++i) {
       if (i < n_mine) fetch(i);
       cp_async_commit();
     }
@@ -650,31 +702,36 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
     int seg_p0 = use.p;  // the segment's first page
     int L = 0;
     int stage = 0;
-    for (int i = 0; i < n_mine; ++i) {
-      if (i + kSt - 1 < n_mine) fetch(stage == 0 ? kSt - 1 : stage - 1);
-      cp_async_commit();
+    for (int i = 0; i < n_mine;) {
       if (fresh) {
         st.begin(a.q + ((int64_t)use.b * a.nq + use.kvh * G) * D, G, a.scale_log2, lane);
         L = min(a.kv_len[use.b], a.max_blocks * PAGE);
         seg_p0 = use.p;
         fresh = false;
       }
-      cp_async_wait<kSt - 1>();
+      cp_async_wait<kSt - 2>();
       __syncwarp();
-      const uint8_t* src = smem + S::kRing + (warp * kSt + stage) * kStageBytes;
-      uint4 k[4], v[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        k[c] = *reinterpret_cast<const uint4*>(src + c * 512 + lane * 16);
-        v[c] = *reinterpret_cast<const uint4*>(src + 2048 + c * 512 + lane * 16);
+      const int stage1 = stage + 1 == kSt ? 0 : stage + 1;
+      const uint8_t* const src[2] = {smem + warp * S::kWarpBytes + stage * kStageBytes,
+                                     smem + warp * S::kWarpBytes + stage1 * kStageBytes};
+      const bool two = i + 1 < n_mine && use.p + 1 < use.pages;
+      const int live[2] = {(bad >> stage) & 1 ? 0 : min(PAGE, L - use.p * PAGE),
+                           (bad >> stage1) & 1 ? 0 : min(PAGE, L - use.p * PAGE - PAGE)};
+      if (two) st.template pages<2>(src, live, lane);
+      else st.template pages<1>(src, live, lane);
+      __syncwarp();
+      if (i + kSt < n_mine) fetch(stage);
+      cp_async_commit();
+      if (two) {
+        if (i + 1 + kSt < n_mine) fetch(stage1);
+        cp_async_commit();
       }
-      const uint8_t* e = src + 4096;
-      const int ke[2] = {e[g], e[g + 8]}, ve[2] = {e[16 + g], e[24 + g]};
-      if (!((bad >> stage) & 1)) st.page(k, v, ke, ve, min(PAGE, L - use.p * PAGE), lane);
-      stage = stage + 1 == kSt ? 0 : stage + 1;
-      ++use.p;
+      const int used = two ? 2 : 1;
+      stage = two ? (stage1 + 1 == kSt ? 0 : stage1 + 1) : stage1;
+      i += used;
+      use.p += used;
       const bool ends = use.p == use.pages;
-      if (!ends && i + 1 < n_mine) continue;
+      if (!ends && i < n_mine) continue;
       // ---- the segment is done
       st.end();
       const float vs = pow2(max(st.vr, -118) - 8);
@@ -697,12 +754,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
             *reinterpret_cast<uint4*>(dst + 8) = pack_from<__nv_bfloat16>(f + 8);
           }
       } else {
-        // began earlier: slot 0; begins here and goes on (the warp's last
-        // segment, its ring is free): slot 1
+        // began earlier: slot 0; begins here and goes on: slot 1. The run's last
+        // segment leaves its state in the ring, an earlier one in global memory.
         const int slot = seg_p0 == 0 ? 1 : 0;
-        float* po = reinterpret_cast<float*>(slot == 0 ? smem + S::kSlot + warp * S::kSlotBytes
-                                                       : smem + S::kRing + warp * kSt * kStageBytes);
-        float2* ml = reinterpret_cast<float2*>(smem + S::kMl) + (slot * kWarps + warp) * S::kHeads;
+        const bool far = i < n_mine;
+        float* po = far ? near_part(warp) : reinterpret_cast<float*>(smem + warp * S::kWarpBytes);
+        float2* ml = reinterpret_cast<float2*>(smem + S::kMl) + (slot * kW + warp) * S::kHeads;
         __syncwarp();
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -720,42 +777,43 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
           SegMeta& sm = meta[slot][warp];
           sm.valid = 1;
           sm.ends = ends;
+          sm.far = far;
           sm.b = use.b;
           sm.kvh = use.kvh;
-          sm.begin = (int)(u0 + i + 1) - use.p;
+          sm.begin = (int)(u0 + i) - use.p;
           sm.pages = use.pages;
         }
       }
-      if (ends && i + 1 < n_mine) next_pair(use);
+      if (ends && i < n_mine) next_pair(use);
       fresh = true;
     }
   }
   __syncthreads();
 
   // ---- fold the warps' partials: chain a = -1 entered the CTA's run, chain a
-  // in 0..kWarps-1 begins in warp a's
+  // in 0..kW-1 begins in warp a's
   const float2* ml = reinterpret_cast<const float2*>(smem + S::kMl);
-  auto piece = [&](int slot, int w, int head) {
-    const uint8_t* p = slot == 0 ? smem + S::kSlot + w * S::kSlotBytes : smem + S::kRing + w * kSt * kStageBytes;
-    return *reinterpret_cast<const float4*>(p + (head * kRow + lane * 4) * 4);
+  auto piece = [&](bool far, int w, int head) {
+    const float* p = far ? near_part(w) : reinterpret_cast<const float*>(smem + w * S::kWarpBytes);
+    return *reinterpret_cast<const float4*>(p + head * kRow + lane * 4);
   };
   float2* part_ml = reinterpret_cast<float2*>(a.part + (int64_t)gridDim.x * 2 * S::kHeads * D);
-  const int span = kWarps * run;  // pages per CTA
+  const int span = kW * run;  // pages per CTA
   int out_chain[2] = {-2, -2};    // chains that reach into other CTAs, by global slot (0: entered, 1: begins here)
-  for (int c = -1; c < kWarps; ++c) {
+  for (int c = -1; c < kW; ++c) {
     const SegMeta& sm = c < 0 ? meta[0][0] : meta[1][c];
     if (!sm.valid) continue;
     int last = c;  // the chain's last warp in this CTA
     bool ended = false;
-    while (!ended && last + 1 < kWarps && meta[0][last + 1].valid) ended = meta[0][++last].ends;
+    while (!ended && last + 1 < kW && meta[0][last + 1].valid) ended = meta[0][++last].ends;
     const bool whole = c >= 0 && ended;
     if (!whole) out_chain[c < 0 ? 0 : 1] = c;
-    for (int head = warp; head < G; head += kWarps) {
+    for (int head = warp; head < G; head += kW) {
       Fold f;
-      if (c >= 0) f.add(ml[(kWarps + c) * S::kHeads + head].x, ml[(kWarps + c) * S::kHeads + head].y, piece(1, c, head));
+      if (c >= 0) f.add(ml[(kW + c) * S::kHeads + head].x, ml[(kW + c) * S::kHeads + head].y, piece(false, c, head));
       for (int w = c + 1; w <= last; ++w) {
         const float2 x = ml[w * S::kHeads + head];
-        f.add(x.x, x.y, piece(0, w, head));
+        f.add(x.x, x.y, piece(meta[0][w].far, w, head));
       }
       if (whole) {
         f.store(a.o + ((int64_t)sm.b * a.nq + sm.kvh * G + head) * D, lane);
@@ -789,7 +847,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
     __threadfence();
     const SegMeta& sm = out_chain[slot] < 0 ? meta[0][0] : meta[1][out_chain[slot]];
     const int c0 = s_last[slot], c1 = (sm.begin + sm.pages - 1) / span;
-    for (int head = warp; head < G; head += kWarps) {
+    for (int head = warp; head < G; head += kW) {
       Fold f;
 #pragma unroll 4
       for (int c = c0; c <= c1; ++c) {
@@ -851,10 +909,13 @@ int decode_kv8_grid(int B, int nkv, int max_blocks) {
   MBX_CUDA_CHECK(cudaGetDevice(&dev));
   MBX_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   const int64_t pages = (int64_t)B * nkv * max_blocks;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(sms, (pages + kWarps - 1) / kWarps));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(sms, (pages + kWarps<2> - 1) / kWarps<2>));
 }
 
-size_t decode_kv8_part_floats(int grid) { return (size_t)grid * 2 * 16 * (D + 2); }
+size_t decode_kv8_part_floats(int grid) {
+  static_assert(kWarps<1> * 8 == kWarps<2> * 16, "both forms keep as many heads per CTA");
+  return (size_t)grid * (2 * 16 * (D + 2) + kWarps<1> * 8 * kRow);
+}
 
 void decode_attention_kv8_launch(const void* q, const Kv8Cache& c, void* o, const int* kv_len, const int* block_table,
                                  int64_t bt_stride, int max_blocks, int B, int nq, int nkv, int grid, float* part,
@@ -867,11 +928,11 @@ void decode_attention_kv8_launch(const void* q, const Kv8Cache& c, void* o, cons
   if (nq / nkv <= 8) {
     static SmemLimit limit;
     limit.ensure((const void*)decode_kv8_kernel<1>, DecodeSmem<1>::kTotal);
-    launch_k(decode_kv8_kernel<1>, dim3(grid), dim3(kWarps * 32), DecodeSmem<1>::kTotal, s, a);
+    launch_k(decode_kv8_kernel<1>, dim3(grid), dim3(kWarps<1> * 32), DecodeSmem<1>::kTotal, s, a);
   } else {
     static SmemLimit limit;
     limit.ensure((const void*)decode_kv8_kernel<2>, DecodeSmem<2>::kTotal);
-    launch_k(decode_kv8_kernel<2>, dim3(grid), dim3(kWarps * 32), DecodeSmem<2>::kTotal, s, a);
+    launch_k(decode_kv8_kernel<2>, dim3(grid), dim3(kWarps<2> * 32), DecodeSmem<2>::kTotal, s, a);
   }
   MBX_CUDA_CHECK(cudaGetLastError());
 }
