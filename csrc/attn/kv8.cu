@@ -259,8 +259,7 @@ struct Kv8DecodeArgs {
   const uint8_t *kv, *vv, *ke, *ve;
   int64_t ke_sb, ke_sh, ve_sb, ve_sh;
   __nv_bfloat16* o;        // [B, nq, D]
-  float* part;             // partials of pairs that span CTAs [grid][2][heads][D], their (m, l), partials that wait
-                           // for the CTA's merge [grid][warps][heads][kRow]
+  float* part;             // partials of pairs that span CTAs [grid][2][heads][D], then their (m, l)
   int* counters;           // [grid] arrivals, zero between launches
   const int* kv_len;       // [B]
   const int* block_table;  // [B, max_blocks], row stride bt_s
@@ -347,7 +346,7 @@ struct HeadState {
   template <int P>
   MBX_DEVICE void pages(const uint8_t* const (&src)[2], const int (&live)[2], int lane) {
     const int g = lane >> 2, t = lane & 3;
-    float s[P][NT][4];
+    float s[P][NT][4], s2[P][NT][4];  // halves of the sum: a shorter chain
     uint4 k[P][4];
 #pragma unroll
     for (int p = 0; p < P; ++p)
@@ -356,7 +355,9 @@ struct HeadState {
 #pragma unroll
     for (int p = 0; p < P; ++p)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[p][n][0] = s[p][n][1] = s[p][n][2] = s[p][n][3] = 0.f;
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[p][n][i] = s2[p][n][i] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
@@ -366,7 +367,7 @@ struct HeadState {
         const uint32_t r8 = (ks & 3) == 0 ? w8.x : (ks & 3) == 1 ? w8.y : (ks & 3) == 2 ? w8.z : w8.w;
         const uint32_t af[4] = {f16x2_of(r0, 0), f16x2_of(r8, 0), f16x2_of(r0, 1), f16x2_of(r8, 1)};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16(s[p][n], af, qf[n][ks][0], qf[n][ks][1]);
+        for (int n = 0; n < NT; ++n) mma_f16((ks & 1) ? s2[p][n] : s[p][n], af, qf[n][ks][0], qf[n][ks][1]);
       }
     int vx[P][2];
     bool grow = false;
@@ -383,7 +384,7 @@ struct HeadState {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float x = on ? s[p][n][2 * r + c] * (kf * qs[n][c]) : -INFINITY;
+            const float x = on ? (s[p][n][2 * r + c] + s2[p][n][2 * r + c]) * (kf * qs[n][c]) : -INFINITY;
             s[p][n][2 * r + c] = x;
             grow |= x > m[n][c] + 4.f;
           }
@@ -485,21 +486,49 @@ struct HeadState {
 //     last of those CTAs to arrive folds these in CTA order.
 // All orders are fixed, so results do not depend on timing. At most one pair
 // enters a CTA's run and one leaves it, hence two global partials per CTA.
-template <int NT>
-constexpr int kWarps = NT == 1 ? 16 : 8;
+constexpr int kWarps = 8;
+constexpr int kAlone = 8;          // pages a warp takes alone rather than share them and merge
+constexpr float kMergeCost = 1.f;  // see plan_work
 constexpr int kStageBytes = 2 * PAGE * D + 64;  // K, V, 2 x 16 exponents
 constexpr int kRow = D + 4;                     // floats per head of a partial in shared memory (bank spread)
 
 template <int NT>
-constexpr int kStages = NT == 1 ? 3 : 6;
+constexpr int kStages = NT == 1 ? 5 : 4;
+
+// x / n for x / n below 2^20.
+MBX_DEVICE int quotient(int x, int n) {
+  int q = __float2int_rz(__fdividef((float)x, (float)n));
+  const int r = x - q * n;
+  return q + (r >= n) - (r < 0);
+}
+
+// How the work is cut. kList: runs of `run` pages of the list. Where no pair is
+// longer than a few pages, sharing and merging it costs more than it saves:
+// kWarp gives each warp a pair, kCta each CTA one (its warps `run` pages each).
+enum Cut : int { kList, kWarp, kCta };
+struct WorkPlan {
+  int cut, run;
+};
+// pages: of all requests together; top: of the longest.
+MBX_DEVICE WorkPlan plan_work(int pages, int top, int pairs, int nkv, int grid, int warps) {
+  if (top <= kAlone && pairs <= grid * warps) return {kWarp, top};
+  if (top <= kAlone * warps && pairs <= grid) return {kCta, (top + warps - 1) / warps};
+  const int n = grid * warps;
+  // with few pairs, one more CTA per pair costs its merge more than it saves
+  float root;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"((float)top));
+  return {kList, max(max(1, quotient(pages * nkv + n - 1, n)), (int)(root * (kMergeCost / warps) + 0.999f))};
+}
 
 template <int NT>
 struct DecodeSmem {
   static constexpr int kHeads = 8 * NT;
   static constexpr int kWarpBytes = kStages<NT> * kStageBytes;  // a warp's ring, then its last segment's partial
-  static constexpr int kMl = kWarps<NT> * kWarpBytes;           // float2 [2][kWarps][kHeads]
-  static constexpr int kTotal = kMl + 2 * kWarps<NT> * kHeads * 8;
-  static_assert(kWarpBytes >= kHeads * kRow * 4, "a partial fits in the ring");
+  static constexpr int kPartBytes = kHeads * kRow * 4;
+  static constexpr int kPart = kWarps * kWarpBytes;             // [kWarps] partials of the warps' first segments
+  static constexpr int kMl = kPart + kWarps * kPartBytes;       // float2 [2][kWarps][kHeads]
+  static constexpr int kTotal = kMl + 2 * kWarps * kHeads * 8;
+  static_assert(kWarpBytes >= kPartBytes, "a partial fits in the ring");
 };
 
 MBX_DEVICE uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -515,120 +544,119 @@ MBX_DEVICE void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// What a warp's first (it began before the warp's run) and last (it goes on
-// behind it) segments left for the merge.
-struct SegMeta {
-  int valid;   // there is a partial
-  int ends;    // first segment only: the pair's pages end in this warp's run
-  int far;     // first segment only: its state is in global memory
-  int b, kvh;
-  int begin;   // list index of the pair's first page
-  int pages;
-};
+// What a warp left for the merge: of its first segment, where that began before
+// the warp's run (slot 0), and of its last, where that goes on behind it (slot
+// 1). kEnds: the pair's pages end in this warp's run.
+enum SegFlags : int { kHere = 1, kEnds = 2 };
 
-// One merge of partials of one head by one warp: lane l owns dims 4l..4l+3.
-struct Fold {
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  MBX_DEVICE void add(float pm, float pl, const float4& po) {
-    const float nm = fmaxf(m, pm);
-    const float a = nm == -INFINITY ? 0.f : ex2(m - nm), b = nm == -INFINITY ? 0.f : ex2(pm - nm);
-    m = nm;
-    l = l * a + pl * b;
-    o.x = o.x * a + po.x * b;
-    o.y = o.y * a + po.y * b;
-    o.z = o.z * a + po.z * b;
-    o.w = o.w * a + po.w * b;
-  }
-  MBX_DEVICE void store(__nv_bfloat16* dst, int lane) const {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x * inv, o.y * inv);
-    const __nv_bfloat162 hi = __floats2bfloat162_rn(o.z * inv, o.w * inv);
-    uint2 w;
-    w.x = *reinterpret_cast<const uint32_t*>(&lo);
-    w.y = *reinterpret_cast<const uint32_t*>(&hi);
-    *reinterpret_cast<uint2*>(dst + lane * 4) = w;
-  }
-};
-
-template <int W>
-MBX_DEVICE int block_sum(int v, int* red) {
+MBX_DEVICE float merge_weight(float m, float M) { return M == -INFINITY ? 0.f : ex2(m - M); }
+MBX_DEVICE float warp_max(float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int s = 0;
-#pragma unroll
-  for (int i = 0; i < W; ++i) s += red[i];
-  return s;
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
-
+// 1 / l, or 0 for a row without keys. One unit in the last place of fp32 is
+// far below the bf16 rounding that follows.
+MBX_DEVICE float inverse(float l) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(l));
+  return l == 0.f ? 0.f : r;
+}
+// Loads of partials: shared memory, or global memory past L1 (other CTAs may
+// have written them).
+MBX_DEVICE float4 ld_partial4(const float* p) {
+  float4 v;
+  asm volatile("ld.volatile.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+MBX_DEVICE float2 ld_partial2(const float* p) {
+  float2 v;
+  asm volatile("ld.volatile.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p));
+  return v;
+}
+MBX_DEVICE void add_scaled(float4& o, float w, const float4& x) {
+  o.x += w * x.x;
+  o.y += w * x.y;
+  o.z += w * x.z;
+  o.w += w * x.w;
+}
 template <int NT>
-__global__ void __launch_bounds__(kWarps<NT> * 32, 1) decode_kv8_kernel(Kv8DecodeArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArgs a) {
   using S = DecodeSmem<NT>;
-  constexpr int kSt = kStages<NT>, kW = kWarps<NT>;
+  constexpr int kSt = kStages<NT>, kW = kWarps;
   pdl_wait();
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int red[kW];
-  __shared__ int start_b[kW], start_off[kW];
-  __shared__ SegMeta meta[2][kW];
+  __shared__ int flags[2][kW];   // SegFlags
+  __shared__ int4 pairs[2][kW];  // of these segments: request, kv head, list index of the pair's first page, its pages
   __shared__ int s_last[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = a.nq / a.nkv;
-  auto pages_of = [&](int b) {
-    return (min(max(a.kv_len[b], 0), a.max_blocks * PAGE) + PAGE - 1) / PAGE;
-  };
-  // partials that wait for the CTA's merge while their warp works on
-  auto near_part = [&](int w) {
-    return a.part + (int64_t)gridDim.x * 2 * S::kHeads * (D + 2) + ((int64_t)blockIdx.x * kW + w) * S::kHeads * kRow;
-  };
-  // ---- this warp's run [u0, u1) of the page list, and where it starts
-  if (threadIdx.x < 2 * kW) meta[threadIdx.x / kW][threadIdx.x % kW].valid = 0;
-  const int first = (int)threadIdx.x < a.B ? pages_of(threadIdx.x) : 0;
-  int sum = first;
-  for (int b = threadIdx.x + blockDim.x; b < a.B; b += blockDim.x) sum += pages_of(b);
-  const int total = block_sum<kW>(sum, red) * a.nkv;
-  const int n_warps = gridDim.x * kW;
-  const int run = max(1, (total + n_warps - 1) / n_warps);
-  const int cta_u0 = blockIdx.x * kW * run;
-  for (int b0 = 0, carry = 0; b0 < a.B; b0 += blockDim.x) {
-    const int b = b0 + threadIdx.x;
-    const int n = b0 == 0 ? first : (b < a.B ? pages_of(b) : 0);
-    int inc = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += up;
-    }
-    __syncthreads();
-    if (lane == 31) red[warp] = inc;
-    __syncthreads();
-    int before = carry;
-#pragma unroll
-    for (int i = 0; i < kW; ++i) {
-      if (i < warp) before += red[i];
-      carry += red[i];
-    }
-    const int64_t lo = (int64_t)(before + inc - n) * a.nkv, hi = lo + (int64_t)n * a.nkv;
-    if (n > 0 && lo < (int64_t)cta_u0 + kW * run && hi > cta_u0)
-      for (int w = 0; w < kW; ++w) {
-        const int64_t u = (int64_t)cta_u0 + w * run;
-        if (u >= lo && u < hi) {
-          start_b[w] = b;
-          start_off[w] = (int)(u - lo);
-        }
-      }
-    // requests without keys: zeros, by the CTAs in turn
-    if (b < a.B && n == 0 && b % gridDim.x == blockIdx.x) {
-      uint4* dst = reinterpret_cast<uint4*>(a.o + (int64_t)b * a.nq * D);
-      for (int i = 0; i < a.nq * D / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
-    }
+  const int max_keys = a.max_blocks * PAGE;
+  auto pages_of = [&](int b) { return b < a.B ? (min(max(a.kv_len[b], 0), max_keys) + PAGE - 1) / PAGE : 0; };
+  if (lane < 2) flags[lane][warp] = 0;
+  // ---- this warp's run of pages, and where it starts: every warp for itself.
+  // Lane c holds the pages of requests 32c .. 32c + 31 (of each 1024).
+  int total = 0, top = 0, sums = 0;
+#pragma unroll 1
+  for (int c0 = 0; c0 * 32 < a.B; c0 += 2) {
+    const int x = pages_of(c0 * 32 + lane), y = pages_of(c0 * 32 + 32 + lane);
+    const int sx = __reduce_add_sync(0xffffffffu, x), sy = __reduce_add_sync(0xffffffffu, y);
+    top = max(top, max(x, y));
+    total += sx + sy;
+    if (lane == c0) sums = sx;
+    if (lane == c0 + 1) sums = sy;
   }
-  __syncthreads();
+  top = __reduce_max_sync(0xffffffffu, top);
+  const WorkPlan plan = plan_work(total, top, a.B * a.nkv, a.nkv, gridDim.x, kW);
+  const int run = plan.run;
+  const int u0 = (blockIdx.x * kW + warp) * run;  // first page in the list
+  int n_mine = 0;
+  int4 at = make_int4(0, 0, 0, 0);  // request, kv head, page and the pair's pages there
+  if (plan.cut == kList) {
+    n_mine = max(0, min(run, total * a.nkv - u0));
+    if (n_mine > 0) {
+      auto scan = [&](int v) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, v, o);
+          if (lane >= o) v += x;
+        }
+        return v;
+      };
+      int before = 0, b0 = 0;  // pages of the requests in front; first of the 1024 looked at
+      int end = scan(sums);
+#pragma unroll 1
+      while (__shfl_sync(0xffffffffu, end, 31) * a.nkv <= u0) {
+        before = __shfl_sync(0xffffffffu, end, 31);
+        b0 += 1024;
+        sums = 0;
+#pragma unroll 1
+        for (int c = 0; c < 32; ++c) {
+          const int x = __reduce_add_sync(0xffffffffu, pages_of(b0 + c * 32 + lane));
+          if (lane == c) sums = x;
+        }
+        end = before + scan(sums);
+      }
+      const int c = __popc(__ballot_sync(0xffffffffu, end * a.nkv <= u0));
+      before = __shfl_sync(0xffffffffu, end - sums, c);
+      const int n = pages_of(b0 + c * 32 + lane);
+      end = before + scan(n);
+      const int r = __popc(__ballot_sync(0xffffffffu, end * a.nkv <= u0));
+      at.x = b0 + c * 32 + r;
+      at.w = __shfl_sync(0xffffffffu, n, r);
+      const int off = u0 - __shfl_sync(0xffffffffu, end - n, r) * a.nkv;
+      at.y = quotient(off, at.w);
+      at.z = off - at.y * at.w;
+    }
+  } else {
+    const int pair = plan.cut == kCta ? blockIdx.x : blockIdx.x * kW + warp;
+    at.x = quotient(pair, a.nkv);
+    at.y = pair - at.x * a.nkv;
+    at.z = plan.cut == kCta ? warp * run : 0;
+    at.w = pages_of(at.x);
+    n_mine = max(0, min(run, at.w - at.z));
+  }
 
-  const int64_t u0 = (int64_t)cta_u0 + warp * run;
-  const int n_mine = u0 >= total ? 0 : (int)min((int64_t)run, total - u0);
   const uint32_t ring = smem_addr(smem) + warp * S::kWarpBytes;
   if (n_mine > 0) {
     // cursors into the list: the pages being fetched and the ones being used
@@ -636,10 +664,10 @@ __global__ void __launch_bounds__(kWarps<NT> * 32, 1) decode_kv8_kernel(Kv8Decod
       int b, kvh, p, pages;
     };
     Cursor in, use;
-    in.b = start_b[warp];
-    in.pages = pages_of(in.b);
-    in.kvh = start_off[warp] / in.pages;
-    in.p = start_off[warp] % in.pages;
+    in.b = at.x;
+    in.kvh = at.y;
+    in.p = at.z;
+    in.pages = at.w;
     use = in;
     auto next_pair = [&](Cursor& c) {
       c.p = 0;
@@ -647,7 +675,7 @@ __global__ void __launch_bounds__(kWarps<NT> * 32, 1) decode_kv8_kernel(Kv8Decod
       c.kvh = 0;
       do {
         ++c.b;
-        c.pages = pages_of(c.b);
+        c.pages = pages_of(c.b);  // there is another: the run is not at its end
       } while (c.pages == 0);
     };
     // Each copy instruction reads 512 contiguous bytes (four rows, lane l the
@@ -692,7 +720,7 @@ __global__ void __launch_bounds__(kWarps<NT> * 32, 1) decode_kv8_kernel(Kv8Decod
       ++in.p;
     };
     // groups 0..kSt-1: the first pages; then one group per page used, in order
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < kSt; ++i) {
       if (i < n_mine) fetch(i);
       cp_async_commit();
@@ -705,7 +733,7 @@ __global__ void __launch_bounds__(kWarps<NT> * 32, 1) decode_kv8_kernel(Kv8Decod
     for (int i = 0; i < n_mine;) {
       if (fresh) {
         st.begin(a.q + ((int64_t)use.b * a.nq + use.kvh * G) * D, G, a.scale_log2, lane);
-        L = min(a.kv_len[use.b], a.max_blocks * PAGE);
+        L = min(a.kv_len[use.b], max_keys);
         seg_p0 = use.p;
         fresh = false;
       }
@@ -716,20 +744,17 @@ __global__ void __launch_bounds__(kWarps<NT> * 32, 1) decode_kv8_kernel(Kv8Decod
                                      smem + warp * S::kWarpBytes + stage1 * kStageBytes};
       const bool two = i + 1 < n_mine && use.p + 1 < use.pages;
       const int live[2] = {(bad >> stage) & 1 ? 0 : min(PAGE, L - use.p * PAGE),
-                           (bad >> stage1) & 1 ? 0 : min(PAGE, L - use.p * PAGE - PAGE)};
-      if (two) st.template pages<2>(src, live, lane);
-      else st.template pages<1>(src, live, lane);
+                           !two || ((bad >> stage1) & 1) ? 0 : min(PAGE, L - use.p * PAGE - PAGE)};
+      st.template pages<2>(src, live, lane);
       __syncwarp();
-      if (i + kSt < n_mine) fetch(stage);
-      cp_async_commit();
-      if (two) {
-        if (i + 1 + kSt < n_mine) fetch(stage1);
+#pragma unroll 1
+      for (int u = two ? 2 : 1; u > 0; --u) {
+        if (i + kSt < n_mine) fetch(stage);
         cp_async_commit();
+        stage = stage + 1 == kSt ? 0 : stage + 1;
+        ++i;
+        ++use.p;
       }
-      const int used = two ? 2 : 1;
-      stage = two ? (stage1 + 1 == kSt ? 0 : stage1 + 1) : stage1;
-      i += used;
-      use.p += used;
       const bool ends = use.p == use.pages;
       if (!ends && i < n_mine) continue;
       // ---- the segment is done
@@ -742,7 +767,7 @@ __global__ void __launch_bounds__(kWarps<NT> * 32, 1) decode_kv8_kernel(Kv8Decod
           for (int c = 0; c < 2; ++c) {
             const int head = n * 8 + 2 * t + c;
             if (head >= G) continue;
-            const float inv = st.l[n][c] == 0.f ? 0.f : vs / st.l[n][c];
+            const float inv = vs * inverse(st.l[n][c]);
             float f[16];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -754,11 +779,10 @@ __global__ void __launch_bounds__(kWarps<NT> * 32, 1) decode_kv8_kernel(Kv8Decod
             *reinterpret_cast<uint4*>(dst + 8) = pack_from<__nv_bfloat16>(f + 8);
           }
       } else {
-        // began earlier: slot 0; begins here and goes on: slot 1. The run's last
-        // segment leaves its state in the ring, an earlier one in global memory.
+        // began earlier: slot 0; begins here and goes on behind the run, whose
+        // ring is free then: slot 1
         const int slot = seg_p0 == 0 ? 1 : 0;
-        const bool far = i < n_mine;
-        float* po = far ? near_part(warp) : reinterpret_cast<float*>(smem + warp * S::kWarpBytes);
+        float* po = reinterpret_cast<float*>(smem + (slot == 0 ? S::kPart + warp * S::kPartBytes : warp * S::kWarpBytes));
         float2* ml = reinterpret_cast<float2*>(smem + S::kMl) + (slot * kW + warp) * S::kHeads;
         __syncwarp();
 #pragma unroll
@@ -774,89 +798,142 @@ __global__ void __launch_bounds__(kWarps<NT> * 32, 1) decode_kv8_kernel(Kv8Decod
             if (g == 0) ml[head] = make_float2(st.m[n][c], st.l[n][c]);
           }
         if (lane == 0) {
-          SegMeta& sm = meta[slot][warp];
-          sm.valid = 1;
-          sm.ends = ends;
-          sm.far = far;
-          sm.b = use.b;
-          sm.kvh = use.kvh;
-          sm.begin = (int)(u0 + i) - use.p;
-          sm.pages = use.pages;
+          flags[slot][warp] = kHere | (ends ? kEnds : 0);
+          pairs[slot][warp] = make_int4(use.b, use.kvh, u0 + i - use.p, use.pages);
         }
       }
       if (ends && i < n_mine) next_pair(use);
       fresh = true;
     }
   }
+  // requests without keys: zeros, by the CTAs in turn
+#pragma unroll 1
+  for (int b = blockIdx.x + gridDim.x * warp; b < a.B; b += gridDim.x * kW) {
+    if (pages_of(b) > 0) continue;
+    uint4* dst = reinterpret_cast<uint4*>(a.o + (int64_t)b * a.nq * D);
+#pragma unroll 1
+    for (int i = lane; i < a.nq * D / 8; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
+  }
   __syncthreads();
 
-  // ---- fold the warps' partials: chain a = -1 entered the CTA's run, chain a
-  // in 0..kW-1 begins in warp a's
-  const float2* ml = reinterpret_cast<const float2*>(smem + S::kMl);
-  auto piece = [&](bool far, int w, int head) {
-    const float* p = far ? near_part(w) : reinterpret_cast<const float*>(smem + w * S::kWarpBytes);
-    return *reinterpret_cast<const float4*>(p + head * kRow + lane * 4);
-  };
-  float2* part_ml = reinterpret_cast<float2*>(a.part + (int64_t)gridDim.x * 2 * S::kHeads * D);
-  const int span = kW * run;  // pages per CTA
-  int out_chain[2] = {-2, -2};    // chains that reach into other CTAs, by global slot (0: entered, 1: begins here)
-  for (int c = -1; c < kW; ++c) {
-    const SegMeta& sm = c < 0 ? meta[0][0] : meta[1][c];
-    if (!sm.valid) continue;
-    int last = c;  // the chain's last warp in this CTA
-    bool ended = false;
-    while (!ended && last + 1 < kW && meta[0][last + 1].valid) ended = meta[0][++last].ends;
-    const bool whole = c >= 0 && ended;
-    if (!whole) out_chain[c < 0 ? 0 : 1] = c;
-    for (int head = warp; head < G; head += kW) {
-      Fold f;
-      if (c >= 0) f.add(ml[(kW + c) * S::kHeads + head].x, ml[(kW + c) * S::kHeads + head].y, piece(false, c, head));
-      for (int w = c + 1; w <= last; ++w) {
-        const float2 x = ml[w * S::kHeads + head];
-        f.add(x.x, x.y, piece(meta[0][w].far, w, head));
-      }
-      if (whole) {
-        f.store(a.o + ((int64_t)sm.b * a.nq + sm.kvh * G + head) * D, lane);
-      } else {
-        const int64_t at = ((int64_t)blockIdx.x * 2 + (c < 0 ? 0 : 1)) * S::kHeads + head;
-        *reinterpret_cast<float4*>(a.part + at * D + lane * 4) = f.o;
-        if (lane == 0) part_ml[at] = make_float2(f.m, f.l);
-      }
-    }
-  }
-  if (out_chain[0] == -2 && out_chain[1] == -2) return;
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    int last = -1;
-    const int c = out_chain[threadIdx.x];
-    if (c != -2) {
-      const SegMeta& sm = c < 0 ? meta[0][0] : meta[1][c];
-      const int c0 = sm.begin / span, c1 = (sm.begin + sm.pages - 1) / span;
-      if (atomicAdd(a.counters + c0, 1) == c1 - c0) {
-        a.counters[c0] = 0;  // for the next launch
-        last = c0;
-      }
-    }
-    s_last[threadIdx.x] = last;
-  }
-  __syncthreads();
+  // ---- merges. Level 0, the warps' partials: chain 0 entered the CTA's run,
+  // chain c + 1 begins in warp c's; it goes on through the first segments of the
+  // warps that follow, up to the first that ends. Level 1, by the last CTA to
+  // arrive: the CTAs' partials of a pair that reaches over CTAs. One code for
+  // both (what runs once a launch waits for its instructions, too): partial 0
+  // lies by itself, the others a stride apart. A warp per (chain, head): lane i
+  // has partial i's (m, l), so that the weights 2^(m_i - M) come at once and the
+  // rows (lane l: dims 4l..4l+3) are independent loads.
+  const int f0 = lane < kW ? flags[0][lane] : 0, f1 = lane < kW ? flags[1][lane] : 0;
+  const uint32_t held = __ballot_sync(0xffffffffu, f0 != 0), ended = __ballot_sync(0xffffffffu, f0 & kEnds),
+                 begun = __ballot_sync(0xffffffffu, f1 != 0);
+  float* part_ml = a.part + (int64_t)gridDim.x * 2 * S::kHeads * D;
+  const int span = kW * run;     // pages per CTA
+  const bool out0 = held & 1;    // chain 0 is one of several CTAs'
+  int out1 = -1;                 // the warp in whose run a pair begins that goes on in the next CTA
+  uint32_t todo = (begun << 1) | (held & 1);
 #pragma unroll 1
-  for (int slot = 0; slot < 2; ++slot) {
-    if (s_last[slot] < 0) continue;
-    __threadfence();
-    const SegMeta& sm = out_chain[slot] < 0 ? meta[0][0] : meta[1][out_chain[slot]];
-    const int c0 = s_last[slot], c1 = (sm.begin + sm.pages - 1) / span;
-    for (int head = warp; head < G; head += kW) {
-      Fold f;
-#pragma unroll 4
-      for (int c = c0; c <= c1; ++c) {
-        const int64_t at = ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * S::kHeads + head;
-        const float2 x = __ldcg(part_ml + at);
-        f.add(x.x, x.y, __ldcg(reinterpret_cast<const float4*>(a.part + at * D) + lane));
+  for (int level = 0; level < 2; ++level) {
+    int turn = warp;
+#pragma unroll 1
+    for (; todo != 0; todo &= todo - 1) {
+      const int c = __ffs(todo) - 2;  // -1, or the warp whose run the pair begins in
+      const int begins = c >= 0;
+      const int4 pair = begins ? pairs[1][c] : pairs[0][0];
+      int n;
+      bool whole = true;
+      const float *row0, *row1, *ml0, *ml1;  // rows and (m, l) of partials 0 and 1 of head 0
+      int row_step, ml_step, head_step;      // in floats
+      if (level == 0) {
+        const uint32_t ends = ended >> (c + 1);
+        n = begins + (ends ? __ffs(ends) : __popc(held >> (c + 1)));
+        whole = begins && ends;
+        if (begins && !ends) out1 = c;
+        const float* const parts = reinterpret_cast<const float*>(smem + S::kPart);
+        const float* const ml = reinterpret_cast<const float*>(smem + S::kMl);
+        row_step = S::kPartBytes / 4;
+        row1 = parts + (c + 1 + !begins) * row_step;
+        row0 = begins ? reinterpret_cast<const float*>(smem + c * S::kWarpBytes) : parts;
+        ml_step = 2 * S::kHeads;
+        ml1 = ml + (c + 1 + !begins) * ml_step;
+        ml0 = ml + (begins ? kW + c : 0) * ml_step;
+        head_step = kRow;
+      } else {
+        const int c0 = s_last[begins];
+        n = quotient(pair.z + pair.w - 1, span) - c0 + 1;
+        row_step = 2 * S::kHeads * D;
+        row0 = a.part + (int64_t)(2 * c0 + 1) * S::kHeads * D;
+        row1 = row0 + S::kHeads * D;
+        ml_step = 4 * S::kHeads;
+        ml0 = part_ml + (2 * c0 + 1) * S::kHeads * 2;
+        ml1 = ml0 + 2 * S::kHeads;
+        head_step = D;
       }
-      f.store(a.o + ((int64_t)sm.b * a.nq + sm.kvh * G + head) * D, lane);
+#pragma unroll 1
+      for (; turn < G; turn += kW) {
+        const int head = turn;
+        float M = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int kBlock = 8;  // partials loaded at once
+#pragma unroll 1
+        for (int i0 = 0; i0 < n; i0 += kBlock) {
+          const int mine = i0 + lane;
+          const bool has = lane < kBlock && mine < n;
+          float2 x = make_float2(-INFINITY, 0.f);
+          if (has) x = ld_partial2((mine == 0 ? ml0 : ml1 + (mine - 1) * ml_step) + 2 * head);
+          float4 y[kBlock];
+#pragma unroll
+          for (int j = 0; j < kBlock; ++j) {
+            const int i = min(i0 + j, n - 1);
+            y[j] = ld_partial4((i == 0 ? row0 : row1 + (int64_t)(i - 1) * row_step) + head * head_step + lane * 4);
+          }
+          const float nm = fmaxf(M, warp_max(x.x));
+          const float keep = merge_weight(M, nm);
+          const float w = has ? merge_weight(x.x, nm) : 0.f;
+          M = nm;
+          l = l * keep + warp_sum(has ? w * x.y : 0.f);
+          o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll
+          for (int j = 0; j < kBlock; ++j) {
+            const float wj = __shfl_sync(0xffffffffu, w, j);
+            if (i0 + j < n) add_scaled(o, wj, y[j]);
+          }
+        }
+        if (whole) {
+          const float inv = inverse(l);
+          const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x * inv, o.y * inv);
+          const __nv_bfloat162 hi = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+          uint2 y;
+          y.x = *reinterpret_cast<const uint32_t*>(&lo);
+          y.y = *reinterpret_cast<const uint32_t*>(&hi);
+          *reinterpret_cast<uint2*>(a.o + ((int64_t)pair.x * a.nq + pair.y * G + head) * D + lane * 4) = y;
+        } else {
+          const int to = (blockIdx.x * 2 + begins) * S::kHeads + head;
+          *reinterpret_cast<float4*>(a.part + (int64_t)to * D + lane * 4) = o;
+          if (lane == 0) *reinterpret_cast<float2*>(part_ml + 2 * to) = make_float2(M, l);
+        }
+      }
+      turn -= G;
     }
+    if (level == 1 || (!out0 && out1 < 0)) return;
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      int last = -1;
+      if (threadIdx.x == 0 ? out0 : out1 >= 0) {
+        const int4 pair = threadIdx.x == 0 ? pairs[0][0] : pairs[1][out1];
+        const int c0 = quotient(pair.z, span), c1 = quotient(pair.z + pair.w - 1, span);
+        // this CTA's partials before the count, the count before the others' partials
+        int seen;
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(a.counters + c0) : "memory");
+        if (seen == c1 - c0) {
+          a.counters[c0] = 0;  // for the next launch
+          last = c0;
+        }
+      }
+      s_last[threadIdx.x] = last;
+    }
+    __syncthreads();
+    todo = (s_last[0] >= 0 ? 1u : 0u) | (s_last[1] >= 0 ? 2u << out1 : 0u);
   }
 }
 
@@ -909,13 +986,10 @@ int decode_kv8_grid(int B, int nkv, int max_blocks) {
   MBX_CUDA_CHECK(cudaGetDevice(&dev));
   MBX_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   const int64_t pages = (int64_t)B * nkv * max_blocks;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(sms, (pages + kWarps<2> - 1) / kWarps<2>));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(sms, (pages + kWarps - 1) / kWarps));
 }
 
-size_t decode_kv8_part_floats(int grid) {
-  static_assert(kWarps<1> * 8 == kWarps<2> * 16, "both forms keep as many heads per CTA");
-  return (size_t)grid * (2 * 16 * (D + 2) + kWarps<1> * 8 * kRow);
-}
+size_t decode_kv8_part_floats(int grid) { return (size_t)grid * 2 * 16 * (D + 2); }
 
 void decode_attention_kv8_launch(const void* q, const Kv8Cache& c, void* o, const int* kv_len, const int* block_table,
                                  int64_t bt_stride, int max_blocks, int B, int nq, int nkv, int grid, float* part,
@@ -928,11 +1002,11 @@ void decode_attention_kv8_launch(const void* q, const Kv8Cache& c, void* o, cons
   if (nq / nkv <= 8) {
     static SmemLimit limit;
     limit.ensure((const void*)decode_kv8_kernel<1>, DecodeSmem<1>::kTotal);
-    launch_k(decode_kv8_kernel<1>, dim3(grid), dim3(kWarps<1> * 32), DecodeSmem<1>::kTotal, s, a);
+    launch_k(decode_kv8_kernel<1>, dim3(grid), dim3(kWarps * 32), DecodeSmem<1>::kTotal, s, a);
   } else {
     static SmemLimit limit;
     limit.ensure((const void*)decode_kv8_kernel<2>, DecodeSmem<2>::kTotal);
-    launch_k(decode_kv8_kernel<2>, dim3(grid), dim3(kWarps<2> * 32), DecodeSmem<2>::kTotal, s, a);
+    launch_k(decode_kv8_kernel<2>, dim3(grid), dim3(kWarps * 32), DecodeSmem<2>::kTotal, s, a);
   }
   MBX_CUDA_CHECK(cudaGetLastError());
 }

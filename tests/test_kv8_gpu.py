@@ -383,7 +383,9 @@ def test_decode_non_finite_inputs_stay_in_their_rows():
     lens, nq, nkv = [50, 50, 50, 600], 8, 2
     k8, v8, kvl, table = _cache(lens, nkv, seed=8)
     q = torch.randn(4, nq, D, device="cuda", generator=_gen(8)).to(torch.bfloat16)
-    want = ops.decode_attention(q, k8, v8, kvl, table)
+    exact = [_attention(q[b:b + 1], _row(k8, table[b], n), _row(v8, table[b], n), D ** -0.5)
+             for b, n in enumerate(lens)]
+    want, tol = (torch.cat(x) for x in zip(*exact))
     q[0, 1, 5] = float("nan")
     q[1, 2, 9] = float("inf")
     _bytes_of(v8)[table[2, 1].long(), 1, 3, 7] = 0x7F    # one element of one row: heads 4..7, dim 7
@@ -394,7 +396,10 @@ def test_decode_non_finite_inputs_stay_in_their_rows():
     bad[2, 4:, 7] = True
     bad[3, :4] = True
     assert torch.isnan(out[bad]).all()
-    assert torch.equal(out[~bad], want[~bad])
+    # The others: the definition's values. Not the same bits as without the
+    # NaN, since the heads that share a kv head move their running maxima
+    # together, and the weights' rounding goes with them.
+    assert ((out.double() - want).abs() <= tol)[~bad].all()
 
 
 def test_decode_tables_lengths_and_pages_outside():
