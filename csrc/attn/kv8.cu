@@ -295,28 +295,37 @@ struct HeadState {
   float m[NT][2], l[NT][2];  // l: this lane's keys only
   int vr;
 
-  MBX_DEVICE void begin(const __nv_bfloat16* q, int G, float scale_log2, int lane) {
-    const int g = lane >> 2, t = lane & 3;
+  // This lane's elements of q [G, D] (heads behind G: zeros), in two steps, so
+  // that the loads can be issued ahead of their use.
+  struct Query {
+    uint4 w[NT][4];
+    MBX_DEVICE void load(const __nv_bfloat16* q, int G, int lane) {
+      const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          w[n][c] = n * 8 + g < G ? ld_v4(q + (n * 8 + g) * D + (t + 4 * (c >> 1)) * 16 + (c & 1) * 8)
+                                  : make_uint4(0, 0, 0, 0);
+    }
+  };
+  MBX_DEVICE void begin(const Query& q, float scale_log2, int lane) {
+    const int t = lane & 3;
     vr = kNoExp;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int head = n * 8 + g;
       float x[2][16];
       float top = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int c = 0; c < 4; ++c) {
+        float f[8] = {};
+        unpack_add<__nv_bfloat16>(q.w[n][c], f);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (head < G) w = ld_v4(q + head * D + (t + 4 * h) * 16 + c * 8);
-          float f[8] = {};
-          unpack_add<__nv_bfloat16>(w, f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            x[h][c * 8 + i] = f[i];
-            top = fmaxf(top, fabsf(f[i]));
-          }
+        for (int i = 0; i < 8; ++i) {
+          x[c >> 1][(c & 1) * 8 + i] = f[i];
+          top = fmaxf(top, fabsf(f[i]));
         }
+      }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e = max((int)(__float_as_uint(top) >> 23) - 127, -112);
@@ -489,6 +498,7 @@ struct HeadState {
 constexpr int kWarps = 8;
 constexpr int kAlone = 8;          // pages a warp takes alone rather than share them and merge
 constexpr float kMergeCost = 1.f;  // see plan_work
+constexpr int kPad = 2;            // pages that a pair costs a warp besides its own, see plan_work
 constexpr int kStageBytes = 2 * PAGE * D + 64;  // K, V, 2 x 16 exponents
 constexpr int kRow = D + 4;                     // floats per head of a partial in shared memory (bank spread)
 
@@ -502,22 +512,30 @@ MBX_DEVICE int quotient(int x, int n) {
   return q + (r >= n) - (r < 0);
 }
 
-// How the work is cut. kList: runs of `run` pages of the list. Where no pair is
-// longer than a few pages, sharing and merging it costs more than it saves:
-// kWarp gives each warp a pair, kCta each CTA one (its warps `run` pages each).
+// How the work is cut. kList: runs of `run` entries of the list, in which every
+// pair is followed by `pad` empty ones. Where no pair is longer than a few
+// pages, sharing and merging it costs more than it saves: kWarp gives each warp
+// a pair, kCta each CTA one (its warps `run` pages each).
 enum Cut : int { kList, kWarp, kCta };
 struct WorkPlan {
-  int cut, run;
+  int cut, run, pad;
 };
-// pages: of all requests together; top: of the longest.
-MBX_DEVICE WorkPlan plan_work(int pages, int top, int pairs, int nkv, int grid, int warps) {
-  if (top <= kAlone && pairs <= grid * warps) return {kWarp, top};
-  if (top <= kAlone * warps && pairs <= grid) return {kCta, (top + warps - 1) / warps};
+// pages, some: of all requests together, and how many have any; top, low: the
+// longest and the shortest of those.
+MBX_DEVICE WorkPlan plan_work(int pages, int some, int top, int low, int pairs, int nkv, int grid, int warps) {
+  if (top <= kAlone && pairs <= grid * warps) return {kWarp, top, 0};
+  if (top <= kAlone * warps && pairs <= grid) return {kCta, (top + warps - 1) / warps, 0};
   const int n = grid * warps;
+  int run = max(1, quotient(pages * nkv + n - 1, n));
+  // Beginning and ending a pair takes a warp about as long as two pages. Where
+  // runs can hold whole pairs, warps with many short ones would come late; where
+  // they cannot, empty entries would only move pairs off the runs' borders.
+  const int pad = low < run ? kPad : 0;
+  if (pad) run = max(1, quotient((pages + pad * some) * nkv + n - 1, n));
   // with few pairs, one more CTA per pair costs its merge more than it saves
   float root;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"((float)top));
-  return {kList, max(max(1, quotient(pages * nkv + n - 1, n)), (int)(root * (kMergeCost / warps) + 0.999f))};
+  return {kList, max(run, (int)(root * (kMergeCost / warps) + 0.999f)), pad};
 }
 
 template <int NT>
@@ -595,26 +613,31 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
   auto pages_of = [&](int b) { return b < a.B ? (min(max(a.kv_len[b], 0), max_keys) + PAGE - 1) / PAGE : 0; };
   if (lane < 2) flags[lane][warp] = 0;
   // ---- this warp's run of pages, and where it starts: every warp for itself.
-  // Lane c holds the pages of requests 32c .. 32c + 31 (of each 1024).
-  int total = 0, top = 0, sums = 0;
+  // Lane c holds the pages of requests 32c .. 32c + 31 (of each 1024), and how
+  // many of them have any.
+  int total = 0, some = 0, top = 0, low = 1 << 30, sums = 0, counts = 0;
 #pragma unroll 1
-  for (int c0 = 0; c0 * 32 < a.B; c0 += 2) {
-    const int x = pages_of(c0 * 32 + lane), y = pages_of(c0 * 32 + 32 + lane);
-    const int sx = __reduce_add_sync(0xffffffffu, x), sy = __reduce_add_sync(0xffffffffu, y);
-    top = max(top, max(x, y));
-    total += sx + sy;
-    if (lane == c0) sums = sx;
-    if (lane == c0 + 1) sums = sy;
+  for (int c0 = 0; c0 * 32 < a.B; ++c0) {
+    const int x = pages_of(c0 * 32 + lane);
+    const int sx = __reduce_add_sync(0xffffffffu, x), nx = __popc(__ballot_sync(0xffffffffu, x > 0));
+    total += sx;
+    some += nx;
+    top = max(top, x);
+    low = x > 0 ? min(low, x) : low;
+    if (lane == c0) sums = sx, counts = nx;
   }
   top = __reduce_max_sync(0xffffffffu, top);
-  const WorkPlan plan = plan_work(total, top, a.B * a.nkv, a.nkv, gridDim.x, kW);
-  const int run = plan.run;
+  low = __reduce_min_sync(0xffffffffu, low);
+  const WorkPlan plan = plan_work(total, some, top, low, a.B * a.nkv, a.nkv, gridDim.x, kW);
+  const int run = plan.run, pad = plan.pad;
+  auto in_list = [&](int pages) { return pages > 0 ? pages + pad : 0; };
   const int u0 = (blockIdx.x * kW + warp) * run;  // first page in the list
-  int n_mine = 0;
+  int left = 0;     // of the run (list entries)
   int4 at = make_int4(0, 0, 0, 0);  // request, kv head, page and the pair's pages there
   if (plan.cut == kList) {
-    n_mine = max(0, min(run, total * a.nkv - u0));
-    if (n_mine > 0) {
+    sums += counts * pad;
+    left = max(0, min(run, (total + some * pad) * a.nkv - u0));
+    if (left > 0) {
       auto scan = [&](int v) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -632,21 +655,22 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
         sums = 0;
 #pragma unroll 1
         for (int c = 0; c < 32; ++c) {
-          const int x = __reduce_add_sync(0xffffffffu, pages_of(b0 + c * 32 + lane));
+          const int x = __reduce_add_sync(0xffffffffu, in_list(pages_of(b0 + c * 32 + lane)));
           if (lane == c) sums = x;
         }
         end = before + scan(sums);
       }
       const int c = __popc(__ballot_sync(0xffffffffu, end * a.nkv <= u0));
       before = __shfl_sync(0xffffffffu, end - sums, c);
-      const int n = pages_of(b0 + c * 32 + lane);
+      const int n = in_list(pages_of(b0 + c * 32 + lane));
       end = before + scan(n);
       const int r = __popc(__ballot_sync(0xffffffffu, end * a.nkv <= u0));
       at.x = b0 + c * 32 + r;
-      at.w = __shfl_sync(0xffffffffu, n, r);
+      const int len = __shfl_sync(0xffffffffu, n, r);
       const int off = u0 - __shfl_sync(0xffffffffu, end - n, r) * a.nkv;
-      at.y = quotient(off, at.w);
-      at.z = off - at.y * at.w;
+      at.y = quotient(off, len);
+      at.z = off - at.y * len;
+      at.w = len - pad;
     }
   } else {
     const int pair = plan.cut == kCta ? blockIdx.x : blockIdx.x * kW + warp;
@@ -654,30 +678,48 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
     at.y = pair - at.x * a.nkv;
     at.z = plan.cut == kCta ? warp * run : 0;
     at.w = pages_of(at.x);
-    n_mine = max(0, min(run, at.w - at.z));
+    left = max(0, min(run, at.w - at.z));
   }
 
   const uint32_t ring = smem_addr(smem) + warp * S::kWarpBytes;
-  if (n_mine > 0) {
-    // cursors into the list: the pages being fetched and the ones being used
+  if (left > 0) {
+    // cursors: the pages being used, and the ones being fetched
     struct Cursor {
-      int b, kvh, p, pages;
+      int b, kvh, p, pages, left;
     };
-    Cursor in, use;
-    in.b = at.x;
-    in.kvh = at.y;
-    in.p = at.z;
-    in.pages = at.w;
-    use = in;
-    auto next_pair = [&](Cursor& c) {
+    Cursor use{at.x, at.y, at.z, at.w, left};
+    int pos = u0;  // use's place in the list
+    auto pages_in = [&](int keys) { return (min(max(keys, 0), max_keys) + PAGE - 1) / PAGE; };
+    auto keys_of = [&](int b) { return b < a.B ? a.kv_len[b] : 0; };
+    // to the next pair (there is one), with the length of the next request in hand
+    auto next_pair = [&](Cursor& c, int next_keys) {
       c.p = 0;
-      if (++c.kvh < a.nkv) return;
+      if (++c.kvh < a.nkv) return false;
       c.kvh = 0;
-      do {
-        ++c.b;
-        c.pages = pages_of(c.b);  // there is another: the run is not at its end
-      } while (c.pages == 0);
+      ++c.b;
+      c.pages = pages_in(next_keys);
+#pragma unroll 1
+      while (c.pages == 0) c.pages = pages_of(++c.b);
+      return true;
     };
+    if (use.p >= use.pages) {  // the run starts in the room behind a pair
+      use.left -= use.pages + pad - use.p;
+      pos += use.pages + pad - use.p;
+      if (use.left > 0) next_pair(use, keys_of(use.b + 1));
+    }
+    Cursor in = use;
+    // What the cursors will need is loaded ahead: lane i holds the block of page
+    // win + i of the request being fetched, of page win + 32 + i, of page i of
+    // it and of the next request, whose length next_keys is.
+    auto ids_of = [&](int b, int p) {
+      return b < a.B && p + lane < a.max_blocks ? a.block_table[b * a.bt_s + p + lane] : -1;
+    };
+    int win = in.p, id = ids_of(in.b, win), id_next = ids_of(in.b, win + 32);
+    int first = ids_of(in.b, 0), next_first = ids_of(in.b + 1, 0), next_keys = keys_of(in.b + 1);
+    typename HeadState<NT>::Query query;
+    auto load_query = [&](int b, int kvh) { query.load(a.q + ((int64_t)b * a.nq + kvh * G) * D, G, lane); };
+    if (use.left > 0) load_query(use.b, use.kvh);
+    int keys = keys_of(use.b), use_next_keys = next_keys;
     // Each copy instruction reads 512 contiguous bytes (four rows, lane l the
     // l-th 16) and places them where pages() reads them.
     uint32_t k_dst[2], v_dst[2];
@@ -687,27 +729,36 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
       k_dst[i] = k_place(row, ch);
       v_dst[i] = 2048 + v_place(row, ch);
     }
-    int win = -1;       // first page of the table window that the lanes hold
-    int id = -1;
-    uint32_t bad = 0;   // stages whose page is not in the cache
+    uint32_t bad = 0;  // stages whose page is not in the cache
     auto fetch = [&](int st) {
       if (in.p == in.pages) {
-        next_pair(in);
-        win = -1;
+        in.left -= pad;
+        if (in.left <= 0) return;
+        const int b = in.b;
+        if (next_pair(in, next_keys)) {
+          first = in.b == b + 1 ? next_first : ids_of(in.b, 0);
+          next_first = ids_of(in.b + 1, 0);
+          next_keys = keys_of(in.b + 1);
+        }
+        win = 0;
+        id = first;
+        id_next = in.pages > 32 ? ids_of(in.b, 32) : -1;
       }
-      if (win < 0 || in.p >= win + 32) {
-        win = in.p;
-        id = in.p + lane < in.pages ? a.block_table[in.b * a.bt_s + in.p + lane] : -1;
+      if (in.left <= 0) return;
+      if (in.p == win + 32) {
+        win += 32;
+        id = id_next;
+        id_next = ids_of(in.b, win + 32);
       }
       const int blk = __shfl_sync(0xffffffffu, id, in.p - win);
       const uint32_t dst = ring + st * kStageBytes;
       if (blk >= 0 && blk < a.num_blocks) {
         bad &= ~(1u << st);
-        const int64_t base = ((int64_t)blk * a.nkv + in.kvh) * PAGE * D;
+        const int64_t base = ((int64_t)blk * a.nkv + in.kvh) * PAGE * D + lane * 16;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          cp_async16(dst + k_dst[i & 1] + (i >> 1) * 1024, a.kv + base + i * 512 + lane * 16);
-          cp_async16(dst + v_dst[i & 1] + (i >> 1) * 1024, a.vv + base + i * 512 + lane * 16);
+          cp_async16(dst + k_dst[i & 1] + (i >> 1) * 1024, a.kv + base + i * 512);
+          cp_async16(dst + v_dst[i & 1] + (i >> 1) * 1024, a.vv + base + i * 512);
         }
         if (lane < 8) {
           const uint8_t* e = lane < 4 ? a.ke + blk * a.ke_sb + in.kvh * a.ke_sh + lane * 4
@@ -718,11 +769,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
         bad |= 1u << st;
       }
       ++in.p;
+      --in.left;
     };
     // groups 0..kSt-1: the first pages; then one group per page used, in order
 #pragma unroll 1
     for (int i = 0; i < kSt; ++i) {
-      if (i < n_mine) fetch(i);
+      fetch(i);
       cp_async_commit();
     }
     HeadState<NT> st;
@@ -730,33 +782,39 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
     int seg_p0 = use.p;  // the segment's first page
     int L = 0;
     int stage = 0;
-    for (int i = 0; i < n_mine;) {
+    while (use.left > 0) {
       if (fresh) {
-        st.begin(a.q + ((int64_t)use.b * a.nq + use.kvh * G) * D, G, a.scale_log2, lane);
-        L = min(a.kv_len[use.b], max_keys);
+        st.begin(query, a.scale_log2, lane);
+        L = min(keys, max_keys);
         seg_p0 = use.p;
         fresh = false;
+        // the next pair's query, where this warp will come to it
+        if (NT == 1 && use.left > use.pages - use.p + pad) {
+          const bool same = use.kvh + 1 < a.nkv;
+          load_query(same ? use.b : min(use.b + 1, a.B - 1), same ? use.kvh + 1 : 0);
+        }
       }
       cp_async_wait<kSt - 2>();
       __syncwarp();
       const int stage1 = stage + 1 == kSt ? 0 : stage + 1;
       const uint8_t* const src[2] = {smem + warp * S::kWarpBytes + stage * kStageBytes,
                                      smem + warp * S::kWarpBytes + stage1 * kStageBytes};
-      const bool two = i + 1 < n_mine && use.p + 1 < use.pages;
+      const bool two = use.left > 1 && use.p + 1 < use.pages;
       const int live[2] = {(bad >> stage) & 1 ? 0 : min(PAGE, L - use.p * PAGE),
                            !two || ((bad >> stage1) & 1) ? 0 : min(PAGE, L - use.p * PAGE - PAGE)};
       st.template pages<2>(src, live, lane);
       __syncwarp();
 #pragma unroll 1
       for (int u = two ? 2 : 1; u > 0; --u) {
-        if (i + kSt < n_mine) fetch(stage);
+        fetch(stage);
         cp_async_commit();
         stage = stage + 1 == kSt ? 0 : stage + 1;
-        ++i;
+        ++pos;
         ++use.p;
+        --use.left;
       }
       const bool ends = use.p == use.pages;
-      if (!ends && i < n_mine) continue;
+      if (!ends && use.left > 0) continue;
       // ---- the segment is done
       st.end();
       const float vs = pow2(max(st.vr, -118) - 8);
@@ -799,11 +857,20 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
           }
         if (lane == 0) {
           flags[slot][warp] = kHere | (ends ? kEnds : 0);
-          pairs[slot][warp] = make_int4(use.b, use.kvh, u0 + i - use.p, use.pages);
+          pairs[slot][warp] = make_int4(use.b, use.kvh, pos - use.p, use.pages);
         }
       }
-      if (ends && i < n_mine) next_pair(use);
       fresh = true;
+      if (!ends) break;
+      use.left -= pad;
+      pos += pad;
+      if (use.left <= 0) break;
+      const int b = use.b;
+      if (next_pair(use, use_next_keys)) {
+        keys = use.b == b + 1 ? use_next_keys : keys_of(use.b);
+        use_next_keys = keys_of(use.b + 1);
+      }
+      if (NT > 1 || use.b > b + 1) load_query(use.b, use.kvh);
     }
   }
   // requests without keys: zeros, by the CTAs in turn
@@ -894,10 +961,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
           l = l * keep + warp_sum(has ? w * x.y : 0.f);
           o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
 #pragma unroll
-          for (int j = 0; j < kBlock; ++j) {
-            const float wj = __shfl_sync(0xffffffffu, w, j);
-            if (i0 + j < n) add_scaled(o, wj, y[j]);
-          }
+          for (int j = 0; j < kBlock; ++j)  // behind the last partial: its row again, weight 0
+            add_scaled(o, __shfl_sync(0xffffffffu, w, j), y[j]);
         }
         if (whole) {
           const float inv = inverse(l);

@@ -695,7 +695,7 @@ torch::Tensor decode_attention_kv8(torch::Tensor q, torch::Tensor kv, torch::Ten
   check_lens(kv_len);
   TORCH_CHECK(kv_len.numel() == B, "kv_len must be int32 [B]");
   check_table(block_table, "block_table", B);
-  TORCH_CHECK(B * nkv * std::max<int64_t>(1, block_table.size(1)) < (int64_t)1 << 30, "decode: too many pages");
+  TORCH_CHECK(B * nkv * (block_table.size(1) + 4) < (int64_t)1 << 30, "decode: too many pages");
   check_devices({{"q", &q}, {"k_cache", &kv}, {"k_cache exps", &ke}, {"v_cache", &vv}, {"v_cache exps", &ve},
                  {"out", out_opt ? &*out_opt : nullptr}, {"kv_len", &kv_len}, {"block_table", &block_table}});
   const at::cuda::CUDAGuard guard(q.device());
