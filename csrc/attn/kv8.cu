@@ -84,76 +84,187 @@ struct AppendArgs {
   int max_pos, nq, nkv;
 };
 
-// One warp per (token, head of [q | k | v]). Lane l holds dims 2l, 2l + 1 and
-// their rotation partners 2l + 64, 2l + 65. k is normalised and rotated in 64
-// bits, so that the stored byte is the one of the real number.
-__global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int heads = a.nq + 2 * a.nkv;
-  const int64_t task = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (task >= a.T * heads) return;
-  const int64_t t = task / heads;
-  const int h = (int)(task % heads);
-  const int j = 2 * lane;
-  const __nv_bfloat16* src = a.qkv + task * D;
-  float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src + j));
-  float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src + 64 + j));
-  const int p = min(max(a.pos[t], 0), a.max_pos - 1);
-  const float* cs = a.cos_sin + (int64_t)p * D;
-  const float c0 = cs[j], c1 = cs[j + 1], s0 = cs[64 + j], s1 = cs[64 + j + 1];
-  if (h < a.nq) {
-    if (a.q_norm != nullptr) {
-      const float r = rsqrtf(warp_sum(x.x * x.x + x.y * x.y + y.x * y.x + y.y * y.y) * (1.f / D) + (float)a.eps);
-      x.x = x.x * r * __bfloat162float(a.q_norm[j]);
-      x.y = x.y * r * __bfloat162float(a.q_norm[j + 1]);
-      y.x = y.x * r * __bfloat162float(a.q_norm[64 + j]);
-      y.y = y.y * r * __bfloat162float(a.q_norm[64 + j + 1]);
-    }
-    __nv_bfloat16* dst = a.q_out + (t * a.nq + h) * D;
-    *reinterpret_cast<__nv_bfloat162*>(dst + j) = __floats2bfloat162_rn(x.x * c0 - y.x * s0, x.y * c1 - y.y * s1);
-    *reinterpret_cast<__nv_bfloat162*>(dst + 64 + j) = __floats2bfloat162_rn(y.x * c0 + x.x * s0, y.y * c1 + x.y * s1);
-    return;
+// A row (one head of one token) takes eight lanes: lane i of them holds dims 8i
+// .. 8i + 7 and their rotation partners 8i + 64 .. 8i + 71, two 16-byte loads,
+// so a warp streams four rows at once and a row's maximum is three shuffles.
+struct Row {
+  uint4 lo, hi;
+  MBX_DEVICE void load(const __nv_bfloat16* src, int i) {
+    lo = ld_v4(src + 8 * i);
+    hi = ld_v4(src + 64 + 8 * i);
   }
-  const int64_t slot = a.slots[t];
-  if (slot < 0 || slot >= a.n_slots) return;
-  // a slot that a later token names as well holds that token's row
-  bool later = false;
-  for (int64_t u = t + 1 + lane; u < a.T; u += 32) later |= a.slots[u] == slot;
-  if (__any_sync(0xffffffffu, later)) return;
-  const bool is_k = h < a.nq + a.nkv;
-  const int kh = is_k ? h - a.nq : h - a.nq - a.nkv;
-  float v[4] = {x.x, x.y, y.x, y.y};
-  if (is_k) {
-    double d[4] = {x.x, x.y, y.x, y.y};
-    if (a.k_norm != nullptr) {
-      double ss = d[0] * d[0] + d[1] * d[1] + d[2] * d[2] + d[3] * d[3];
+};
+struct Angles {
+  float c[8], s[8];
+  MBX_DEVICE void load(const float* cs, int i) {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const double r = 1.0 / sqrt(ss * (1.0 / D) + a.eps);
-      d[0] *= r * __bfloat162float(a.k_norm[j]);
-      d[1] *= r * __bfloat162float(a.k_norm[j + 1]);
-      d[2] *= r * __bfloat162float(a.k_norm[64 + j]);
-      d[3] *= r * __bfloat162float(a.k_norm[64 + j + 1]);
+    for (int k = 0; k < 2; ++k) {
+      const float4 x = *reinterpret_cast<const float4*>(cs + 8 * i + 4 * k);
+      const float4 y = *reinterpret_cast<const float4*>(cs + 64 + 8 * i + 4 * k);
+      c[4 * k] = x.x, c[4 * k + 1] = x.y, c[4 * k + 2] = x.z, c[4 * k + 3] = x.w;
+      s[4 * k] = y.x, s[4 * k + 1] = y.y, s[4 * k + 2] = y.z, s[4 * k + 3] = y.w;
     }
-    v[0] = round_to_odd(d[0] * c0 - d[2] * s0);
-    v[1] = round_to_odd(d[1] * c1 - d[3] * s1);
-    v[2] = round_to_odd(d[2] * c0 + d[0] * s0);
-    v[3] = round_to_odd(d[3] * c1 + d[1] * s1);
   }
-  float top = fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])), fmaxf(finite_abs(v[2]), finite_abs(v[3])));
+};
+template <typename F>
+MBX_DEVICE F eighth_sum(F v) {  // over a row's eight lanes
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// A row rounded into the cache, at dst and *exp.
+MBX_DEVICE void store_e4m3(const float (&x)[8], const float (&y)[8], uint8_t* dst, uint8_t* exp, int i, bool keep) {
+  float top = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = fmaxf(top, fmaxf(finite_abs(x[k]), finite_abs(y[k])));
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const int e = row_exp(top);
   const float inv = pow2(-e);
-  const int64_t blk = slot / PAGE;
-  const int off = (int)(slot % PAGE);
-  uint8_t* dst = (is_k ? a.kv : a.vv) + ((blk * a.nkv + kh) * PAGE + off) * D;
-  *reinterpret_cast<uint16_t*>(dst + j) = (uint16_t)e4m3x2(v[0] * inv, v[1] * inv);
-  *reinterpret_cast<uint16_t*>(dst + 64 + j) = (uint16_t)e4m3x2(v[2] * inv, v[3] * inv);
-  if (lane == 0) {
-    if (is_k) a.ke[blk * a.ke_sb + kh * a.ke_sh + off] = (uint8_t)(e + 127);
-    else a.ve[blk * a.ve_sb + kh * a.ve_sh + off] = (uint8_t)(e + 127);
+  uint2 lo, hi;
+  lo.x = e4m3x2(x[0] * inv, x[1] * inv) | e4m3x2(x[2] * inv, x[3] * inv) << 16;
+  lo.y = e4m3x2(x[4] * inv, x[5] * inv) | e4m3x2(x[6] * inv, x[7] * inv) << 16;
+  hi.x = e4m3x2(y[0] * inv, y[1] * inv) | e4m3x2(y[2] * inv, y[3] * inv) << 16;
+  hi.y = e4m3x2(y[4] * inv, y[5] * inv) | e4m3x2(y[6] * inv, y[7] * inv) << 16;
+  if (!keep) return;
+  *reinterpret_cast<uint2*>(dst + 8 * i) = lo;
+  *reinterpret_cast<uint2*>(dst + 64 + 8 * i) = hi;
+  if (i == 0) *exp = (uint8_t)(e + 127);
+}
+
+constexpr int kAppendWarps = 8;
+constexpr int kMaxTokens = 32;  // of a CTA that writes k and v
+
+// CTAs 0 .. kv_ctas - 1 write k and v of `tokens` tokens each, the others rotate
+// q: a warp takes `passes` times four heads of one token, whose angles it loads
+// once. k is normalised and rotated in 64 bits, so that the stored byte is the
+// one of the real number: two fp32 products and a sum would land on the other
+// side of a rounding border now and then.
+template <bool kNorm>
+__global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(AppendArgs a, int kv_ctas, int tokens, int passes) {
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane >> 3, i = lane & 7;
+  const int heads = a.nq + 2 * a.nkv;
+  auto angles_at = [&](int64_t t) { return a.cos_sin + (int64_t)min(max(a.pos[t], 0), a.max_pos - 1) * D; };
+  if ((int)blockIdx.x >= kv_ctas) {
+    const int per = (a.nq + 4 * passes - 1) / (4 * passes);  // tasks per token
+    const int64_t task = (int64_t)(blockIdx.x - kv_ctas) * kAppendWarps + warp;
+    const int64_t t = task / per;
+    if (t >= a.T) return;
+    const int h0 = (int)(task % per) * 4 * passes + sub;
+    const __nv_bfloat16* src = a.qkv + t * heads * D;
+    Row row;
+    row.load(src + (int64_t)min(h0, a.nq - 1) * D, i);
+    Angles g;
+    g.load(angles_at(t), i);
+#pragma unroll 1
+    for (int p = 0; p < passes; ++p) {
+      const int h = h0 + 4 * p;
+      float x[8] = {}, y[8] = {};
+      unpack_add<__nv_bfloat16>(row.lo, x);
+      unpack_add<__nv_bfloat16>(row.hi, y);
+      if (p + 1 < passes) row.load(src + (int64_t)min(h + 4, a.nq - 1) * D, i);
+      if (kNorm) {
+        float ss = 0.f, w[8] = {}, v[8] = {};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) ss += x[k] * x[k] + y[k] * y[k];
+        const float r = rsqrtf(eighth_sum(ss) * (1.f / D) + (float)a.eps);
+        unpack_add<__nv_bfloat16>(ld_v4(a.q_norm + 8 * i), w);
+        unpack_add<__nv_bfloat16>(ld_v4(a.q_norm + 64 + 8 * i), v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          x[k] = x[k] * r * w[k];
+          y[k] = y[k] * r * v[k];
+        }
+      }
+      float u[8], v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        u[k] = x[k] * g.c[k] - y[k] * g.s[k];
+        v[k] = y[k] * g.c[k] + x[k] * g.s[k];
+      }
+      if (h < a.nq) {
+        __nv_bfloat16* dst = a.q_out + (t * a.nq + h) * D;
+        *reinterpret_cast<uint4*>(dst + 8 * i) = pack_from<__nv_bfloat16>(u);
+        *reinterpret_cast<uint4*>(dst + 64 + 8 * i) = pack_from<__nv_bfloat16>(v);
+      }
+    }
+    return;
+  }
+  __shared__ int64_t slot_of[kMaxTokens];
+  __shared__ int taken[kMaxTokens];  // the slot is a later token's as well, which is stored instead
+  const int64_t t0 = (int64_t)blockIdx.x * tokens;
+  const int n = (int)min((int64_t)tokens, a.T - t0);
+  const int rows = n * 2 * a.nkv;  // token by token: its k heads, its v heads
+  // four rows a warp and pass; what lies behind the last row repeats it unstored
+  auto place = [&](int r, int& j, int& h) {
+    const int x = min(r, rows - 1);
+    j = x / (2 * a.nkv);
+    h = x - j * 2 * a.nkv;
+  };
+  int j, h, r = warp * 4 + sub;
+  place(r, j, h);
+  Row row;
+  row.load(a.qkv + ((t0 + j) * heads + a.nq + h) * D, i);
+  if ((int)threadIdx.x < n) {
+    const int64_t s = a.slots[t0 + threadIdx.x];
+    slot_of[threadIdx.x] = s >= 0 && s < a.n_slots ? s : -1;
+    taken[threadIdx.x] = 0;
+  }
+  __syncthreads();
+  if (t0 + 1 < a.T) {
+    int64_t lo = slot_of[0], hi = lo;
+    for (int k = 1; k < n; ++k) {
+      lo = min(lo, slot_of[k]);
+      hi = max(hi, slot_of[k]);
+    }
+    for (int64_t u = t0 + 1 + threadIdx.x; u < a.T; u += blockDim.x) {
+      const int64_t s = a.slots[u];
+      if (s < lo || s > hi || s < 0) continue;
+      for (int k = 0; k < n; ++k)
+        if (slot_of[k] == s && u > t0 + k) taken[k] = 1;
+    }
+    __syncthreads();
+  }
+#pragma unroll 1
+  for (int r0 = 0; r0 < rows; r0 += kAppendWarps * 4) {
+    const int64_t t = t0 + j, slot = slot_of[j];
+    const bool keep = r0 + r < rows && slot >= 0 && !taken[j];
+    const bool is_k = h < a.nkv;
+    const int kh = is_k ? h : h - a.nkv;
+    float x[8] = {}, y[8] = {};
+    unpack_add<__nv_bfloat16>(row.lo, x);
+    unpack_add<__nv_bfloat16>(row.hi, y);
+    if (r0 + kAppendWarps * 4 < rows) {
+      place(r0 + kAppendWarps * 4 + r, j, h);
+      row.load(a.qkv + ((t0 + j) * heads + a.nq + h) * D, i);
+    }
+    if (__any_sync(0xffffffffu, is_k)) {
+      Angles g;
+      g.load(angles_at(t), i);
+      double rs = 1.0;
+      float w[8] = {}, v[8] = {};
+      if (kNorm) {
+        double ss = 0.0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) ss += (double)x[k] * x[k] + (double)y[k] * y[k];
+        rs = 1.0 / sqrt(eighth_sum(ss) * (1.0 / D) + a.eps);
+        unpack_add<__nv_bfloat16>(ld_v4(a.k_norm + 8 * i), w);
+        unpack_add<__nv_bfloat16>(ld_v4(a.k_norm + 64 + 8 * i), v);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const double p = kNorm ? rs * w[k] * x[k] : (double)x[k], q = kNorm ? rs * v[k] * y[k] : (double)y[k];
+        const float px = round_to_odd(p * g.c[k] - q * g.s[k]), py = round_to_odd(q * g.c[k] + p * g.s[k]);
+        x[k] = is_k ? px : x[k];
+        y[k] = is_k ? py : y[k];
+      }
+    }
+    const int64_t blk = slot / PAGE;
+    const int off = (int)(slot % PAGE);
+    store_e4m3(x, y, (is_k ? a.kv : a.vv) + ((blk * a.nkv + kh) * PAGE + off) * D,
+               is_k ? a.ke + blk * a.ke_sb + kh * a.ke_sh + off : a.ve + blk * a.ve_sb + kh * a.ve_sh + off, i, keep);
   }
 }
 
@@ -170,7 +281,7 @@ struct ReadArgs {
   int max_blocks, nkv, num_blocks;
 };
 
-// 16 e4m3 numbers to bf16, times 2^e (exact).
+// 16 e4m3 numbers to bf16, times 2^e (exact), one 32-byte store.
 MBX_DEVICE void emit16(const uint4& w, float scale, __nv_bfloat16* dst) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
   float f[16];
@@ -181,35 +292,48 @@ MBX_DEVICE void emit16(const uint4& w, float scale, __nv_bfloat16* dst) {
     f[2 * i] = p.x * scale;
     f[2 * i + 1] = p.y * scale;
   }
-  *reinterpret_cast<uint4*>(dst) = pack_from<__nv_bfloat16>(f);
-  *reinterpret_cast<uint4*>(dst + 8) = pack_from<__nv_bfloat16>(f + 8);
+  const uint4 a = pack_from<__nv_bfloat16>(f), b = pack_from<__nv_bfloat16>(f + 8);
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w),
+               "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
 }
 
-// One block of 128 threads per (page, kv head, request): a thread per 16
-// elements. Rows behind the length are written as zeros, so that whatever
-// reads whole pages never meets what an earlier user of the page left there.
-__global__ void __launch_bounds__(128) read_pages_kernel(ReadArgs a) {
+// One warp per (page, kv head): ten loads in flight a lane, lane l the 16
+// elements of row l / 8 (of four at a time) from 16 (l % 8). Rows behind the
+// length are written as zeros, so that whatever reads whole pages never meets
+// what an earlier user of the page left there.
+constexpr int kReadWarps = 8;
+__global__ void __launch_bounds__(kReadWarps * 32) read_pages_kernel(ReadArgs a, int tasks) {
   pdl_wait();
-  const int i = blockIdx.x, h = blockIdx.y, r = blockIdx.z;
+  const int task = blockIdx.x * kReadWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (task >= tasks) return;
+  const int page = task / a.nkv, h = task - page * a.nkv;
+  const int r = page / a.max_blocks, i = page - r * a.max_blocks;
   const int L = a.kv_len[r];
-  if (i * PAGE >= L) return;
   const int blk = a.block_table[r * a.bt_s + i];
-  const int64_t to = a.out_table ? a.out_table[r * a.ot_s + i] : (int64_t)r * a.max_blocks + i;
-  if (to < 0 || to >= a.out_pages) return;
-  const int row = threadIdx.x >> 3;
-  const bool live = i * PAGE + row < L && blk >= 0 && blk < a.num_blocks;
-  const int64_t src = live ? ((int64_t)blk * a.nkv + h) * PAGE * D + threadIdx.x * 16 : 0;
-  const int64_t dst = (to * a.nkv + h) * PAGE * D + threadIdx.x * 16;
-  uint4 k = make_uint4(0, 0, 0, 0), v = k;
-  float ks = 0.f, vs = 0.f;
-  if (live) {
-    k = ld_v4(a.kv + src);
-    v = ld_v4(a.vv + src);
-    ks = __uint_as_float((uint32_t)a.ke[blk * a.ke_sb + h * a.ke_sh + row] << 23);
-    vs = __uint_as_float((uint32_t)a.ve[blk * a.ve_sb + h * a.ve_sh + row] << 23);
+  const int64_t to = a.out_table ? a.out_table[r * a.ot_s + i] : page;
+  if (i * PAGE >= L || to < 0 || to >= a.out_pages) return;
+  const int live = blk >= 0 && blk < a.num_blocks ? L - i * PAGE : 0;  // rows that count
+  const int64_t src = live > 0 ? ((int64_t)blk * a.nkv + h) * PAGE * D + lane * 16 : 0;
+  const uint4 ke = live > 0 ? ld_v4(a.ke + blk * a.ke_sb + h * a.ke_sh) : make_uint4(0, 0, 0, 0);
+  const uint4 ve = live > 0 ? ld_v4(a.ve + blk * a.ve_sb + h * a.ve_sh) : make_uint4(0, 0, 0, 0);
+  uint4 k[4], v[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const bool on = c * 4 + (lane >> 3) < live;
+    k[c] = on ? ld_v4(a.kv + src + c * 512) : make_uint4(0, 0, 0, 0);
+    v[c] = on ? ld_v4(a.vv + src + c * 512) : make_uint4(0, 0, 0, 0);
   }
-  emit16(k, ks, a.k_out + dst);
-  emit16(v, vs, a.v_out + dst);
+  const int64_t dst = (to * a.nkv + h) * PAGE * D + lane * 16;
+  const uint32_t kw[4] = {ke.x, ke.y, ke.z, ke.w}, vw[4] = {ve.x, ve.y, ve.z, ve.w};
+  const int byte = (lane >> 3) * 8;
+  auto scale = [&](uint32_t w, int c) {
+    return c * 4 + (lane >> 3) < live ? __uint_as_float(((w >> byte) & 0xffu) << 23) : 0.f;
+  };
+#pragma unroll
+  for (int c = 0; c < 4; ++c) emit16(k[c], scale(kw[c], c), a.k_out + dst + c * 512);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) emit16(v[c], scale(vw[c], c), a.v_out + dst + c * 512);
 }
 
 // ---------------------------------------------------------------- decode
@@ -1030,8 +1154,17 @@ void rope_and_cache_kv8_launch(const void* qkv, const int* pos, const float* cos
   a.max_pos = (int)max_pos;
   a.nq = nq;
   a.nkv = nkv;
-  const int64_t tasks = T * (nq + 2 * nkv);
-  launch_k(append_kernel, dim3((unsigned)((tasks + 3) / 4)), dim3(128), 0, s, a);
+  // Tokens per k/v CTA: one where there are few; more for many, since every CTA
+  // looks through all later slots for its own.
+  const int tokens = T <= 128 ? 1 : (int)std::min<int64_t>(kMaxTokens, std::max<int64_t>(4, (T + 1023) / 1024));
+  const int passes = T * nq >= 16384 ? 2 : 1;
+  const int64_t kv_ctas = (T + tokens - 1) / tokens;
+  const int64_t q_tasks = T * ((nq + 4 * passes - 1) / (4 * passes));
+  const dim3 grid((unsigned)(kv_ctas + (q_tasks + kAppendWarps - 1) / kAppendWarps));
+  if (q_norm != nullptr)
+    launch_k(append_kernel<true>, grid, dim3(kAppendWarps * 32), 0, s, a, (int)kv_ctas, tokens, passes);
+  else
+    launch_k(append_kernel<false>, grid, dim3(kAppendWarps * 32), 0, s, a, (int)kv_ctas, tokens, passes);
   MBX_CUDA_CHECK(cudaGetLastError());
 }
 
@@ -1042,7 +1175,8 @@ void read_pages_kv8_launch(const Kv8Cache& c, int nkv, const int* block_table, i
   ReadArgs a{c.kv, c.vv, c.ke, c.ve, c.ke_sb, c.ke_sh, c.ve_sb, c.ve_sh, block_table, out_table, kv_len,
              bt_stride, ot_stride, static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), out_pages,
              max_blocks, nkv, (int)c.blocks};
-  launch_k(read_pages_kernel, dim3(max_blocks, nkv, R), dim3(128), 0, s, a);
+  const int tasks = R * max_blocks * nkv;
+  launch_k(read_pages_kernel, dim3((tasks + kReadWarps - 1) / kReadWarps), dim3(kReadWarps * 32), 0, s, a, tasks);
   MBX_CUDA_CHECK(cudaGetLastError());
 }
 

@@ -1,0 +1,1095 @@
+// The paged KV cache in 8 bits: writing it, reading it back, and attention of
+// one new token per request over it (head_dim 128, pages of 16 tokens).
+//
+// A cached row x (one token, one kv head) is held as e4m3 numbers with one
+// power-of-two scale:
+//   e = the smallest integer with max|x_i| <= 448 * 2^e, at least -117
+//   values_i = round_to_nearest_even_e4m3(x_i / 2^e),  exps = e + 127
+// and stands for values_i * 2^e. e4m3 is a floating format, so a scale finer
+// than a power of two would buy at most one exponent of range and no
+// accuracy, while a power of two makes every scaling exact: a stored row is
+// exact in bf16 and in fp32 products, and which e4m3 number a value rounds to
+// does not depend on a division. Elements that are not finite are stored as
+// NaN and do not take part in the maximum.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+
+#include "../common.cuh"
+#include "../kernels.h"
+
+namespace mbx {
+namespace {
+
+constexpr int D = 128;
+constexpr int PAGE = 16;
+constexpr int kMinExp = -117;  // 2^-9 * 2^-117 = 2^-126: every stored number is a normal fp32 / bf16 number or zero
+
+// A row's exponent from the largest magnitude of its finite elements (fp32):
+// 448 = 1.75 * 2^8.
+MBX_DEVICE int row_exp(float top) {
+  const uint32_t b = __float_as_uint(top);
+  const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return max(e, kMinExp);
+}
+
+// 2^e for e in [-126, 127].
+MBX_DEVICE float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Two e4m3 numbers from lo and hi (lo in the low byte); what is not finite becomes NaN.
+MBX_DEVICE uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  const float nan = __uint_as_float(0x7fffffffu);
+  lo = fabsf(lo) <= 3.4e38f ? lo : nan;
+  hi = fabsf(hi) <= 3.4e38f ? hi : nan;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// e4m3 x 2 (the low or high half of w) to f16 x 2, exact.
+MBX_DEVICE uint32_t f16x2_of(uint32_t w, int half) {
+  uint32_t r;
+  const uint16_t h = (uint16_t)(half ? w >> 16 : w);
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(h));
+  return r;
+}
+
+// The fp32 number whose further rounding to fewer bits (22 or less) equals
+// rounding x itself: x cut to 24 bits, the last one set if anything was cut.
+MBX_DEVICE float round_to_odd(double x) {
+  const float f = __double2float_rz(x);
+  return (double)f != x ? __uint_as_float(__float_as_uint(f) | 1u) : f;
+}
+
+MBX_DEVICE float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= 3.4e38f ? a : 0.f;
+}
+
+// ---------------------------------------------------------------- append
+struct AppendArgs {
+  const __nv_bfloat16* qkv;  // [T, (nq + 2 nkv) * D]
+  const int* pos;            // [T]
+  const float* cos_sin;      // [max_pos, D]: cos(64) | sin(64)
+  const int64_t* slots;      // [T]: block * PAGE + offset; negative or past the cache: not written
+  __nv_bfloat16* q_out;      // [T, nq, D]
+  uint8_t *kv, *vv;          // [blocks, nkv, PAGE, D] e4m3
+  uint8_t *ke, *ve;          // [blocks, nkv, PAGE], row strides below
+  int64_t ke_sb, ke_sh, ve_sb, ve_sh;
+  const __nv_bfloat16 *q_norm, *k_norm;  // [D] or nullptr
+  double eps;
+  int64_t T, n_slots;
+  int max_pos, nq, nkv;
+};
+
+// One warp per (token, head of [q | k | v]). Lane l holds dims 2l, 2l + 1 and
+// their rotation partners 2l + 64, 2l + 65. k is normalised and rotated in 64
+// bits, so that the stored byte is the one of the real number.
+__global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int heads = a.nq + 2 * a.nkv;
+  const int64_t task = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (task >= a.T * heads) return;
+  const int64_t t = task / heads;
+  const int h = (int)(task % heads);
+  const int j = 2 * lane;
+  const __nv_bfloat16* src = a.qkv + task * D;
+  float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src + j));
+  float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src + 64 + j));
+  const int p = min(max(a.pos[t], 0), a.max_pos - 1);
+  const float* cs = a.cos_sin + (int64_t)p * D;
+  const float c0 = cs[j], c1 = cs[j + 1], s0 = cs[64 + j], s1 = cs[64 + j + 1];
+  if (h < a.nq) {
+    if (a.q_norm != nullptr) {
+      const float r = rsqrtf(warp_sum(x.x * x.x + x.y * x.y + y.x * y.x + y.y * y.y) * (1.f / D) + (float)a.eps);
+      x.x = x.x * r * __bfloat162float(a.q_norm[j]);
+      x.y = x.y * r * __bfloat162float(a.q_norm[j + 1]);
+      y.x = y.x * r * __bfloat162float(a.q_norm[64 + j]);
+      y.y = y.y * r * __bfloat162float(a.q_norm[64 + j + 1]);
+    }
+    __nv_bfloat16* dst = a.q_out + (t * a.nq + h) * D;
+    *reinterpret_cast<__nv_bfloat162*>(dst + j) = __floats2bfloat162_rn(x.x * c0 - y.x * s0, x.y * c1 - y.y * s1);
+    *reinterpret_cast<__nv_bfloat162*>(dst + 64 + j) = __floats2bfloat162_rn(y.x * c0 + x.x * s0, y.y * c1 + x.y * s1);
+    return;
+  }
+  const int64_t slot = a.slots[t];
+  if (slot < 0 || slot >= a.n_slots) return;
+  // a slot that a later token names as well holds that token's row
+  bool later = false;
+  for (int64_t u = t + 1 + lane; u < a.T; u += 32) later |= a.slots[u] == slot;
+  if (__any_sync(0xffffffffu, later)) return;
+  const bool is_k = h < a.nq + a.nkv;
+  const int kh = is_k ? h - a.nq : h - a.nq - a.nkv;
+  float v[4] = {x.x, x.y, y.x, y.y};
+  if (is_k) {
+    double d[4] = {x.x, x.y, y.x, y.y};
+    if (a.k_norm != nullptr) {
+      double ss = d[0] * d[0] + d[1] * d[1] + d[2] * d[2] + d[3] * d[3];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const double r = 1.0 / sqrt(ss * (1.0 / D) + a.eps);
+      d[0] *= r * __bfloat162float(a.k_norm[j]);
+      d[1] *= r * __bfloat162float(a.k_norm[j + 1]);
+      d[2] *= r * __bfloat162float(a.k_norm[64 + j]);
+      d[3] *= r * __bfloat162float(a.k_norm[64 + j + 1]);
+    }
+    v[0] = round_to_odd(d[0] * c0 - d[2] * s0);
+    v[1] = round_to_odd(d[1] * c1 - d[3] * s1);
+    v[2] = round_to_odd(d[2] * c0 + d[0] * s0);
+    v[3] = round_to_odd(d[3] * c1 + d[1] * s1);
+  }
+  float top = fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])), fmaxf(finite_abs(v[2]), finite_abs(v[3])));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const int e = row_exp(top);
+  const float inv = pow2(-e);
+  const int64_t blk = slot / PAGE;
+  const int off = (int)(slot % PAGE);
+  uint8_t* dst = (is_k ? a.kv : a.vv) + ((blk * a.nkv + kh) * PAGE + off) * D;
+  *reinterpret_cast<uint16_t*>(dst + j) = (uint16_t)e4m3x2(v[0] * inv, v[1] * inv);
+  *reinterpret_cast<uint16_t*>(dst + 64 + j) = (uint16_t)e4m3x2(v[2] * inv, v[3] * inv);
+  if (lane == 0) {
+    if (is_k) a.ke[blk * a.ke_sb + kh * a.ke_sh + off] = (uint8_t)(e + 127);
+    else a.ve[blk * a.ve_sb + kh * a.ve_sh + off] = (uint8_t)(e + 127);
+  }
+}
+
+// ---------------------------------------------------------------- read
+struct ReadArgs {
+  const uint8_t *kv, *vv, *ke, *ve;
+  int64_t ke_sb, ke_sh, ve_sb, ve_sh;
+  const int* block_table;  // [R, max_blocks], row stride bt_s
+  const int* out_table;    // [R, max_blocks], row stride ot_s, or nullptr (page i of request r at r * max_blocks + i)
+  const int* kv_len;       // [R]
+  int64_t bt_s, ot_s;
+  __nv_bfloat16 *k_out, *v_out;  // [out_pages, nkv, PAGE, D]
+  int64_t out_pages;
+  int max_blocks, nkv, num_blocks;
+};
+
+// 16 e4m3 numbers to bf16, times 2^e (exact).
+MBX_DEVICE void emit16(const uint4& w, float scale, __nv_bfloat16* dst) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  float f[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t h = f16x2_of(u[i >> 1], i & 1);
+    const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    f[2 * i] = p.x * scale;
+    f[2 * i + 1] = p.y * scale;
+  }
+  *reinterpret_cast<uint4*>(dst) = pack_from<__nv_bfloat16>(f);
+  *reinterpret_cast<uint4*>(dst + 8) = pack_from<__nv_bfloat16>(f + 8);
+}
+
+// One block of 128 threads per (page, kv head, request): a thread per 16
+// elements. Rows behind the length are written as zeros, so that whatever
+// reads whole pages never meets what an earlier user of the page left there.
+__global__ void __launch_bounds__(128) read_pages_kernel(ReadArgs a) {
+  pdl_wait();
+  const int i = blockIdx.x, h = blockIdx.y, r = blockIdx.z;
+  const int L = a.kv_len[r];
+  if (i * PAGE >= L) return;
+  const int blk = a.block_table[r * a.bt_s + i];
+  const int64_t to = a.out_table ? a.out_table[r * a.ot_s + i] : (int64_t)r * a.max_blocks + i;
+  if (to < 0 || to >= a.out_pages) return;
+  const int row = threadIdx.x >> 3;
+  const bool live = i * PAGE + row < L && blk >= 0 && blk < a.num_blocks;
+  const int64_t src = live ? ((int64_t)blk * a.nkv + h) * PAGE * D + threadIdx.x * 16 : 0;
+  const int64_t dst = (to * a.nkv + h) * PAGE * D + threadIdx.x * 16;
+  uint4 k = make_uint4(0, 0, 0, 0), v = k;
+  float ks = 0.f, vs = 0.f;
+  if (live) {
+    k = ld_v4(a.kv + src);
+    v = ld_v4(a.vv + src);
+    ks = __uint_as_float((uint32_t)a.ke[blk * a.ke_sb + h * a.ke_sh + row] << 23);
+    vs = __uint_as_float((uint32_t)a.ve[blk * a.ve_sb + h * a.ve_sh + row] << 23);
+  }
+  emit16(k, ks, a.k_out + dst);
+  emit16(v, vs, a.v_out + dst);
+}
+
+// ---------------------------------------------------------------- decode
+// Attention of one query row per request. The G = nq / nkv query heads that
+// share a kv head are the columns of the tensor-core tiles: per page of 16
+// keys, S^T = K Q^T (16 keys x 8 heads) and O^T += V^T P^T (128 dims x 8
+// heads) as m16n8k16 f16 MMAs with fp32 sums.
+//  * e4m3 is exact in f16, and the order of the contracted dimension is free:
+//    lane (g, t) = (lane / 4, lane % 4) of a K fragment takes 16 contiguous
+//    bytes of its rows g and g + 8, and Q is laid out to match. V fragments
+//    pair two keys per register; a lane takes the same 16 dims of four keys
+//    and pairs them with byte permutes.
+//  * q is scaled per head by a power of two to [2^14, 2^15) before it becomes
+//    f16: elements down to 2^-28 of the head's largest keep all their bits.
+//  * softmax in base 2 with a running maximum m. The value exponents join the
+//    weights: w = 2^(s - m) * 2^(ve - vr + 8) in f16 with vr a running maximum
+//    of ve, so weights down to 2^-22 of the largest keep 11 bits (bf16 would
+//    keep 8). m and vr only move when a page exceeds them by more than 2^4 and
+//    2^3: then w <= 2^15 stays inside f16. The row sum uses the fp32 weights.
+MBX_DEVICE float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+MBX_DEVICE void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+MBX_DEVICE uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+MBX_DEVICE uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ long long g_trace[148*16];
+#define TR(i) do { if ((threadIdx.x & 31) == 0 && (threadIdx.x>>5)==0) { long long t_; asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t_)); g_trace[blockIdx.x*16+(i)] = t_; } } while (0)
+struct Kv8DecodeArgs {
+  const __nv_bfloat16* q;  // [B, nq, D]
+  const uint8_t *kv, *vv, *ke, *ve;
+  int64_t ke_sb, ke_sh, ve_sb, ve_sh;
+  __nv_bfloat16* o;        // [B, nq, D]
+  float* part;             // partials of pairs that span CTAs [grid][2][heads][D], then their (m, l)
+  int* counters;           // [grid] arrivals, zero between launches
+  const int* kv_len;       // [B]
+  const int* block_table;  // [B, max_blocks], row stride bt_s
+  int64_t bt_s;
+  int B, max_blocks, num_blocks, nq, nkv;
+  float scale_log2;
+};
+
+constexpr int kNoExp = -1000;  // value exponent of a masked key, and vr before the first page
+
+// Where a fetched page's 16-byte chunks lie in shared memory. The reader of a
+// K chunk (row r, chunk c) is lane (g, t) = (r % 8, c % 4), of a V chunk lane
+// (c, r % 8 / 2), one of its four chunks each; the exclusive ors spread the
+// writes (8 chunks of a row at once) and the reads over all banks.
+MBX_DEVICE uint32_t k_place(int row, int ch) {
+  const int slot = (row >> 3) * 2 + (ch >> 2);
+  return slot * 512 + ((((row & 7) * 4 + (ch & 3)) ^ ((ch >> 2) << 2)) << 4);
+}
+MBX_DEVICE uint32_t v_place(int row, int ch) {
+  const int slot = (row >> 3) * 2 + (row & 1), t = (row & 7) >> 1;
+  return slot * 512 + ((t * 8 + (ch ^ (2 * t))) << 4);
+}
+
+// One warp's running state over the pages of one (request, kv head); NT tiles
+// of 8 query heads. Of tile n, lane (g, t) holds heads 8n + 2t and 8n + 2t + 1
+// at dims 16g..16g+15 (o[n][i][0], [2]: dims 16g + 2i, 16g + 2i + 1 of the
+// first head; [1], [3]: of the second).
+template <int NT>
+struct HeadState {
+  uint32_t qf[NT][8][2];
+  float qs[NT][2];  // softmax scale * log2(e) * the power of two taken out of q
+  float o[NT][8][4];
+  float m[NT][2], l[NT][2];  // l: this lane's keys only
+  int vr;
+
+  // This lane's elements of q [G, D] (heads behind G: zeros), in two steps, so
+  // that the loads can be issued ahead of their use.
+  struct Query {
+    uint4 w[NT][4];
+    MBX_DEVICE void load(const __nv_bfloat16* q, int G, int lane) {
+      const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          w[n][c] = n * 8 + g < G ? ld_v4(q + (n * 8 + g) * D + (t + 4 * (c >> 1)) * 16 + (c & 1) * 8)
+                                  : make_uint4(0, 0, 0, 0);
+    }
+  };
+  MBX_DEVICE void begin(const Query& q, float scale_log2, int lane) {
+    const int t = lane & 3;
+    vr = kNoExp;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float x[2][16];
+      float top = 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float f[8] = {};
+        unpack_add<__nv_bfloat16>(q.w[n][c], f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[c >> 1][(c & 1) * 8 + i] = f[i];
+          top = fmaxf(top, fabsf(f[i]));
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = max((int)(__float_as_uint(top) >> 23) - 127, -112);
+      const float up = pow2(14 - e);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        const float* f = &x[ks >> 2][(ks & 3) * 4];
+        qf[n][ks][0] = pack_f16(f[0] * up, f[1] * up);
+        qf[n][ks][1] = pack_f16(f[2] * up, f[3] * up);
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        qs[n][c] = scale_log2 * pow2(__shfl_sync(0xffffffffu, e, (2 * t + c) * 4) - 14);
+        m[n][c] = -INFINITY;
+        l[n][c] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    }
+  }
+
+  // P pages at once (independent chains of tensor-core work), as fetched into
+  // shared memory: K (k_place), V (v_place), then the exponents of the 16 keys
+  // and of the 16 values. A lane takes K rows g and g + 8, chunks t and t + 4,
+  // and chunk g of V's rows 2t, 2t + 1, 2t + 8, 2t + 9. Only a page's first
+  // live[p] keys count.
+  template <int P>
+  MBX_DEVICE void pages(const uint8_t* const (&src)[2], const int (&live)[2], int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    float s[P][NT][4], s2[P][NT][4];  // halves of the sum: a shorter chain
+    uint4 k[P][4];
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) k[p][c] = *reinterpret_cast<const uint4*>(src[p] + k_place(g + 8 * (c >> 1), t + 4 * (c & 1)));
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[p][n][i] = s2[p][n][i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const uint4 &w0 = k[p][ks >> 2], &w8 = k[p][2 + (ks >> 2)];
+        const uint32_t r0 = (ks & 3) == 0 ? w0.x : (ks & 3) == 1 ? w0.y : (ks & 3) == 2 ? w0.z : w0.w;
+        const uint32_t r8 = (ks & 3) == 0 ? w8.x : (ks & 3) == 1 ? w8.y : (ks & 3) == 2 ? w8.z : w8.w;
+        const uint32_t af[4] = {f16x2_of(r0, 0), f16x2_of(r8, 0), f16x2_of(r0, 1), f16x2_of(r8, 1)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16((ks & 1) ? s2[p][n] : s[p][n], af, qf[n][ks][0], qf[n][ks][1]);
+      }
+    int vx[P][2];
+    bool grow = false;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint8_t* e = src[p] + 4096 + g + 8 * r;
+        const bool on = g + 8 * r < live[p];
+        vx[p][r] = on ? (int)e[16] - 127 : kNoExp;
+        grow |= vx[p][r] > vr + 3;
+        const float kf = __uint_as_float((uint32_t)e[0] << 23);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float x = on ? (s[p][n][2 * r + c] + s2[p][n][2 * r + c]) * (kf * qs[n][c]) : -INFINITY;
+            s[p][n][2 * r + c] = x;
+            grow |= x > m[n][c] + 4.f;
+          }
+      }
+    if (__any_sync(0xffffffffu, grow)) {
+      int nv = vr;
+#pragma unroll
+      for (int p = 0; p < P; ++p) nv = max(nv, max(vx[p][0], vx[p][1]));
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) nv = max(nv, __shfl_xor_sync(0xffffffffu, nv, off));
+      const float vc = ex2((float)(vr - nv));
+      vr = nv;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float corr[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float nm = m[n][c];
+#pragma unroll
+          for (int p = 0; p < P; ++p) nm = fmaxf(nm, fmaxf(s[p][n][c], s[p][n][2 + c]));
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, off));
+          corr[c] = nm == -INFINITY ? 1.f : ex2(m[n][c] - nm);
+          m[n][c] = nm;
+          l[n][c] *= corr[c];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          o[n][i][0] *= corr[0] * vc;
+          o[n][i][1] *= corr[1] * vc;
+          o[n][i][2] *= corr[0] * vc;
+          o[n][i][3] *= corr[1] * vc;
+        }
+      }
+    }
+    uint32_t pf[P][NT][2];
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float vf = pow2(max(vx[p][r] - vr + 8, -126));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float w[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float x = ex2(s[p][n][2 * r + c] - (m[n][c] == -INFINITY ? 0.f : m[n][c]));
+            l[n][c] += x;
+            w[c] = x * vf;
+          }
+          pf[p][n][r] = transpose8x8(pack_f16(w[0], w[1]));
+        }
+      }
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      uint4 v[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[c] = *reinterpret_cast<const uint4*>(src[p] + 2048 + v_place(2 * t + (c & 1) + 8 * (c >> 1), g));
+      if (live[p] < PAGE) {  // rows behind the length may hold anything: 0 * NaN would not be 0
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (2 * t + (i & 1) + 8 * (i >> 1) >= live[p]) v[i] = make_uint4(0, 0, 0, 0);
+      }
+      const uint32_t vw[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w},
+                                 {v[1].x, v[1].y, v[1].z, v[1].w},
+                                 {v[2].x, v[2].y, v[2].z, v[2].w},
+                                 {v[3].x, v[3].y, v[3].z, v[3].w}};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
+        const uint32_t a01 = __byte_perm(vw[0][i >> 1], vw[1][i >> 1], sel);
+        const uint32_t a89 = __byte_perm(vw[2][i >> 1], vw[3][i >> 1], sel);
+        const uint32_t af[4] = {f16x2_of(a01, 0), f16x2_of(a01, 1), f16x2_of(a89, 0), f16x2_of(a89, 1)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16(o[n][i], af, pf[p][n][0], pf[p][n][1]);
+      }
+    }
+  }
+
+  MBX_DEVICE void end() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], off);
+  }
+};
+
+// ---- the work's division
+// The pages of all (request, kv head) pairs form one list, pairs one after
+// another; every warp of the grid takes an equal run of it, whatever the
+// lengths are (they live on the device, so a captured graph adapts too). A
+// pair's pages inside one warp's run are a segment of that warp:
+//   * a pair that lies in one warp's run is finished by the warp alone;
+//   * otherwise each warp leaves a partial state (m, l, O) in shared memory, and
+//     the CTA folds its warps' partials, in order, into the output or, for a
+//     pair that reaches into other CTAs, into one partial in global memory; the
+//     last of those CTAs to arrive folds these in CTA order.
+// All orders are fixed, so results do not depend on timing. At most one pair
+// enters a CTA's run and one leaves it, hence two global partials per CTA.
+constexpr int kWarps = 8;
+constexpr int kAlone = 8;          // pages a warp takes alone rather than share them and merge
+constexpr float kMergeCost = 1.f;  // see plan_work
+constexpr int kPad = 2;            // pages that a pair costs a warp besides its own, see plan_work
+constexpr int kStageBytes = 2 * PAGE * D + 64;  // K, V, 2 x 16 exponents
+constexpr int kRow = D + 4;                     // floats per head of a partial in shared memory (bank spread)
+
+template <int NT>
+constexpr int kStages = NT == 1 ? 5 : 4;
+
+// x / n for x / n below 2^20.
+MBX_DEVICE int quotient(int x, int n) {
+  int q = __float2int_rz(__fdividef((float)x, (float)n));
+  const int r = x - q * n;
+  return q + (r >= n) - (r < 0);
+}
+
+// How the work is cut. kList: runs of `run` entries of the list, in which every
+// pair is followed by `pad` empty ones. Where no pair is longer than a few
+// pages, sharing and merging it costs more than it saves: kWarp gives each warp
+// a pair, kCta each CTA one (its warps `run` pages each).
+enum Cut : int { kList, kWarp, kCta };
+struct WorkPlan {
+  int cut, run, pad;
+};
+// pages, some: of all requests together, and how many have any; top, low: the
+// longest and the shortest of those.
+MBX_DEVICE WorkPlan plan_work(int pages, int some, int top, int low, int pairs, int nkv, int grid, int warps) {
+  if (top <= kAlone && pairs <= grid * warps) return {kWarp, top, 0};
+  if (top <= kAlone * warps && pairs <= grid) return {kCta, (top + warps - 1) / warps, 0};
+  const int n = grid * warps;
+  int run = max(1, quotient(pages * nkv + n - 1, n));
+  // Beginning and ending a pair takes a warp about as long as two pages. Where
+  // runs can hold whole pairs, warps with many short ones would come late; where
+  // they cannot, empty entries would only move pairs off the runs' borders.
+  const int pad = low < run ? kPad : 0;
+  if (pad) run = max(1, quotient((pages + pad * some) * nkv + n - 1, n));
+  // with few pairs, one more CTA per pair costs its merge more than it saves
+  float root;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"((float)top));
+  return {kList, max(run, (int)(root * (kMergeCost / warps) + 0.999f)), pad};
+}
+
+template <int NT>
+struct DecodeSmem {
+  static constexpr int kHeads = 8 * NT;
+  static constexpr int kWarpBytes = kStages<NT> * kStageBytes;  // a warp's ring, then its last segment's partial
+  static constexpr int kPartBytes = kHeads * kRow * 4;
+  static constexpr int kPart = kWarps * kWarpBytes;             // [kWarps] partials of the warps' first segments
+  static constexpr int kMl = kPart + kWarps * kPartBytes;       // float2 [2][kWarps][kHeads]
+  static constexpr int kTotal = kMl + 2 * kWarps * kHeads * 8;
+  static_assert(kWarpBytes >= kPartBytes, "a partial fits in the ring");
+};
+
+MBX_DEVICE uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+MBX_DEVICE void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+MBX_DEVICE void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+MBX_DEVICE void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+MBX_DEVICE void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// What a warp left for the merge: of its first segment, where that began before
+// the warp's run (slot 0), and of its last, where that goes on behind it (slot
+// 1). kEnds: the pair's pages end in this warp's run.
+enum SegFlags : int { kHere = 1, kEnds = 2 };
+
+MBX_DEVICE float merge_weight(float m, float M) { return M == -INFINITY ? 0.f : ex2(m - M); }
+MBX_DEVICE float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+// 1 / l, or 0 for a row without keys. One unit in the last place of fp32 is
+// far below the bf16 rounding that follows.
+MBX_DEVICE float inverse(float l) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(l));
+  return l == 0.f ? 0.f : r;
+}
+// Loads of partials: shared memory, or global memory past L1 (other CTAs may
+// have written them).
+MBX_DEVICE float4 ld_partial4(const float* p) {
+  float4 v;
+  asm volatile("ld.volatile.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+MBX_DEVICE float2 ld_partial2(const float* p) {
+  float2 v;
+  asm volatile("ld.volatile.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p));
+  return v;
+}
+MBX_DEVICE void add_scaled(float4& o, float w, const float4& x) {
+  o.x += w * x.x;
+  o.y += w * x.y;
+  o.z += w * x.z;
+  o.w += w * x.w;
+}
+template <int NT>
+__global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArgs a) {
+  using S = DecodeSmem<NT>;
+  constexpr int kSt = kStages<NT>, kW = kWarps;
+  TR(0);
+  pdl_wait();
+  TR(1);
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int flags[2][kW];   // SegFlags
+  __shared__ int4 pairs[2][kW];  // of these segments: request, kv head, list index of the pair's first page, its pages
+  __shared__ int s_last[2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int G = a.nq / a.nkv;
+  const int max_keys = a.max_blocks * PAGE;
+  auto pages_of = [&](int b) { return b < a.B ? (min(max(a.kv_len[b], 0), max_keys) + PAGE - 1) / PAGE : 0; };
+  if (lane < 2) flags[lane][warp] = 0;
+  // ---- this warp's run of pages, and where it starts: every warp for itself.
+  // Lane c holds the pages of requests 32c .. 32c + 31 (of each 1024), and how
+  // many of them have any.
+  int total = 0, some = 0, top = 0, low = 1 << 30, sums = 0, counts = 0;
+#pragma unroll 1
+  for (int c0 = 0; c0 * 32 < a.B; ++c0) {
+    const int x = pages_of(c0 * 32 + lane);
+    const int sx = __reduce_add_sync(0xffffffffu, x), nx = __popc(__ballot_sync(0xffffffffu, x > 0));
+    total += sx;
+    some += nx;
+    top = max(top, x);
+    low = x > 0 ? min(low, x) : low;
+    if (lane == c0) sums = sx, counts = nx;
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  low = __reduce_min_sync(0xffffffffu, low);
+  const WorkPlan plan = plan_work(total, some, top, low, a.B * a.nkv, a.nkv, gridDim.x, kW);
+  const int run = plan.run, pad = plan.pad;
+  auto in_list = [&](int pages) { return pages > 0 ? pages + pad : 0; };
+  const int u0 = (blockIdx.x * kW + warp) * run;  // first page in the list
+  int left = 0;     // of the run (list entries)
+  int4 at = make_int4(0, 0, 0, 0);  // request, kv head, page and the pair's pages there
+  if (plan.cut == kList) {
+    sums += counts * pad;
+    left = max(0, min(run, (total + some * pad) * a.nkv - u0));
+    if (left > 0) {
+      auto scan = [&](int v) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, v, o);
+          if (lane >= o) v += x;
+        }
+        return v;
+      };
+      int before = 0, b0 = 0;  // pages of the requests in front; first of the 1024 looked at
+      int end = scan(sums);
+#pragma unroll 1
+      while (__shfl_sync(0xffffffffu, end, 31) * a.nkv <= u0) {
+        before = __shfl_sync(0xffffffffu, end, 31);
+        b0 += 1024;
+        sums = 0;
+#pragma unroll 1
+        for (int c = 0; c < 32; ++c) {
+          const int x = __reduce_add_sync(0xffffffffu, in_list(pages_of(b0 + c * 32 + lane)));
+          if (lane == c) sums = x;
+        }
+        end = before + scan(sums);
+      }
+      const int c = __popc(__ballot_sync(0xffffffffu, end * a.nkv <= u0));
+      before = __shfl_sync(0xffffffffu, end - sums, c);
+      const int n = in_list(pages_of(b0 + c * 32 + lane));
+      end = before + scan(n);
+      const int r = __popc(__ballot_sync(0xffffffffu, end * a.nkv <= u0));
+      at.x = b0 + c * 32 + r;
+      const int len = __shfl_sync(0xffffffffu, n, r);
+      const int off = u0 - __shfl_sync(0xffffffffu, end - n, r) * a.nkv;
+      at.y = quotient(off, len);
+      at.z = off - at.y * len;
+      at.w = len - pad;
+    }
+  } else {
+    const int pair = plan.cut == kCta ? blockIdx.x : blockIdx.x * kW + warp;
+    at.x = quotient(pair, a.nkv);
+    at.y = pair - at.x * a.nkv;
+    at.z = plan.cut == kCta ? warp * run : 0;
+    at.w = pages_of(at.x);
+    left = max(0, min(run, at.w - at.z));
+  }
+
+  TR(2);
+  const uint32_t ring = smem_addr(smem) + warp * S::kWarpBytes;
+  if (left > 0) {
+    // cursors: the pages being used, and the ones being fetched
+    struct Cursor {
+      int b, kvh, p, pages, left;
+    };
+    Cursor use{at.x, at.y, at.z, at.w, left};
+    int pos = u0;  // use's place in the list
+    auto pages_in = [&](int keys) { return (min(max(keys, 0), max_keys) + PAGE - 1) / PAGE; };
+    auto keys_of = [&](int b) { return b < a.B ? a.kv_len[b] : 0; };
+    // to the next pair (there is one), with the length of the next request in hand
+    auto next_pair = [&](Cursor& c, int next_keys) {
+      c.p = 0;
+      if (++c.kvh < a.nkv) return false;
+      c.kvh = 0;
+      ++c.b;
+      c.pages = pages_in(next_keys);
+#pragma unroll 1
+      while (c.pages == 0) c.pages = pages_of(++c.b);
+      return true;
+    };
+    if (use.p >= use.pages) {  // the run starts in the room behind a pair
+      use.left -= use.pages + pad - use.p;
+      pos += use.pages + pad - use.p;
+      if (use.left > 0) next_pair(use, keys_of(use.b + 1));
+    }
+    Cursor in = use;
+    // What the cursors will need is loaded ahead: lane i holds the block of page
+    // win + i of the request being fetched, of page win + 32 + i, of page i of
+    // it and of the next request, whose length next_keys is.
+    auto ids_of = [&](int b, int p) {
+      return b < a.B && p + lane < a.max_blocks ? a.block_table[b * a.bt_s + p + lane] : -1;
+    };
+    int win = in.p, id = ids_of(in.b, win), id_next = ids_of(in.b, win + 32);
+    int first = ids_of(in.b, 0), next_first = ids_of(in.b + 1, 0), next_keys = keys_of(in.b + 1);
+    typename HeadState<NT>::Query query;
+    auto load_query = [&](int b, int kvh) { query.load(a.q + ((int64_t)b * a.nq + kvh * G) * D, G, lane); };
+    if (use.left > 0) load_query(use.b, use.kvh);
+    int keys = keys_of(use.b), use_next_keys = next_keys;
+    // Each copy instruction reads 512 contiguous bytes (four rows, lane l the
+    // l-th 16) and places them where pages() reads them.
+    uint32_t k_dst[2], v_dst[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = i * 4 + (lane >> 3), ch = lane & 7;
+      k_dst[i] = k_place(row, ch);
+      v_dst[i] = 2048 + v_place(row, ch);
+    }
+    uint32_t bad = 0;  // stages whose page is not in the cache
+    auto fetch = [&](int st) {
+      if (in.p == in.pages) {
+        in.left -= pad;
+        if (in.left <= 0) return;
+        const int b = in.b;
+        if (next_pair(in, next_keys)) {
+          first = in.b == b + 1 ? next_first : ids_of(in.b, 0);
+          next_first = ids_of(in.b + 1, 0);
+          next_keys = keys_of(in.b + 1);
+        }
+        win = 0;
+        id = first;
+        id_next = in.pages > 32 ? ids_of(in.b, 32) : -1;
+      }
+      if (in.left <= 0) return;
+      if (in.p == win + 32) {
+        win += 32;
+        id = id_next;
+        id_next = ids_of(in.b, win + 32);
+      }
+      const int blk = __shfl_sync(0xffffffffu, id, in.p - win);
+      const uint32_t dst = ring + st * kStageBytes;
+      if (blk >= 0 && blk < a.num_blocks) {
+        bad &= ~(1u << st);
+        const int64_t base = ((int64_t)blk * a.nkv + in.kvh) * PAGE * D + lane * 16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          cp_async16(dst + k_dst[i & 1] + (i >> 1) * 1024, a.kv + base + i * 512);
+          cp_async16(dst + v_dst[i & 1] + (i >> 1) * 1024, a.vv + base + i * 512);
+        }
+        if (lane < 8) {
+          const uint8_t* e = lane < 4 ? a.ke + blk * a.ke_sb + in.kvh * a.ke_sh + lane * 4
+                                      : a.ve + blk * a.ve_sb + in.kvh * a.ve_sh + (lane - 4) * 4;
+          cp_async4(dst + 4096 + lane * 4, e);
+        }
+      } else {
+        bad |= 1u << st;
+      }
+      ++in.p;
+      --in.left;
+    };
+    // groups 0..kSt-1: the first pages; then one group per page used, in order
+#pragma unroll 1
+    for (int i = 0; i < kSt; ++i) {
+      fetch(i);
+      cp_async_commit();
+    }
+    TR(3);
+    HeadState<NT> st;
+    bool fresh = true;
+    int seg_p0 = use.p;  // the segment's first page
+    int L = 0;
+    int stage = 0;
+    while (use.left > 0) {
+      if (fresh) {
+        st.begin(query, a.scale_log2, lane);
+        L = min(keys, max_keys);
+        seg_p0 = use.p;
+        fresh = false;
+        // the next pair's query, where this warp will come to it
+        if (NT == 1 && use.left > use.pages - use.p + pad) {
+          const bool same = use.kvh + 1 < a.nkv;
+          load_query(same ? use.b : min(use.b + 1, a.B - 1), same ? use.kvh + 1 : 0);
+        }
+      }
+      cp_async_wait<kSt - 2>();
+      __syncwarp();
+      if (i == 0) TR(4);
+      const int stage1 = stage + 1 == kSt ? 0 : stage + 1;
+      const uint8_t* const src[2] = {smem + warp * S::kWarpBytes + stage * kStageBytes,
+                                     smem + warp * S::kWarpBytes + stage1 * kStageBytes};
+      const bool two = use.left > 1 && use.p + 1 < use.pages;
+      const int live[2] = {(bad >> stage) & 1 ? 0 : min(PAGE, L - use.p * PAGE),
+                           !two || ((bad >> stage1) & 1) ? 0 : min(PAGE, L - use.p * PAGE - PAGE)};
+      st.template pages<2>(src, live, lane);
+      __syncwarp();
+#pragma unroll 1
+      for (int u = two ? 2 : 1; u > 0; --u) {
+        fetch(stage);
+        cp_async_commit();
+        stage = stage + 1 == kSt ? 0 : stage + 1;
+        ++pos;
+        ++use.p;
+        --use.left;
+      }
+      const bool ends = use.p == use.pages;
+      if (!ends && use.left > 0) continue;
+      // ---- the segment is done
+      st.end();
+      const float vs = pow2(max(st.vr, -118) - 8);
+      if (seg_p0 == 0 && ends) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int head = n * 8 + 2 * t + c;
+            if (head >= G) continue;
+            const float inv = vs * inverse(st.l[n][c]);
+            float f[16];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              f[2 * j] = st.o[n][j][c] * inv;
+              f[2 * j + 1] = st.o[n][j][2 + c] * inv;
+            }
+            __nv_bfloat16* dst = a.o + ((int64_t)use.b * a.nq + use.kvh * G + head) * D + g * 16;
+            *reinterpret_cast<uint4*>(dst) = pack_from<__nv_bfloat16>(f);
+            *reinterpret_cast<uint4*>(dst + 8) = pack_from<__nv_bfloat16>(f + 8);
+          }
+      } else {
+        // began earlier: slot 0; begins here and goes on behind the run, whose
+        // ring is free then: slot 1
+        const int slot = seg_p0 == 0 ? 1 : 0;
+        float* po = reinterpret_cast<float*>(smem + (slot == 0 ? S::kPart + warp * S::kPartBytes : warp * S::kWarpBytes));
+        float2* ml = reinterpret_cast<float2*>(smem + S::kMl) + (slot * kW + warp) * S::kHeads;
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int head = n * 8 + 2 * t + c;
+            if (head >= G) continue;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<float2*>(po + head * kRow + g * 16 + 2 * j) =
+                  make_float2(st.o[n][j][c] * vs, st.o[n][j][2 + c] * vs);
+            if (g == 0) ml[head] = make_float2(st.m[n][c], st.l[n][c]);
+          }
+        if (lane == 0) {
+          flags[slot][warp] = kHere | (ends ? kEnds : 0);
+          pairs[slot][warp] = make_int4(use.b, use.kvh, pos - use.p, use.pages);
+        }
+      }
+      fresh = true;
+      if (!ends) break;
+      use.left -= pad;
+      pos += pad;
+      if (use.left <= 0) break;
+      const int b = use.b;
+      if (next_pair(use, use_next_keys)) {
+        keys = use.b == b + 1 ? use_next_keys : keys_of(use.b);
+        use_next_keys = keys_of(use.b + 1);
+      }
+      if (NT > 1 || use.b > b + 1) load_query(use.b, use.kvh);
+    }
+  }
+  // requests without keys: zeros, by the CTAs in turn
+#pragma unroll 1
+  for (int b = blockIdx.x + gridDim.x * warp; b < a.B; b += gridDim.x * kW) {
+    if (pages_of(b) > 0) continue;
+    uint4* dst = reinterpret_cast<uint4*>(a.o + (int64_t)b * a.nq * D);
+#pragma unroll 1
+    for (int i = lane; i < a.nq * D / 8; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
+  }
+  TR(5);
+  __syncthreads();
+  TR(6);
+
+  // ---- merges. Level 0, the warps' partials: chain 0 entered the CTA's run,
+  // chain c + 1 begins in warp c's; it goes on through the first segments of the
+  // warps that follow, up to the first that ends. Level 1, by the last CTA to
+  // arrive: the CTAs' partials of a pair that reaches over CTAs. One code for
+  // both (what runs once a launch waits for its instructions, too): partial 0
+  // lies by itself, the others a stride apart. A warp per (chain, head): lane i
+  // has partial i's (m, l), so that the weights 2^(m_i - M) come at once and the
+  // rows (lane l: dims 4l..4l+3) are independent loads.
+  const int f0 = lane < kW ? flags[0][lane] : 0, f1 = lane < kW ? flags[1][lane] : 0;
+  const uint32_t held = __ballot_sync(0xffffffffu, f0 != 0), ended = __ballot_sync(0xffffffffu, f0 & kEnds),
+                 begun = __ballot_sync(0xffffffffu, f1 != 0);
+  float* part_ml = a.part + (int64_t)gridDim.x * 2 * S::kHeads * D;
+  const int span = kW * run;
+  if (threadIdx.x==0) { g_trace[blockIdx.x*16+11]=begun; g_trace[blockIdx.x*16+12]=held; g_trace[blockIdx.x*16+13]=0; g_trace[blockIdx.x*16+14]=ended; }
+  const bool out0 = held & 1;    // chain 0 is one of several CTAs'
+  int out1 = -1;                 // the warp in whose run a pair begins that goes on in the next CTA
+  uint32_t todo = (begun << 1) | (held & 1);
+#pragma unroll 1
+  for (int level = 0; level < 2; ++level) {
+    int turn = warp;
+#pragma unroll 1
+    for (; todo != 0; todo &= todo - 1) {
+      const int c = __ffs(todo) - 2;  // -1, or the warp whose run the pair begins in
+      const int begins = c >= 0;
+      const int4 pair = begins ? pairs[1][c] : pairs[0][0];
+      int n;
+      bool whole = true;
+      const float *row0, *row1, *ml0, *ml1;  // rows and (m, l) of partials 0 and 1 of head 0
+      int row_step, ml_step, head_step;      // in floats
+      if (level == 0) {
+        const uint32_t ends = ended >> (c + 1);
+        n = begins + (ends ? __ffs(ends) : __popc(held >> (c + 1)));
+        whole = begins && ends;
+        if (begins && !ends) out1 = c;
+        const float* const parts = reinterpret_cast<const float*>(smem + S::kPart);
+        const float* const ml = reinterpret_cast<const float*>(smem + S::kMl);
+        row_step = S::kPartBytes / 4;
+        row1 = parts + (c + 1 + !begins) * row_step;
+        row0 = begins ? reinterpret_cast<const float*>(smem + c * S::kWarpBytes) : parts;
+        ml_step = 2 * S::kHeads;
+        ml1 = ml + (c + 1 + !begins) * ml_step;
+        ml0 = ml + (begins ? kW + c : 0) * ml_step;
+        head_step = kRow;
+      } else {
+        const int c0 = s_last[begins];
+        n = quotient(pair.z + pair.w - 1, span) - c0 + 1;
+        row_step = 2 * S::kHeads * D;
+        row0 = a.part + (int64_t)(2 * c0 + 1) * S::kHeads * D;
+        row1 = row0 + S::kHeads * D;
+        ml_step = 4 * S::kHeads;
+        ml0 = part_ml + (2 * c0 + 1) * S::kHeads * 2;
+        ml1 = ml0 + 2 * S::kHeads;
+        head_step = D;
+      }
+#pragma unroll 1
+      for (; turn < G; turn += kW) {
+        const int head = turn;
+        float M = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int kBlock = 8;  // partials loaded at once
+#pragma unroll 1
+        for (int i0 = 0; i0 < n; i0 += kBlock) {
+          const int mine = i0 + lane;
+          const bool has = lane < kBlock && mine < n;
+          float2 x = make_float2(-INFINITY, 0.f);
+          if (has) x = ld_partial2((mine == 0 ? ml0 : ml1 + (mine - 1) * ml_step) + 2 * head);
+          float4 y[kBlock];
+#pragma unroll
+          for (int j = 0; j < kBlock; ++j) {
+            const int i = min(i0 + j, n - 1);
+            y[j] = ld_partial4((i == 0 ? row0 : row1 + (int64_t)(i - 1) * row_step) + head * head_step + lane * 4);
+          }
+          const float nm = fmaxf(M, warp_max(x.x));
+          const float keep = merge_weight(M, nm);
+          const float w = has ? merge_weight(x.x, nm) : 0.f;
+          M = nm;
+          l = l * keep + warp_sum(has ? w * x.y : 0.f);
+          o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll
+          for (int j = 0; j < kBlock; ++j) {
+            const float wj = __shfl_sync(0xffffffffu, w, j);
+            if (i0 + j < n) add_scaled(o, wj, y[j]);
+          }
+        }
+        if (whole) {
+          const float inv = inverse(l);
+          const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x * inv, o.y * inv);
+          const __nv_bfloat162 hi = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+          uint2 y;
+          y.x = *reinterpret_cast<const uint32_t*>(&lo);
+          y.y = *reinterpret_cast<const uint32_t*>(&hi);
+          *reinterpret_cast<uint2*>(a.o + ((int64_t)pair.x * a.nq + pair.y * G + head) * D + lane * 4) = y;
+        } else {
+          const int to = (blockIdx.x * 2 + begins) * S::kHeads + head;
+          *reinterpret_cast<float4*>(a.part + (int64_t)to * D + lane * 4) = o;
+          if (lane == 0) *reinterpret_cast<float2*>(part_ml + 2 * to) = make_float2(M, l);
+        }
+      }
+      turn -= G;
+    }
+    if (level==0) TR(7); else TR(10);
+    if (level == 1 || (!out0 && out1 < 0)) return;
+    __syncthreads();
+    TR(8);
+    if (threadIdx.x < 2) {
+      int last = -1;
+      if (threadIdx.x == 0 ? out0 : out1 >= 0) {
+        const int4 pair = threadIdx.x == 0 ? pairs[0][0] : pairs[1][out1];
+        const int c0 = quotient(pair.z, span), c1 = quotient(pair.z + pair.w - 1, span);
+        // this CTA's partials before the count, the count before the others' partials
+        int seen;
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(a.counters + c0) : "memory");
+        if (seen == c1 - c0) {
+          a.counters[c0] = 0;  // for the next launch
+          last = c0;
+        }
+      }
+      s_last[threadIdx.x] = last;
+    }
+    __syncthreads();
+    TR(9);
+    todo = (s_last[0] >= 0 ? 1u : 0u) | (s_last[1] >= 0 ? 2u << out1 : 0u);
+  }
+}
+
+}  // namespace
+
+void rope_and_cache_kv8_launch(const void* qkv, const int* pos, const float* cos_sin, int64_t max_pos,
+                               const int64_t* slots, void* q_out, const Kv8Cache& c, int64_t T, int nq, int nkv,
+                               cudaStream_t s, const void* q_norm, const void* k_norm, double eps) {
+  if (T == 0) return;
+  AppendArgs a;
+  a.qkv = static_cast<const __nv_bfloat16*>(qkv);
+  a.pos = pos;
+  a.cos_sin = cos_sin;
+  a.slots = slots;
+  a.q_out = static_cast<__nv_bfloat16*>(q_out);
+  a.kv = c.kv;
+  a.vv = c.vv;
+  a.ke = c.ke;
+  a.ve = c.ve;
+  a.ke_sb = c.ke_sb;
+  a.ke_sh = c.ke_sh;
+  a.ve_sb = c.ve_sb;
+  a.ve_sh = c.ve_sh;
+  a.q_norm = static_cast<const __nv_bfloat16*>(q_norm);
+  a.k_norm = static_cast<const __nv_bfloat16*>(k_norm);
+  a.eps = eps;
+  a.T = T;
+  a.n_slots = c.blocks * PAGE;
+  a.max_pos = (int)max_pos;
+  a.nq = nq;
+  a.nkv = nkv;
+  const int64_t tasks = T * (nq + 2 * nkv);
+  launch_k(append_kernel, dim3((unsigned)((tasks + 3) / 4)), dim3(128), 0, s, a);
+  MBX_CUDA_CHECK(cudaGetLastError());
+}
+
+void read_pages_kv8_launch(const Kv8Cache& c, int nkv, const int* block_table, int64_t bt_stride, const int* out_table,
+                           int64_t ot_stride, const int* kv_len, int R, int max_blocks, void* k_out, void* v_out,
+                           int64_t out_pages, cudaStream_t s) {
+  if (R == 0 || max_blocks == 0) return;
+  ReadArgs a{c.kv, c.vv, c.ke, c.ve, c.ke_sb, c.ke_sh, c.ve_sb, c.ve_sh, block_table, out_table, kv_len,
+             bt_stride, ot_stride, static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), out_pages,
+             max_blocks, nkv, (int)c.blocks};
+  launch_k(read_pages_kernel, dim3(max_blocks, nkv, R), dim3(128), 0, s, a);
+  MBX_CUDA_CHECK(cudaGetLastError());
+}
+
+int decode_kv8_grid(int B, int nkv, int max_blocks) {
+  int dev = 0, sms = 0;
+  MBX_CUDA_CHECK(cudaGetDevice(&dev));
+  MBX_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  const int64_t pages = (int64_t)B * nkv * max_blocks;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(sms, (pages + kWarps - 1) / kWarps));
+}
+
+size_t decode_kv8_part_floats(int grid) { return (size_t)grid * 2 * 16 * (D + 2); }
+
+void decode_attention_kv8_launch(const void* q, const Kv8Cache& c, void* o, const int* kv_len, const int* block_table,
+                                 int64_t bt_stride, int max_blocks, int B, int nq, int nkv, int grid, float* part,
+                                 int* counters, float scale, cudaStream_t s) {
+  if (B == 0) return;
+  if (nq % nkv != 0 || nq / nkv > 16) throw std::runtime_error("decode: group size must be <= 16");
+  Kv8DecodeArgs a{static_cast<const __nv_bfloat16*>(q), c.kv, c.vv, c.ke, c.ve, c.ke_sb, c.ke_sh, c.ve_sb, c.ve_sh,
+                  static_cast<__nv_bfloat16*>(o), part, counters, kv_len, block_table, bt_stride, B, max_blocks,
+                  (int)c.blocks, nq, nkv, scale * 1.4426950408889634f};
+  if (nq / nkv <= 8) {
+    static SmemLimit limit;
+    limit.ensure((const void*)decode_kv8_kernel<1>, DecodeSmem<1>::kTotal);
+    launch_k(decode_kv8_kernel<1>, dim3(grid), dim3(kWarps * 32), DecodeSmem<1>::kTotal, s, a);
+  } else {
+    static SmemLimit limit;
+    limit.ensure((const void*)decode_kv8_kernel<2>, DecodeSmem<2>::kTotal);
+    launch_k(decode_kv8_kernel<2>, dim3(grid), dim3(kWarps * 32), DecodeSmem<2>::kTotal, s, a);
+  }
+  MBX_CUDA_CHECK(cudaGetLastError());
+}
+
+}  // namespace mbx
+extern "C" __attribute__((visibility("default"))) void kv8_trace(long long* out) { cudaMemcpyFromSymbol(out, mbx::g_trace, sizeof(mbx::g_trace)); }

@@ -627,8 +627,11 @@ void read_pages_kv8(torch::Tensor kv, torch::Tensor ke, torch::Tensor vv, torch:
   const int64_t R = kv_len.numel();
   check_table(block_table, "block_table", R);
   const int64_t mb = block_table.size(1);
-  check_dense(k_out, "k_out", torch::kBFloat16);
-  check_dense(v_out, "v_out", torch::kBFloat16);
+  for (const auto& [name, t] : {std::pair<const char*, const torch::Tensor*>{"k_out", &k_out}, {"v_out", &v_out}}) {
+    check_dense(*t, name, torch::kBFloat16);
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 32 == 0 || t->numel() == 0, name,
+                " must be 32-byte aligned");
+  }
   TORCH_CHECK(k_out.dim() == 4 && k_out.size(1) == nkv && k_out.size(2) == 16 && k_out.size(3) == 128 &&
                   v_out.sizes() == k_out.sizes(),
               "k_out and v_out must be [pages, nkv, 16, 128]");
