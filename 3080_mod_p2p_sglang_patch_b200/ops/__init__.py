@@ -280,16 +280,15 @@ def rope_and_cache(qkv, positions, cos_sin, nq, nkv, slots=None, k_cache=None, v
     row's definition gives. Slots that are negative or past the cache are not
     written; of tokens that name the same slot the last one is stored; a
     position outside the table takes its nearest row."""
-    T = qkv.shape[0]
-    if q_out is None:
-        q_out = torch.empty((T, nq, 128), dtype=qkv.dtype, device=qkv.device)
     if _is_fp8(k_cache, v_cache) and slots is not None:
         if page != 16:
             raise ValueError("8-bit caches have pages of 16 tokens")
-        cuda_ext().rope_and_cache_kv8(qkv, positions, cos_sin, slots, q_out, k_cache.values, k_cache.exps,
-                                      v_cache.values, v_cache.exps, nq, nkv, q_norm, k_norm, float(eps))
         launches.add(1)
-        return q_out
+        return cuda_ext().rope_and_cache_kv8(qkv, positions, cos_sin, slots, q_out, k_cache.values, k_cache.exps,
+                                             v_cache.values, v_cache.exps, nq, nkv, q_norm, k_norm, eps)
+    T = qkv.shape[0]
+    if q_out is None:
+        q_out = torch.empty((T, nq, 128), dtype=qkv.dtype, device=qkv.device)
     if slots is None:
         k_cache = v_cache = None
     cuda_ext().rope_and_cache(qkv, positions, cos_sin, slots, q_out, k_cache, v_cache, nq, nkv, page, q_norm, k_norm,

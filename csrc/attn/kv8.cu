@@ -1181,9 +1181,15 @@ void read_pages_kv8_launch(const Kv8Cache& c, int nkv, const int* block_table, i
 }
 
 int decode_kv8_grid(int B, int nkv, int max_blocks) {
-  int dev = 0, sms = 0;
+  static std::atomic<int> sms_of[64];  // 0: not asked yet
+  int dev = 0;
   MBX_CUDA_CHECK(cudaGetDevice(&dev));
-  MBX_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  if (dev < 0 || dev >= 64) throw std::runtime_error("decode: device index out of range");
+  int sms = sms_of[dev].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    MBX_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    sms_of[dev].store(sms, std::memory_order_relaxed);
+  }
   const int64_t pages = (int64_t)B * nkv * max_blocks;
   return (int)std::max<int64_t>(1, std::min<int64_t>(sms, (pages + kWarps - 1) / kWarps));
 }

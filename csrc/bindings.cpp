@@ -582,17 +582,21 @@ void check_lens(const torch::Tensor& t) {
               "kv_len must be contiguous int32 [requests]");
 }
 
-void rope_and_cache_kv8(torch::Tensor qkv, torch::Tensor positions, torch::Tensor cos_sin, torch::Tensor slots,
-                        torch::Tensor q_out, torch::Tensor kv, torch::Tensor ke, torch::Tensor vv, torch::Tensor ve,
-                        int64_t nq, int64_t nkv, c10::optional<torch::Tensor> q_norm,
-                        c10::optional<torch::Tensor> k_norm, double eps) {
+torch::Tensor rope_and_cache_kv8(const torch::Tensor& qkv, const torch::Tensor& positions,
+                                 const torch::Tensor& cos_sin, const torch::Tensor& slots,
+                                 const c10::optional<torch::Tensor>& q_out_opt, const torch::Tensor& kv,
+                                 const torch::Tensor& ke, const torch::Tensor& vv, const torch::Tensor& ve, int64_t nq,
+                                 int64_t nkv, const c10::optional<torch::Tensor>& q_norm,
+                                 const c10::optional<torch::Tensor>& k_norm, double eps) {
   check_dense(qkv, "qkv", torch::kBFloat16);
   TORCH_CHECK(nq > 0 && nkv > 0 && qkv.dim() == 2 && qkv.size(1) == (nq + 2 * nkv) * 128,
               "qkv must be [T, (nq + 2 nkv) * 128]");
   const Kv8Cache c = kv8_cache(kv, ke, vv, ve, nkv);
   const int64_t T = qkv.size(0);
-  check_dense(q_out, "q_out", torch::kBFloat16);
-  TORCH_CHECK(q_out.numel() == T * nq * 128, "q_out must be [T, nq, 128]");
+  if (q_out_opt.has_value()) {
+    check_dense(*q_out_opt, "q_out", torch::kBFloat16);
+    TORCH_CHECK(q_out_opt->numel() == T * nq * 128, "q_out must be [T, nq, 128]");
+  }
   TORCH_CHECK(positions.scalar_type() == torch::kInt32 && positions.numel() == T && positions.is_contiguous(),
               "positions must be contiguous int32 [T]");
   TORCH_CHECK(slots.scalar_type() == torch::kInt64 && slots.numel() == T && slots.is_contiguous(),
@@ -609,18 +613,22 @@ void rope_and_cache_kv8(torch::Tensor qkv, torch::Tensor positions, torch::Tenso
     TORCH_CHECK(q_norm->numel() == 128 && k_norm->numel() == 128, "q_norm / k_norm must be [128]");
   }
   check_devices({{"qkv", &qkv}, {"positions", &positions}, {"cos_sin", &cos_sin}, {"slots", &slots},
-                 {"q_out", &q_out}, {"k_cache", &kv}, {"k_cache exps", &ke}, {"v_cache", &vv}, {"v_cache exps", &ve},
-                 {"q_norm", q_norm ? &*q_norm : nullptr}, {"k_norm", k_norm ? &*k_norm : nullptr}});
+                 {"q_out", q_out_opt ? &*q_out_opt : nullptr}, {"k_cache", &kv}, {"k_cache exps", &ke},
+                 {"v_cache", &vv}, {"v_cache exps", &ve}, {"q_norm", q_norm ? &*q_norm : nullptr},
+                 {"k_norm", k_norm ? &*k_norm : nullptr}});
   const at::cuda::CUDAGuard guard(qkv.device());
+  const torch::Tensor q_out = q_out_opt ? *q_out_opt : torch::empty({T, nq, 128}, qkv.options());
   rope_and_cache_kv8_launch(qkv.data_ptr(), positions.data_ptr<int>(), cos_sin.data_ptr<float>(), cos_sin.size(0),
                             slots.data_ptr<int64_t>(), q_out.data_ptr(), c, T, (int)nq, (int)nkv, cur_stream(),
                             q_norm ? q_norm->data_ptr() : nullptr, k_norm ? k_norm->data_ptr() : nullptr, eps);
+  return q_out;
 }
 
-void read_pages_kv8(torch::Tensor kv, torch::Tensor ke, torch::Tensor vv, torch::Tensor ve, torch::Tensor block_table,
-                    torch::Tensor kv_len, c10::optional<torch::Tensor> out_table, torch::Tensor k_out,
-                    torch::Tensor v_out) {
-  check_pages8(kv, ke, "k_cache");
+void read_pages_kv8(const torch::Tensor& kv, const torch::Tensor& ke, const torch::Tensor& vv, const torch::Tensor& ve,
+                    const torch::Tensor& block_table, const torch::Tensor& kv_len,
+                    const c10::optional<torch::Tensor>& out_table, const torch::Tensor& k_out,
+                    const torch::Tensor& v_out) {
+  TORCH_CHECK(kv.dim() == 4, "k_cache values must be float8_e4m3fn [blocks, nkv, 16, 128] with at least one block");
   const int64_t nkv = kv.size(1);
   const Kv8Cache c = kv8_cache(kv, ke, vv, ve, nkv);
   check_lens(kv_len);
@@ -682,16 +690,17 @@ DecodeKv8Ws decode_kv8_ws(const torch::Tensor& q, cudaStream_t stream) {
   return ws;
 }
 
-torch::Tensor decode_attention_kv8(torch::Tensor q, torch::Tensor kv, torch::Tensor ke, torch::Tensor vv,
-                                   torch::Tensor ve, c10::optional<torch::Tensor> out_opt, torch::Tensor kv_len,
-                                   torch::Tensor block_table, double scale) {
+torch::Tensor decode_attention_kv8(const torch::Tensor& q, const torch::Tensor& kv, const torch::Tensor& ke,
+                                   const torch::Tensor& vv, const torch::Tensor& ve,
+                                   const c10::optional<torch::Tensor>& out_opt, const torch::Tensor& kv_len,
+                                   const torch::Tensor& block_table, double scale) {
   check_dense(q, "q", torch::kBFloat16);
   TORCH_CHECK(q.dim() == 3 && q.size(2) == 128, "q must be [B, nq, 128]");
   if (out_opt.has_value()) {
     check_dense(*out_opt, "out", torch::kBFloat16);
     TORCH_CHECK(out_opt->sizes() == q.sizes(), "out must have q's shape");
   }
-  check_pages8(kv, ke, "k_cache");
+  TORCH_CHECK(kv.dim() == 4, "k_cache values must be float8_e4m3fn [blocks, nkv, 16, 128] with at least one block");
   const int64_t B = q.size(0), nq = q.size(1), nkv = kv.size(1);
   const Kv8Cache c = kv8_cache(kv, ke, vv, ve, nkv);
   TORCH_CHECK(nq > 0 && nq % nkv == 0 && nq / nkv <= 16, "q heads must be 1 to 16 per kv head, a whole number");
