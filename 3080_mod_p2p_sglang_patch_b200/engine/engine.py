@@ -27,7 +27,7 @@ from ..ops import oracle
 from ..utils import nvtx
 from ..models import LlamaConfig, LlamaTP, LlamaWeights
 from .graph_runner import DecodeGraphRunner, PrefillGraphRunner
-from .kv_cache import PAGE, PagedKVCache, PrefixCache
+from .kv_cache import PAGE, PagedKVCache, PrefixCache, kv_dtype
 from .sampling import GREEDY, SamplingParams, adjust_logits, sample
 from .scheduler import Request, Scheduler
 
@@ -38,7 +38,10 @@ class LLMEngine:
                  graph_sizes=(1, 8, 32, 64), full_init: bool = False, device=None, prefill_graph: bool = False,
                  sp: bool = None, weights=None, prefix_cache: bool = False, mem_fraction: float = None,
                  mixed_chunk: bool = False, schedule_policy: str = "fcfs", sample_in_graphs: bool = False,
-                 overlap: bool = None, overlap_min_rows: int = 512):
+                 overlap: bool = None, overlap_min_rows: int = 512, kv_cache_dtype: str = "auto"):
+        # storage of the KV cache: "auto" / "bf16", or "fp8_e4m3" (half the
+        # bytes: twice the tokens, and half of what decode attention streams)
+        self.kv_cache_dtype = kv_dtype(kv_cache_dtype)
         if impl == "oracle":  # fp32 torch restatement of every kernel: eager, any device
             use_graphs, prefill_graph = False, False
         if max_seq > cfg.max_pos:
@@ -91,13 +94,14 @@ class LLMEngine:
                 # weights + KV cache within mem_fraction of the device (the rest:
                 # activations, workspaces, CUDA graphs)
                 free, total = torch.cuda.mem_get_info(self.device)
-                block_bytes = PagedKVCache.bytes_per_token(cfg.layers, nkv, cfg.head_dim) * PAGE
+                block_bytes = PagedKVCache.bytes_per_token(cfg.layers, nkv, cfg.head_dim,
+                                                           self.kv_cache_dtype.itemsize) * PAGE
                 fit = PagedKVCache.blocks_for_memory(total, free, mem_fraction, block_bytes)
                 if fit < self.max_blocks_per_seq:
                     raise ValueError(f"mem_fraction {mem_fraction}: the KV cache would hold {fit * PAGE} tokens, "
                                      f"fewer than max_seq {max_seq}")
                 kv_blocks = min(kv_blocks, fit + 1)
-        self.kv = PagedKVCache(cfg.layers, nkv, cfg.head_dim, kv_blocks, self.device)
+        self.kv = PagedKVCache(cfg.layers, nkv, cfg.head_dim, kv_blocks, self.device, self.kv_cache_dtype)
         # prefix caching: off by default (benchmarks must not reuse work)
         self.prefix_cache = PrefixCache(self.kv.alloc) if prefix_cache else None
         self.sched = Scheduler(chunk, max_batch, self.kv.alloc, max_seq, prefix_cache=self.prefix_cache,
@@ -360,13 +364,22 @@ class LLMEngine:
         tiles = self._h2d(ops.prefill_tiles(q_lens))
         scale = self.model.scale
         splits = ops.prefill_splits(tiles.shape[0], self.cfg.heads // self.tp_size, max(kv_lens))
+        kw = self._page_plan(kv_lens)
 
         def attn(li, q, kc, vc):
-            return ops.prefill_attention(q, kc, vc, cu_d, kvl_d, bt, tiles, scale, splits=splits)
+            return ops.prefill_attention(q, kc, vc, cu_d, kvl_d, bt, tiles, scale, splits=splits, **kw)
 
         halves = self._attn_halves(q_lens, kv_lens, bt, T)
         return self.model.forward(ids_d, pos_d, slots_d, self.kv.caches, attn, last_d, return_hidden=return_hidden,
                                   attn_halves=halves)
+
+    def _page_plan(self, kv_lens) -> dict:
+        """Prefill attention's scratch pages over an 8-bit cache, packed by the
+        requests' lengths (nothing for bf16, which is read in place)."""
+        if self.kv_cache_dtype != torch.float8_e4m3fn:
+            return {}
+        plan = ops.page_plan(kv_lens, self.max_blocks_per_seq)
+        return {"plan": ops.PagePlan(self._h2d(plan.table), plan.pages)}
 
     def _attn_halves(self, q_lens, kv_lens, bt, T):
         """Attention of each micro-batch of an overlapped prefill batch
@@ -406,9 +419,10 @@ class LLMEngine:
             bt_h = bt.index_select(0, sel.long())
             tiles_h = self._h2d(ops.prefill_tiles(ql))
             splits_h = ops.prefill_splits(tiles_h.shape[0], nq, max(kl))
+            kw = self._page_plan(kl)
 
-            def f(li, q, kc, vc, cu_h=cu_h, kvl_h=kvl_h, bt_h=bt_h, tiles_h=tiles_h, splits_h=splits_h):
-                return ops.prefill_attention(q, kc, vc, cu_h, kvl_h, bt_h, tiles_h, scale, splits=splits_h)
+            def f(li, q, kc, vc, cu_h=cu_h, kvl_h=kvl_h, bt_h=bt_h, tiles_h=tiles_h, splits_h=splits_h, kw=kw):
+                return ops.prefill_attention(q, kc, vc, cu_h, kvl_h, bt_h, tiles_h, scale, splits=splits_h, **kw)
             fns.append(f)
         return (T1, fns[0], fns[1])
 

@@ -219,6 +219,11 @@ class PrefillGraphRunner:
                 self.halves.append({"cu": torch.tensor([0, n], dtype=torch.int32, device=dev), "tiles": tiles,
                                     "splits": splits, "kvl": torch.full((1,), n, dtype=torch.int32, device=dev)})
             self.halves[1]["kvl"] = self.kvl
+        # over an 8-bit cache: scratch pages for the longest request, in order
+        self.plan = {}
+        if engine.kv_cache_dtype == torch.float8_e4m3fn:
+            n = engine.max_blocks_per_seq
+            self.plan = {"plan": ops.PagePlan(torch.arange(n, dtype=torch.int32).view(1, n).to(dev), n)}
         self.graph = None
         self.out = None
 
@@ -227,14 +232,15 @@ class PrefillGraphRunner:
         scale = e.model.scale
 
         def attn(li, q, kc, vc):
-            return ops.prefill_attention(q, kc, vc, self.cu, self.kvl, self.bt, self.tiles, scale, splits=self.splits)
+            return ops.prefill_attention(q, kc, vc, self.cu, self.kvl, self.bt, self.tiles, scale, splits=self.splits,
+                                         **self.plan)
 
         halves = None
         if self.halves is not None:
             def half_attn(h):
                 def f(li, q, kc, vc):
                     return ops.prefill_attention(q, kc, vc, h["cu"], h["kvl"], self.bt, h["tiles"], scale,
-                                                 splits=h["splits"])
+                                                 splits=h["splits"], **self.plan)
                 return f
             halves = (self.T1, half_attn(self.halves[0]), half_attn(self.halves[1]))
         return e.model.forward(self.ids, self.pos, self.slots, e.kv.caches, attn, self.last, attn_halves=halves)

@@ -1,8 +1,9 @@
-"""Paged KV cache (page = 16 tokens, bf16) and its block allocator.
+"""Paged KV cache (page = 16 tokens, bf16 or 8-bit) and its block allocator.
 
 Layout per layer: k, v = [num_blocks, kv_heads_per_rank, 16, head_dim] - one
 contiguous 4 KB page per (block, kv head), the unit the attention kernels
-stream. Block 0 is reserved as a scratch page for padded decode rows.
+stream, or in 8 bits (``ops.Fp8Pages``) 2 KB of e4m3 numbers and 16 exponents.
+Block 0 is reserved as a scratch page for padded decode rows.
 (The reference relies on sglang's paged cache; it ships none.)
 """
 import collections
@@ -10,7 +11,22 @@ import collections
 import numpy as np
 import torch
 
+from ..ops.fp8_pages import HEAD_DIM, fp8_cache
+
 PAGE = 16
+
+# names of the cache's storage types (sglang's --kv-cache-dtype spelling)
+KV_DTYPES = {"auto": torch.bfloat16, "bf16": torch.bfloat16, "bfloat16": torch.bfloat16,
+             "fp8_e4m3": torch.float8_e4m3fn}
+
+
+def kv_dtype(name) -> torch.dtype:
+    """The storage type a ``KV_DTYPES`` name (or the type itself) stands for."""
+    if isinstance(name, torch.dtype) and name in KV_DTYPES.values():
+        return name
+    if not isinstance(name, str) or name not in KV_DTYPES:
+        raise ValueError(f"KV cache dtype {name!r}: one of {', '.join(KV_DTYPES)}")
+    return KV_DTYPES[name]
 
 
 class BlockAllocator:
@@ -143,8 +159,14 @@ class PagedKVCache:
     def __init__(self, layers: int, kv_heads: int, head_dim: int, num_blocks: int, device, dtype=torch.bfloat16):
         self.layers = layers
         self.num_blocks = num_blocks
-        self.storage = torch.zeros((layers, 2, num_blocks, kv_heads, PAGE, head_dim), dtype=dtype, device=device)
-        self.caches = [(self.storage[l, 0], self.storage[l, 1]) for l in range(layers)]
+        self.dtype = dtype
+        if dtype == torch.float8_e4m3fn:
+            if head_dim != HEAD_DIM:
+                raise ValueError(f"the 8-bit KV cache needs head_dim {HEAD_DIM}, not {head_dim}")
+            self.caches = [fp8_cache(num_blocks, kv_heads, device) for _ in range(layers)]
+        else:
+            self.storage = torch.zeros((layers, 2, num_blocks, kv_heads, PAGE, head_dim), dtype=dtype, device=device)
+            self.caches = [(self.storage[l, 0], self.storage[l, 1]) for l in range(layers)]
         self.alloc = BlockAllocator(num_blocks)
 
     @staticmethod
@@ -153,7 +175,8 @@ class PagedKVCache:
 
     @staticmethod
     def bytes_per_token(layers, kv_heads, head_dim, dtype_bytes=2):
-        return layers * 2 * kv_heads * head_dim * dtype_bytes
+        """``dtype_bytes`` 1: the 8-bit form, with each row's exponent byte."""
+        return layers * 2 * kv_heads * (head_dim * dtype_bytes + (dtype_bytes == 1))
 
     @staticmethod
     def blocks_for_memory(total_bytes: int, free_bytes: int, fraction: float, block_bytes: int) -> int:

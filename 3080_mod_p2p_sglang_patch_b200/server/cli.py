@@ -38,8 +38,9 @@ def build_parser() -> argparse.ArgumentParser:
     # sglang launch flags with the same meaning here
     ap.add_argument("--dtype", default="auto", choices=["auto", "bfloat16", "bf16"],
                     help="compute dtype: bf16 (auto)")
-    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "bfloat16", "bf16"],
-                    help="KV cache dtype: bf16 (auto)")
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "bfloat16", "bf16", "fp8_e4m3"],
+                    help="KV cache dtype: bf16 (auto), or fp8_e4m3 (half the bytes; one power-of-two scale per "
+                         "token and kv head)")
     ap.add_argument("--quantization", default=None, choices=["awq", "awq_marlin"],
                     help="AWQ checkpoints: keep the int4 weights packed (same as --int4-weights)")
     ap.add_argument("--random-seed", "--seed", dest="seed", type=int, default=0,
@@ -243,7 +244,7 @@ def main(argv=None):
                 impl=args.impl, prefill_graph=(args.impl == "native" and not args.no_graphs),
                 prefix_cache=args.prefix_cache, mem_fraction=args.mem_fraction, mixed_chunk=args.mixed_chunk,
                 schedule_policy=args.schedule_policy or ("lpm" if args.prefix_cache else "fcfs"),
-                sample_in_graphs=args.graph_sampled_decode)
+                sample_in_graphs=args.graph_sampled_decode, kv_cache_dtype=args.kv_cache_dtype)
     if args.max_seq is not None:
         opts["max_seq"] = args.max_seq
     if args.max_total_tokens:

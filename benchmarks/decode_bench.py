@@ -1,6 +1,7 @@
 """CUDA-graph decode ITL: Llama-style 8B at TP = world
 size, batch sizes {1, 8, 32, 64}, every request with a 4096-token
-uniform-random-id context prefilled into the paged KV cache (page 16, bf16),
+uniform-random-id context prefilled into the paged KV cache (page 16, bf16
+or --kv-cache-dtype fp8_e4m3),
 then 256 tokens generated greedily.
 
     torchrun --nproc-per-node N benchmarks/decode_bench.py [--impl native|torch]
@@ -27,6 +28,7 @@ def main():
     ap.add_argument("--model", default="8b")
     ap.add_argument("--impl", default="native", choices=["native", "torch"])
     ap.add_argument("--int4", action="store_true", help="random weights packed as AWQ int4 (native only)")
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "bf16", "fp8_e4m3"])
     ap.add_argument("--batches", default="1,8,32,64")
     ap.add_argument("--ctx", type=int, default=4096)
     ap.add_argument("--gen", type=int, default=256)
@@ -47,7 +49,7 @@ def main():
         models.quantize_weights_int4(weights)
     eng = eng_mod.LLMEngine(cfg, tp=tp, max_batch=max_bs, max_seq=args.ctx + args.gen + 16, chunk=8192, seed=0,
                             use_graphs=True, impl=args.impl, graph_sizes=tuple(sorted(set(batches))),
-                            weights=weights, device=dev)
+                            weights=weights, device=dev, kv_cache_dtype=args.kv_cache_dtype)
     g = torch.Generator().manual_seed(7)
     for bs in batches:
         prompts = torch.randint(0, cfg.vocab, (bs, args.ctx), generator=g).tolist()
@@ -84,7 +86,7 @@ def main():
         mean = sum(ts) / len(ts)
         if rank == 0:
             print(json.dumps({"metric": "decode_itl", "model": cfg.name, "impl": args.impl, "tp": world, "batch": bs,
-                              "int4_weights": args.int4,
+                              "int4_weights": args.int4, "kv_cache_dtype": args.kv_cache_dtype,
                               "ctx": args.ctx, "gen": args.gen, "itl_p50_ms": p50, "itl_p99_ms": p99,
                               "decode_tok_s": bs / (mean * 1e-3), "steps": steps}), flush=True)
     if eng.graphs is not None:

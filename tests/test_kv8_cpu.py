@@ -219,3 +219,96 @@ def test_refusals_of_head_counts_and_outputs():
         ops.read_pages(**a, out_table=torch.zeros(3, 2, dtype=torch.int32))
     with pytest.raises(TypeError, match="8-bit caches"):
         ops.read_pages(torch.zeros(1), torch.zeros(1), a["block_table"], a["kv_len"])
+
+
+# ---------------------------------------------------------------- the engine on an 8-bit cache
+def dense_fp8(cfg, w, tokens):
+    """``test_engine_cpu._dense`` (fp32, no cache, no pages) with the rotated k
+    and the v rounded to the 8-bit cache's rows: (hidden [T, H], logits)."""
+    import torch.nn.functional as F
+
+    ops, ref, f8 = sub("ops"), sub("ops.reference"), sub("ops.fp8_pages")
+
+    def rounded(x):
+        return f8.dequantize_rows(*f8.quantize_rows(x))
+
+    T, eps, nq, nkv = len(tokens), cfg.eps, cfg.heads, cfg.kv_heads
+    cs = ops.rope_cos_sin(cfg.max_pos, D, cfg.rope_theta, "cpu")
+    pos = torch.arange(T)
+    res = w.embed.float()[torch.tensor(tokens)]
+    for L in w.layers:
+        qkv = (ref.rmsnorm(res, L["ln1"], eps) @ L["qkv"].float().t()).view(T, -1, D)
+        q, k, v = qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:]
+        if cfg.qk_norm:
+            q, k = ref.rmsnorm(q, L["q_norm"], eps), ref.rmsnorm(k, L["k_norm"], eps)
+        q, k, v = ref.rope(q, pos, cs), rounded(ref.rope(k, pos, cs)), rounded(v)
+        res = res + ref.attention(q, k, v, causal_offset=0).reshape(T, nq * D) @ L["o"].float().t()
+        g, u = (ref.rmsnorm(res, L["ln2"], eps) @ L["gate_up"].float().t()).chunk(2, dim=-1)
+        res = res + (F.silu(g) * u) @ L["down"].float().t()
+    h = ref.rmsnorm(res, w.norm, eps)
+    return h, h @ w.lm_head.float().t()
+
+
+def _near_argmax(cfg, w, prompt, out, tol):
+    seq = list(prompt)
+    for t in out:
+        _, logits = dense_fp8(cfg, w, seq)
+        assert logits[-1][t] >= logits[-1].max() - tol, (len(seq) - len(prompt), t, int(logits[-1].argmax()))
+        seq.append(t)
+
+
+@pytest.mark.parametrize("qk_norm", [False, True])
+def test_engine_prefill_over_an_8_bit_cache_matches_the_dense_forward(qk_norm):
+    """The bounds of the bf16 cache's test, against a dense forward whose k
+    and v rows are rounded the same way."""
+    from test_engine_cpu import CFG, _cos, _engine, _prompt_hidden
+
+    models = sub("models")
+    cfg = models.LlamaConfig(**{**CFG.__dict__, "qk_norm": qk_norm})
+    prompt = torch.randint(0, cfg.vocab, (150,), generator=torch.Generator().manual_seed(1)).tolist()
+    for chunk in (150, 64, 37):
+        eng = _engine(cfg, chunk=chunk, kv_cache_dtype="fp8_e4m3")
+        assert isinstance(eng.kv.caches[0][0], sub("ops").Fp8Pages)
+        got = _prompt_hidden(eng, prompt, chunk)
+        want, _ = dense_fp8(cfg, eng.weights, prompt)
+        assert _cos(got, want[-1]) > 0.999, chunk
+        assert float((got - want[-1]).abs().max()) < 0.05 * float(want[-1].abs().max()), chunk
+
+
+def test_engine_generates_over_an_8_bit_cache():
+    """Chunks, batches, a prefix-cache hit and mixed chunks."""
+    from test_engine_cpu import CFG, LOGIT_TOL, _engine
+
+    g = torch.Generator().manual_seed(2)
+    common = torch.randint(0, CFG.vocab, (48,), generator=g).tolist()
+    prompts = [common + torch.randint(0, CFG.vocab, (n,), generator=g).tolist() for n in (30, 1)] + \
+        [torch.randint(0, CFG.vocab, (70,), generator=g).tolist()]
+    eng = _engine(chunk=32, kv_cache_dtype="fp8_e4m3", prefix_cache=True, mixed_chunk=True)
+    first = eng.generate(prompts[:1], max_new_tokens=5)
+    outs = first + eng.generate(prompts[1:], max_new_tokens=5)
+    assert eng.prefix_cache.hits == 3
+    for p, o in zip(prompts, outs):
+        assert len(o) == 5
+        _near_argmax(CFG, eng.weights, p, o, LOGIT_TOL)
+
+
+def test_cache_dtype_names_and_sizes():
+    from test_engine_cpu import _engine
+
+    kv = sub("engine.kv_cache")
+    assert kv.kv_dtype("auto") == kv.kv_dtype("bfloat16") == torch.bfloat16
+    assert kv.kv_dtype("fp8_e4m3") == kv.kv_dtype(torch.float8_e4m3fn) == torch.float8_e4m3fn
+    for bad in ("fp8_e5m2", "int8", torch.float16, None, 8):
+        with pytest.raises(ValueError, match="KV cache dtype"):
+            kv.kv_dtype(bad)
+    with pytest.raises(ValueError, match="KV cache dtype"):
+        _engine(kv_cache_dtype="fp16")
+    # 8B: 129 bytes per row instead of 256
+    assert kv.PagedKVCache.bytes_per_token(32, 8, 128, 1) == 32 * 2 * 8 * 129
+    c = kv.PagedKVCache(2, 2, 128, 5, "cpu", torch.float8_e4m3fn)
+    per_block = sum(t.numel() for k, v in c.caches for t in (k.values, v.values, k.exps, v.exps)) // 5
+    assert per_block == kv.PagedKVCache.bytes_per_token(2, 2, 128, 1) * kv.PAGE
+    with pytest.raises(ValueError, match="head_dim 128"):
+        kv.PagedKVCache(1, 2, 64, 5, "cpu", torch.float8_e4m3fn)
+    p = sub("server.cli").build_parser()
+    assert p.parse_args(["--kv-cache-dtype", "fp8_e4m3"]).kv_cache_dtype == "fp8_e4m3"

@@ -614,6 +614,57 @@ def test_two_captured_graphs_and_eager_calls_at_once():
     assert all(torch.equal(a, b) for a, b in zip(outs[0], w))
 
 
+# ---------------------------------------------------------------- the engine
+def _native(cfg, **kw):
+    from test_engine_gpu import _engine
+
+    return _engine(cfg, kv_cache_dtype="fp8_e4m3", **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(use_graphs=False, mixed_chunk=True), dict(prefill_graph=True),
+                                dict(impl="torch")])
+def test_native_engine_over_an_8_bit_cache_follows_the_dense_forward(kw):
+    """Greedy tokens of prompts across chunks, one of them a prefix-cache hit,
+    against the dense fp32 forward whose k and v rows are rounded the same
+    way, at the tolerance of the bf16 cache's engine test."""
+    from test_engine_gpu import CFG, TOL, _host
+    from test_kv8_cpu import _near_argmax
+
+    eng = _native(CFG, prefix_cache=True, **kw)
+    w = _host(eng.weights)
+    g = torch.Generator().manual_seed(11)
+    common = torch.randint(0, CFG.vocab, (48,), generator=g).tolist()
+    a, b = (common + torch.randint(0, CFG.vocab, (n,), generator=g).tolist() for n in (30, 9))
+    c = torch.randint(0, CFG.vocab, (200,), generator=g).tolist()
+    out_a, out_c = eng.generate([a, c], max_new_tokens=6)
+    req = eng.add_request(b, 6)
+    eng.run()
+    assert req.cached_pages == 3
+    for p, o in ((a, out_a), (c, out_c), (b, req.output)):
+        assert len(o) == 6
+        _near_argmax(CFG, w, p, o, TOL)
+
+
+def test_native_and_oracle_score_text_alike_over_an_8_bit_cache():
+    """Per-token logprobs of 400 prompt tokens, native against the fp32 oracle
+    on the CPU, both on 8-bit caches; the bf16 cache's bound."""
+    from test_engine_gpu import CFG
+
+    models, eng_mod = sub("models"), sub("engine")
+    prompt = torch.randint(0, CFG.vocab, (400,), generator=torch.Generator().manual_seed(5)).tolist()
+    scores = []
+    for kw in (dict(device="cuda"), dict(device="cpu", impl="oracle")):
+        w = models.LlamaWeights(CFG, 0, 1, "cpu", seed=0, full_init=True)
+        if kw["device"] == "cuda":
+            w.embed, w.norm, w.lm_head = w.embed.cuda(), w.norm.cuda(), w.lm_head.cuda()
+            w.layers = [{k: v.cuda() for k, v in L.items()} for L in w.layers]
+        eng = eng_mod.LLMEngine(CFG, weights=w, max_batch=2, max_seq=512, chunk=128, kv_cache_dtype="fp8_e4m3", **kw)
+        r = eng.add_request(prompt, 1, prompt_logprobs=True)
+        eng.run()
+        scores.append(torch.tensor([x[0] for x in r.prompt_token_logprobs[1:]]))
+    assert (scores[0] - scores[1]).abs().mean().item() < 0.05
+
+
 @pytest.mark.skipif(not torch.cuda.is_available() or torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_second_device_while_the_first_is_current():
     ops = sub("ops")
