@@ -477,14 +477,10 @@ def _prefill_fp8(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, scale, o
     pages = R * cols if plan is None else plan.pages
     table = _page_ids(pages, q.device).view(R, cols) if plan is None else plan.table
     kv = torch.empty((2, max(1, pages)) + tuple(k_cache.shape[1:]), dtype=torch.bfloat16, device=q.device)
-    read_pages(k_cache, v_cache, block_table, kv_len, out_table=table, k_out=kv[0], v_out=kv[1])
-    po = pl = None
-    if splits > 1:
-        part = torch.empty(q.numel() // 128 * splits * 129, dtype=torch.float32, device=q.device)
-        po, pl = part[:q.numel() * splits], part[q.numel() * splits:]
-    with torch.cuda.device(q.device):
-        cuda_ext().prefill_attention_tc(q, kv[0], kv[1], out, cu_q, kv_len, table, tiles, scale,
-                                        workspace(q.device).err, splits, po, pl)
+    k, v = kv.unbind(0)
+    read_pages(k_cache, v_cache, block_table, kv_len, out_table=table, k_out=k, v_out=v)
+    cuda_ext().prefill_attention_pages(q, k, v, out, cu_q, kv_len, table, tiles, scale, workspace(q.device).err,
+                                       splits)
     launches.add(2 if splits > 1 else 1)
     return out
 

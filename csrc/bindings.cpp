@@ -660,6 +660,53 @@ void read_pages_kv8(const torch::Tensor& kv, const torch::Tensor& ke, const torc
                         cur_stream());
 }
 
+// Causal attention of a prefill batch over the pages that read_pages_kv8 wrote
+// (k, v [pages, nkv, 16, 128], placed by a packed `table`); its split-KV
+// scratch comes from the caching allocator, so that calls on other streams and
+// in other graphs have their own.
+torch::Tensor prefill_attention_pages(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                                      const torch::Tensor& out, const torch::Tensor& cu_q, const torch::Tensor& kv_len,
+                                      const torch::Tensor& table, const torch::Tensor& tiles, double scale,
+                                      const torch::Tensor& err, int64_t splits) {
+  check_dense(q, "q", torch::kBFloat16);
+  TORCH_CHECK(q.dim() == 3 && q.size(2) == 128, "q must be [T, nq, 128]");
+  check_dense(out, "out", torch::kBFloat16);
+  TORCH_CHECK(out.sizes() == q.sizes(), "out must have q's shape");
+  check_dense(k, "k", torch::kBFloat16);
+  check_dense(v, "v", torch::kBFloat16);
+  TORCH_CHECK(k.dim() == 4 && k.size(2) == 16 && k.size(3) == 128 && v.sizes() == k.sizes() && k.size(0) > 0 &&
+                  k.size(0) < (int64_t)1 << 31,
+              "k and v must be [pages, nkv, 16, 128]");
+  const int64_t T = q.size(0), nq = q.size(1), nkv = k.size(1);
+  TORCH_CHECK(nkv > 0 && nq > 0 && nq % nkv == 0, "q heads must be a multiple of the kv heads");
+  check_lens(kv_len);
+  const int64_t R = kv_len.numel();
+  TORCH_CHECK(cu_q.scalar_type() == torch::kInt32 && cu_q.is_contiguous() && cu_q.numel() == R + 1,
+              "cu_q must be contiguous int32 [requests + 1]");
+  check_table(table, "plan table", R);
+  TORCH_CHECK(table.is_contiguous(), "plan table must be contiguous");
+  TORCH_CHECK(tiles.scalar_type() == torch::kInt32 && tiles.is_contiguous() && tiles.dim() == 2 && tiles.size(1) == 2,
+              "tiles must be contiguous int32 [n, 2]");
+  TORCH_CHECK(scale > 0, "prefill attention needs a positive scale");
+  TORCH_CHECK(splits >= 1 && splits < 65536 && nq < 65536, "splits and q heads must lie in 1 to 65535");
+  check_devices({{"q", &q}, {"k", &k}, {"v", &v}, {"out", &out}, {"cu_q", &cu_q}, {"kv_len", &kv_len},
+                 {"plan table", &table}, {"tiles", &tiles}, {"err", &err}});
+  const at::cuda::CUDAGuard guard(q.device());
+  torch::Tensor part;
+  float *po = nullptr, *pl = nullptr;
+  if (splits > 1) {
+    part = torch::empty({T * nq * splits * 129}, q.options().dtype(torch::kFloat32));
+    po = part.data_ptr<float>();
+    pl = po + T * nq * splits * 128;
+  }
+  prefill_attention_pages_launch(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_q.data_ptr<int>(),
+                                 kv_len.data_ptr<int>(), table.data_ptr<int>(), (int)table.size(1),
+                                 tiles.data_ptr<int>(), (int)tiles.size(0), (int)T, (int)nq, (int)nkv, k.size(0),
+                                 (float)scale, (int)splits, po, pl,
+                                 reinterpret_cast<uint32_t*>(err.data_ptr<int>()), cur_stream());
+  return out;
+}
+
 // Scratch of decode_attention_kv8: partial results, and arrival counters that
 // every launch finds and leaves at zero. One per stream, since launches on
 // different streams may run at the same time, and one per graph capture, whose
@@ -865,5 +912,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("scale"), py::arg("counters") = c10::nullopt);
   m.def("rope_and_cache_kv8", &rope_and_cache_kv8);
   m.def("read_pages_kv8", &read_pages_kv8);
+  m.def("prefill_attention_pages", &prefill_attention_pages);
   m.def("decode_attention_kv8", &decode_attention_kv8);
 }

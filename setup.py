@@ -49,6 +49,7 @@ ext_modules = [
             src("attn", "attention.cu"),
             src("attn", "decode_noalloc.cu"),
             src("attn", "fmha_tc.cu"),
+            src("attn", "fmha_pages.cu"),
             src("attn", "kv8.cu"),
             src("quant", "awq.cu"),
         ],
