@@ -1,21 +1,22 @@
 // Prefill attention over a batch's own bf16 pages (the 8-bit cache, read back),
 // on the Blackwell tensor cores (tcgen05 + TMEM + TMA).
 //
-// The scratch pages of a request lie one after another, so a tile of 128 keys is
-// one TMA box per 64 dims, and the tiles can be twice those of the kernel over
-// the cache itself (fmha_tc.cu). One CTA = two 128-row query tiles of one head,
-// each with its own softmax warpgroup. Per query tile and tile of 128 keys:
-//   S  = Q K^T    tcgen05.mma 128 x 128, fp32 in TMEM
-//   P  = exp2(S * scale - m) by 4 warps, one thread per row, stored as bf16 over
-//        S in TMEM (64 of its 128 columns)
+// The scratch pages of a request lie one after another, so a tile of keys is one
+// TMA box per 64 dims. One CTA = two 128-row query tiles of one head, each with
+// its own softmax warpgroup. Per query tile and tile of 64 keys:
+//   S  = Q K^T    tcgen05.mma 128 x 64, fp32 in TMEM
+//   P  = exp2(S * scale - m) by 4 warps, one thread per row, stored as bf16 in
+//        TMEM (32 columns)
 //   O += P V      tcgen05.mma with A = P from TMEM, V MN-major from shared memory
-// Why this shape: with 64-key tiles and P in shared memory, Q is read from
-// shared memory twice as often per key and P is written and read there as well;
-// at 128 bytes per cycle that traffic, not the MMAs, bounds the loop. Here the
-// operands take 96 KB per 128 x 128 x 128 pair of products, less than the MMAs.
-// TMEM is full: S/P of two tiles (256 columns) and two O (256). S of the next
-// tile overwrites P, so it is issued once the PV product is complete; the other
-// query tile's products and softmax run meanwhile.
+// Why this shape. Shared memory feeds the tensor core 128 bytes a cycle. With P
+// written to and read from shared memory, as the kernel over the cache itself
+// does (fmha_tc.cu), that port takes 1.75 times as long as the MMAs; with P in
+// TMEM 1.25 times. Tiles of 128 keys would read Q half as often, but then P has
+// to lie over S (TMEM is 512 columns, O takes 256), the next S has to wait for
+// the PV product, and the chain S - softmax - PV leaves the tensor core idle
+// half the time (measured: 155 us against 173 for 1024 queries over 8192 keys,
+// 32 heads). Here S of the next tile is issued as soon as the softmax warps have
+// the present one in registers, and PV runs under the next tile's softmax.
 // Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer, 2-5 / 6-9 softmax and
 // epilogue of query tile 0 / 1. Every mbarrier wait is bounded; on timeout the
 // CTA records an error, drains its copies and MMAs, frees TMEM and exits.
@@ -37,8 +38,8 @@ namespace {
 constexpr int D = 128;
 constexpr int BQ = 128;    // rows per query tile
 constexpr int QT = 2;      // query tiles per CTA
-constexpr int BKV = 128;   // keys per tile
-constexpr int NS = 2;      // K and V stages
+constexpr int BKV = 64;    // keys per tile
+constexpr int NS = 4;      // K and V stages
 constexpr int PAGE = 16;
 constexpr int kTilePages = BKV / PAGE;
 constexpr int kThreads = 320;
@@ -77,6 +78,28 @@ MBX_DEVICE void set_err(uint32_t* err, uint32_t code, volatile int* abort) {
   if (err) atomicCAS(err, 0u, code);
 }
 
+// tc::mbar_wait for waits that last: each try suspends the thread for up to 10 us
+// unless the phase completes. The issuing threads wait most of the time and
+// share their scheduler with softmax warps, which a tight loop would slow down.
+MBX_DEVICE bool mbar_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort, uint64_t timeout_ns) {
+  auto try_wait = [&] {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(tc::smem_u32(bar)), "r"(parity), "r"(10000u)
+        : "memory");
+    return ok != 0;
+  };
+  if (try_wait()) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!try_wait())
+    if (*abort || globaltimer_ns() - t0 > timeout_ns) return false;
+  return true;
+}
+
 // D[tmem] (+)= A[tmem, bf16 pairs in 32-bit columns] * B[smem].
 MBX_DEVICE void mma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -100,7 +123,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* v_full = k_empty + NS;       // [NS]
   uint64_t* v_empty = v_full + NS;       // [NS]
   uint64_t* s_full = v_empty + NS;       // [QT]
-  uint64_t* p_full = s_full + QT;        // [QT]
+  uint64_t* s_empty = s_full + QT;       // [QT]
+  uint64_t* p_full = s_empty + QT;       // [QT]
   uint64_t* pv_done = p_full + QT;       // [QT]
   uint64_t* mma_done = pv_done + QT;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
@@ -143,6 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int t = 0; t < QT; ++t) {
       tc::mbar_init(&s_full[t], 1);
+      tc::mbar_init(&s_empty[t], 4);
       tc::mbar_init(&p_full[t], 4);
       tc::mbar_init(&pv_done[t], 1);
     }
@@ -158,7 +183,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  auto tS = [&](int t) { return tmem + (uint32_t)(t * BKV); };  // S, then P in its first 64 columns
+  auto tS = [&](int t) { return tmem + (uint32_t)(t * BKV); };
+  auto tP = [&](int t) { return tmem + (uint32_t)(QT * BKV + t * (BKV / 2)); };
   auto tO = [&](int t) { return tmem + 256u + (uint32_t)(t * D); };
 
   if (warp == 0) {
@@ -190,13 +216,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < n_cta && !*abort; ++j, ++issued) {
         const int s = j % NS;
         const uint32_t parity = ((j / NS) & 1) ^ 1;
-        if (!tc::mbar_wait(&k_empty[s], parity, abort, a.timeout_ns)) {
+        if (!mbar_wait_long(&k_empty[s], parity, abort, a.timeout_ns)) {
           set_err(a.err, 21, abort);
           break;
         }
         tc::mbar_arrive_expect_tx(&k_full[s], kKVBytes);
         load(smem + Smem::kK + s * kKVBytes, &tmK, &tmK1, &k_full[s], j);
-        if (!tc::mbar_wait(&v_empty[s], parity, abort, a.timeout_ns)) {
+        if (!mbar_wait_long(&v_empty[s], parity, abort, a.timeout_ns)) {
           set_err(a.err, 21, abort);
           volatile int never = 0;
           tc::mbar_wait(&k_full[s], (j / NS) & 1, &never, 200000000ull);  // the K copy just issued
@@ -220,54 +246,54 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t idO = tc::idesc_bf16_f32_major(BQ, D, 0, 1);    // P in TMEM, V MN-major
       bool ok = true;
       auto wait = [&](uint64_t* bar, int parity) {
-        if (ok && !tc::mbar_wait(bar, parity, abort, a.timeout_ns)) {
+        if (ok && !mbar_wait_long(bar, parity, abort, a.timeout_ns)) {
           set_err(a.err, 22, abort);
           ok = false;
         }
         tc::tc_fence_after();
         return ok;
       };
+      // descriptors of the operands' beginnings; an offset adds its 16-byte units
+      const uint64_t dQ = tc::sw128_desc(tc::smem_u32(smem + Smem::kQ), 16, 1024);
+      const uint64_t dK = tc::sw128_desc(tc::smem_u32(smem + Smem::kK), 16, 1024);
+      const uint64_t dV = tc::sw128_desc(tc::smem_u32(smem + Smem::kV), kKVChunk, 1024);
       auto issue_s = [&](int t, int j) {
-        const uint32_t sQ = tc::smem_u32(smem + Smem::kQ + t * kQBytes);
-        const uint32_t sK = tc::smem_u32(smem + Smem::kK + (j % NS) * kKVBytes);
+        const uint64_t q = dQ + t * (kQBytes >> 4), k = dK + (j % NS) * (kKVBytes >> 4);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kQChunk + (kk & 3) * 32;  // kQChunk == kKVChunk
-          tc::mma_bf16(tS(t), tc::sw128_desc(sQ + off, 16, 1024), tc::sw128_desc(sK + off, 16, 1024), idS,
-                       kk > 0 ? 1u : 0u);
-        }
+        for (int kk = 0; kk < D / 16; ++kk)
+          tc::mma_bf16(tS(t), q + (((kk >> 2) * kQChunk + (kk & 3) * 32) >> 4),
+                       k + (((kk >> 2) * kKVChunk + (kk & 3) * 32) >> 4), idS, kk > 0 ? 1u : 0u);
         tc::mma_commit(&s_full[t]);
       };
-      static_assert(kQChunk == kKVChunk, "one offset for both operands of S");
       if (n_cta > 0 && wait(q_full, 0) && wait(&k_full[0], 0)) {
 #pragma unroll
         for (int t = 0; t < QT; ++t)
           if (nt[t] > 0) issue_s(t, 0);
         tc::mma_commit(&k_empty[0]);
       }
-      for (int j = 0; ok && j < n_cta; ++j) {
-        if (!wait(&v_full[j % NS], (j / NS) & 1)) break;
-        const bool more = j + 1 < n_cta;
-        if (more && !wait(&k_full[(j + 1) % NS], ((j + 1) / NS) & 1)) break;
-        const uint32_t sV = tc::smem_u32(smem + Smem::kV + (j % NS) * kKVBytes);
+      // Each tile's products in the order in which its softmax lets them go: P_{j-1}
+      // is stored before S_j is read out. Tile 0's come first, so the two tiles
+      // settle half a turn apart, one's products under the other's softmax.
+      for (int j = 0; ok && j <= n_cta; ++j) {
+        const bool has_v = j >= 1, has_k = j + 1 < n_cta;
+        const int vs = (j + NS - 1) % NS, ks = (j + 1) % NS;
+        if (has_v && !wait(&v_full[vs], ((j - 1) / NS) & 1)) break;
+        const uint64_t v = dV + vs * (kKVBytes >> 4);
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-          if (j < nt[t]) {
-            if (!wait(&p_full[t], j & 1)) break;
+          if (has_v && j - 1 < nt[t] && wait(&p_full[t], (j - 1) & 1)) {
 #pragma unroll
             for (int kk = 0; kk < BKV / 16; ++kk)
               // P: 16 keys = 8 columns; V: 16 key rows of 128 B, the dims' halves a chunk apart
-              mma_bf16_ts(tO(t), tS(t) + kk * 8, tc::sw128_desc(sV + kk * 16 * 128, kKVChunk, 1024), idO,
-                          (j > 0 || kk > 0) ? 1u : 0u);
+              mma_bf16_ts(tO(t), tP(t) + kk * 8, v + (kk * 16 * 128 >> 4), idO, (j > 1 || kk > 0) ? 1u : 0u);
             tc::mma_commit(&pv_done[t]);
           }
-          if (t == QT - 1) tc::mma_commit(&v_empty[j % NS]);
-          if (j + 1 < nt[t]) {
-            if (!wait(&pv_done[t], j & 1)) break;  // S overwrites the P that PV reads
-            issue_s(t, j + 1);
-          }
+          if (has_k && t == 0 && !wait(&k_full[ks], ((j + 1) / NS) & 1)) break;
+          if (has_k && j + 1 < nt[t] && wait(&s_empty[t], j & 1)) issue_s(t, j + 1);
         }
-        if (ok && more) tc::mma_commit(&k_empty[(j + 1) % NS]);
+        if (!ok) break;
+        if (has_v) tc::mma_commit(&v_empty[vs]);
+        if (has_k) tc::mma_commit(&k_empty[ks]);
       }
       tc::mma_commit(mma_done);
       volatile int never = 0;
@@ -285,7 +311,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < my_n; ++j) {
-      // S_j is complete, and with it (it was issued after that) the product P_{j-1} V
       if (!tc::mbar_wait(&s_full[t], j & 1, abort, a.timeout_ns)) {
         if (lane == 0) set_err(a.err, 23, abort);
         ok = false;
@@ -297,6 +322,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < BKV / 32; ++c)
         tc::tmem_ld_32x32b_x32(tS(t) + lane_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&v[c * 32]));
       tc::tmem_ld_wait();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&s_empty[t]);
       const int lim = min(q_pos + 1, kvend_t[t]) - (tb + j) * BKV;  // the row sees the tile's first lim keys
       if (lim < BKV) {
 #pragma unroll
@@ -320,18 +348,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float corr = (m == -INFINITY || !grow) ? 1.f : tc::ex2(m - m_new);
       const float neg = m_new == -INFINITY ? 0.f : -m_new;  // a row without keys so far: 2^(-inf) = 0
       float s8[8] = {};
+      uint32_t pk[BKV / 2];
 #pragma unroll
-      for (int c = 0; c < BKV / 64; ++c) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int i = 0; i < 64; i += 2) {
-          const float p0 = tc::ex2(fmaf(__uint_as_float(v[c * 64 + i]), sc, neg));
-          const float p1 = tc::ex2(fmaf(__uint_as_float(v[c * 64 + i + 1]), sc, neg));
-          s8[(i >> 1) & 7] += p0 + p1;
-          const __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
-          pk[i / 2] = *reinterpret_cast<const uint32_t*>(&h2);
-        }
-        tc::tmem_st_32x32b_x32(tS(t) + lane_addr + c * 32, pk);
+      for (int i = 0; i < BKV; i += 2) {
+        const float p0 = tc::ex2(fmaf(__uint_as_float(v[i]), sc, neg));
+        const float p1 = tc::ex2(fmaf(__uint_as_float(v[i + 1]), sc, neg));
+        s8[(i >> 1) & 7] += p0 + p1;
+        const __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
+        pk[i / 2] = *reinterpret_cast<const uint32_t*>(&h2);
       }
 #pragma unroll
       for (int k = 4; k > 0; k >>= 1)
@@ -339,6 +363,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int q = 0; q < k; ++q) s8[q] += s8[q + k];
       l = l * corr + s8[0];
       m = m_new;
+      if (j > 0) {  // P_{j-1} V is complete before P is overwritten and O rescaled
+        if (!tc::mbar_wait(&pv_done[t], (j - 1) & 1, abort, a.timeout_ns)) {
+          if (lane == 0) set_err(a.err, 23, abort);
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+      }
+      tc::tmem_st_32x32b_x32(tP(t) + lane_addr, pk);
       if (j > 0 && __any_sync(0xffffffffu, corr < 1.f)) {
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
