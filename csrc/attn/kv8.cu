@@ -1154,10 +1154,13 @@ void rope_and_cache_kv8_launch(const void* qkv, const int* pos, const float* cos
   a.max_pos = (int)max_pos;
   a.nq = nq;
   a.nkv = nkv;
-  // Tokens per k/v CTA: one where there are few; more for many, since every CTA
-  // looks through all later slots for its own.
-  const int tokens = T <= 128 ? 1 : (int)std::min<int64_t>(kMaxTokens, std::max<int64_t>(4, (T + 1023) / 1024));
-  const int passes = T * nq >= 16384 ? 2 : 1;
+  // Tokens per k/v CTA: one where there are few (64 tokens of 32 + 2 x 8 heads:
+  // 3.0 us, two 3.6, four 5.2); more for many, since every CTA looks through all
+  // later slots for its own (8005 tokens of 64 + 2 x 8: 2 tokens 88 us, 16
+  // tokens 65). q passes per warp share the angles: one, two and four measure
+  // 81, 69 and 65 us there, and 10.2, 8.0 and 8.6 at 1024 tokens of 32 heads.
+  const int tokens = T <= 128 ? 1 : (int)std::min<int64_t>(kMaxTokens, std::max<int64_t>(2, (T + 511) / 512));
+  const int passes = T * nq >= 1 << 18 ? 4 : T * nq >= 1 << 14 ? 2 : 1;
   const int64_t kv_ctas = (T + tokens - 1) / tokens;
   const int64_t q_tasks = T * ((nq + 4 * passes - 1) / (4 * passes));
   const dim3 grid((unsigned)(kv_ctas + (q_tasks + kAppendWarps - 1) / kAppendWarps));
