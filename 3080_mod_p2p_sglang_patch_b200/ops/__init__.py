@@ -399,7 +399,8 @@ class PagePlan:
 def page_plan(kv_lens, columns: int) -> PagePlan:
     """The plan (on the CPU) that packs the pages of requests of ``kv_lens``
     tokens one after another; ``columns`` is the block table's width. Without a
-    plan every request gets ``columns`` pages of scratch."""
+    plan every request gets ``columns`` pages of scratch (prefill attention
+    counts on a request's pages being consecutive)."""
     counts = torch.tensor([max(0, min(columns, -(-int(n) // 16))) for n in kv_lens], dtype=torch.int32)
     i = torch.arange(columns, dtype=torch.int32)[None, :]
     start = (counts.cumsum(0, dtype=torch.int32) - counts)[:, None]
@@ -454,7 +455,9 @@ def prefill_attention(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, sca
     ``prefill_splits``); the partials are merged by a combine kernel.
 
     ``Fp8Pages`` caches are read back to bf16 scratch pages first
-    (``read_pages``; placed by ``plan``, a ``page_plan`` on the device)."""
+    (``read_pages``; placed by ``plan``, a ``page_plan`` of the same lengths,
+    its table on the device). There ``scale`` has to be positive and rows that
+    see no key are zeros."""
     if out is None:
         out = torch.empty_like(q)
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])

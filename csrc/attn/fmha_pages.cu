@@ -14,20 +14,24 @@
 // TMEM 1.25 times. Tiles of 128 keys would read Q half as often, but then P has
 // to lie over S (TMEM is 512 columns, O takes 256), the next S has to wait for
 // the PV product, and the chain S - softmax - PV leaves the tensor core idle
-// half the time (measured: 155 us against 173 for 1024 queries over 8192 keys,
-// 32 heads). Here S of the next tile is issued as soon as the softmax warps have
-// the present one in registers, and PV runs under the next tile's softmax.
+// half the time. Here S of the next tile is issued as soon as the softmax warps
+// have the present one in registers, and PV runs under the next tile's softmax.
+// Measured, 1024 queries over 8192 keys of 32 heads, read-back (7.5 us) included:
+// 149 us, 867 TFLOP/s (53 % of the measured GEMM rate; 128 of 148 SMs have a
+// CTA); the kernel over the cache itself on the same pages 173, 128-key tiles
+// 155. A turn of 64 keys for both tiles takes 2300 cycles, 1280 of them tensor
+// work: the softmax warps of the two tiles share a scheduler and its exponential
+// unit and lengthen one another. Two threads per row (165 us), packed FMAs (150)
+// and polynomials for some of the exponentials (153 to 159) did not help.
 // Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer, 2-5 / 6-9 softmax and
 // epilogue of query tile 0 / 1. Every mbarrier wait is bounded; on timeout the
 // CTA records an error, drains its copies and MMAs, frees TMEM and exits.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <functional>
 #include <mutex>
 #include <stdexcept>
 #include <string>
-#include <unordered_map>
 
 #include "../gemm/tcgen05.cuh"
 #include "../kernels.h"

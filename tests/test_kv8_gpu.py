@@ -522,6 +522,67 @@ def test_prefill_over_the_cache(nq, nkv, splits, planned):
     _check_prefill(out, q, k8, v8, table, q_lens, kv_lens)
 
 
+def _prefill(ops, q, k8, v8, q_lens, kvl, table, **kw):
+    cu = torch.tensor([0] + q_lens, device="cuda").cumsum(0).to(torch.int32)
+    return ops.prefill_attention(q, k8, v8, cu, kvl, table, ops.prefill_tiles(q_lens).cuda(), **kw)
+
+
+@pytest.mark.parametrize("kv_lens,q_lens", [([63], [63]), ([64], [1]), ([65], [65]), ([129], [2]), ([1], [1]),
+                                            ([2000, 256, 511], [600, 256, 255]), ([1027], [515]),
+                                            ([300, 17, 129, 640], [257, 17, 128, 1])])
+def test_prefill_tile_borders(kv_lens, q_lens):
+    ops = sub("ops")
+    nq, nkv = 4, 2
+    k8, v8, kvl, table = _cache(kv_lens, nkv, seed=kv_lens[0], spread=3)
+    q = torch.randn(sum(q_lens), nq, D, device="cuda", generator=_gen(2)).to(torch.bfloat16)
+    out = _prefill(ops, q, k8, v8, q_lens, kvl, table)
+    _check_prefill(out, q, k8, v8, table, q_lens, kv_lens)
+    assert ops.gemm_error() == 0
+
+
+def test_prefill_rows_without_keys_and_neighbours_with_nan():
+    """A request without cached keys gives zeros; NaN rows of one request stay
+    in it, although its pages lie next to the others' in the scratch."""
+    ops = sub("ops")
+    kv_lens, q_lens, nq, nkv = [70, 0, 30, 100], [20, 9, 30, 5], 4, 2
+    k8, v8, kvl, table = _cache(kv_lens, nkv, seed=3)
+    q = torch.randn(sum(q_lens), nq, D, device="cuda", generator=_gen(2)).to(torch.bfloat16)
+    for splits in (1, 2):
+        out = _prefill(ops, q, k8, v8, q_lens, kvl, table, splits=splits)
+        assert (out[20:29] == 0).all()
+        for r, a, b in ((0, 0, 20), (2, 29, 59), (3, 59, 64)):
+            _check_prefill(out[a:b], q[a:b], k8, v8, table[r:r + 1], [b - a], kv_lens[r:r + 1])
+    good = _prefill(ops, q, k8, v8, q_lens, kvl, table)
+    _bytes_of(v8)[table[2, 0].long()] = 0x7F
+    bad = _prefill(ops, q, k8, v8, q_lens, kvl, table)
+    assert torch.isnan(bad[29:59]).all()
+    assert torch.equal(bad[:29], good[:29]) and torch.equal(bad[59:], good[59:])
+    # nothing to attend with, and no columns at all
+    assert _prefill(ops, q[:0], k8, v8, [], kvl[:0], table[:0]).shape == (0, nq, D)
+    assert (_prefill(ops, q[:5], k8, v8, [5], kvl[:1], table[:1, :0]) == 0).all()
+    with pytest.raises(RuntimeError, match="positive scale"):
+        _prefill(ops, q, k8, v8, q_lens, kvl, table, scale=0.0)
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_decode_drawn_batches(seed):
+    """Batches of mixed lengths, so that runs of the work list begin and end
+    anywhere in pairs, pages and the room behind them."""
+    import random
+
+    ops = sub("ops")
+    rng = random.Random(seed)
+    nkv = rng.choice((1, 2, 3, 8))
+    nq = nkv * rng.choice((1, 2, 5, 8, 11, 16))
+    B = rng.choice((1, 2, 7, 40, 150, 333))
+    top = rng.choice((40, 200, 900, 6000)) if B < 100 else rng.choice((40, 200, 700))
+    lens = [0 if rng.random() < 0.1 else rng.choice((rng.randint(1, 30), rng.randint(1, top))) for _ in range(B)]
+    k8, v8, kvl, table = _cache(lens, nkv, seed=seed, columns=-(-max(max(lens), 1) // PAGE) + rng.randint(0, 3))
+    q = torch.randn(B, nq, D, device="cuda", generator=_gen(seed)).to(torch.bfloat16)
+    out = ops.decode_attention(q, k8, v8, kvl, table)
+    _check_decode(out, q, k8, v8, table, lens)
+
+
 # ---------------------------------------------------------------- together
 def test_append_then_attend():
     """A prompt in two chunks, then tokens one by one, as a model's layer
