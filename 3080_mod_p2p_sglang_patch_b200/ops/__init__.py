@@ -437,7 +437,7 @@ _PAGE_IDS = {}  # device -> [0, 1, 2, ...] in growing lengths: the block table o
 
 
 def _page_ids(n, device):
-    if torch.cuda.is_current_stream_capturing():
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
         return torch.arange(n, dtype=torch.int32, device=device)
     ids = _PAGE_IDS.setdefault(device, [])
     if not ids or ids[-1].numel() < n:
@@ -458,11 +458,11 @@ def prefill_attention(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, sca
     (``read_pages``; placed by ``plan``, a ``page_plan`` of the same lengths,
     its table on the device). There ``scale`` has to be positive and rows that
     see no key are zeros."""
-    if out is None:
-        out = torch.empty_like(q)
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     if _is_fp8(k_cache, v_cache):
         return _prefill_fp8(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, scale, out, splits, plan)
+    if out is None:
+        out = torch.empty_like(q)
     po = pl = None
     if splits > 1:
         T, nq, _ = q.shape
@@ -474,18 +474,16 @@ def prefill_attention(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, sca
 
 
 def _prefill_fp8(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, scale, out, splits, plan):
-    # Scratch comes from the caching allocator call by call, not from the shared
-    # workspace: two captured graphs (or two streams) never meet in it.
-    R, cols = block_table.shape
-    pages = R * cols if plan is None else plan.pages
-    table = _page_ids(pages, q.device).view(R, cols) if plan is None else plan.table
-    kv = torch.empty((2, max(1, pages)) + tuple(k_cache.shape[1:]), dtype=torch.bfloat16, device=q.device)
-    k, v = kv.unbind(0)
-    read_pages(k_cache, v_cache, block_table, kv_len, out_table=table, k_out=k, v_out=v)
-    cuda_ext().prefill_attention_pages(q, k, v, out, cu_q, kv_len, table, tiles, scale, workspace(q.device).err,
-                                       splits)
-    launches.add(2 if splits > 1 else 1)
-    return out
+    if plan is None:
+        R, cols = block_table.shape
+        pages = R * cols
+        table = _page_ids(pages, q.device).view(R, cols)
+    else:
+        table, pages = plan.table, plan.pages
+    launches.add(3 if splits > 1 else 2)
+    err = workspace(q.device).err if q.is_cuda else None
+    return cuda_ext().prefill_attention_kv8(q, k_cache.values, k_cache.exps, v_cache.values, v_cache.exps, out, cu_q,
+                                            kv_len, block_table, table, pages, tiles, scale, err, splits)
 
 
 def prefill_attention_mma(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles64, scale=None, out=None):

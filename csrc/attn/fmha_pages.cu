@@ -63,7 +63,7 @@ struct PagesArgs {
   const int2* tiles;     // (request, q offset): 256-row query-tile pairs
   float* part_o;         // splits > 1: [T, nq, splits, D]
   float* part_lse;       //             [T, nq, splits]
-  int splits, cols, nq, nkv;
+  int splits, cols, nq, nkv, pages;  // pages: of K, behind which V's lie
   float scale_log2;
   uint32_t* err;
   uint64_t timeout_ns;
@@ -115,9 +115,8 @@ MBX_DEVICE void mma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, ui
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
-    fmha_pages_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmK1,
-                      const __grid_constant__ CUtensorMap tmV1, PagesArgs a) {
+    fmha_pages_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKV,
+                      const __grid_constant__ CUtensorMap tmKV1, PagesArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBar);
@@ -205,15 +204,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       // A tile whose pages all hold keys is one box per 64 dims; in the last one
       // the pages behind the last are that page again (masked keys have to be
       // finite, and what follows in the scratch is another request's).
-      auto load = [&](uint8_t* dst, const CUtensorMap* map, const CUtensorMap* map1, uint64_t* bar, int j) {
+      auto load = [&](uint8_t* dst, int first, uint64_t* bar, int j) {
         const int p = (tb + j) * kTilePages;
         for (int c = 0; c < 2; ++c) {
           if (p + kTilePages - 1 <= last_page) {
-            tc::tma_load_4d(dst + c * kKVChunk, map, bar, c * 64, 0, kvh, page0 + p);
+            tc::tma_load_4d(dst + c * kKVChunk, &tmKV, bar, c * 64, 0, kvh, first + p);
           } else {
             for (int i = 0; i < kTilePages; ++i)
-              tc::tma_load_4d(dst + c * kKVChunk + i * (PAGE * 128), map1, bar, c * 64, 0, kvh,
-                              page0 + min(p + i, last_page));
+              tc::tma_load_4d(dst + c * kKVChunk + i * (PAGE * 128), &tmKV1, bar, c * 64, 0, kvh,
+                              first + min(p + i, last_page));
           }
         }
       };
@@ -225,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         tc::mbar_arrive_expect_tx(&k_full[s], kKVBytes);
-        load(smem + Smem::kK + s * kKVBytes, &tmK, &tmK1, &k_full[s], j);
+        load(smem + Smem::kK + s * kKVBytes, page0, &k_full[s], j);
         if (!mbar_wait_long(&v_empty[s], parity, abort, a.timeout_ns)) {
           set_err(a.err, 21, abort);
           volatile int never = 0;
@@ -233,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         tc::mbar_arrive_expect_tx(&v_full[s], kKVBytes);
-        load(smem + Smem::kV + s * kKVBytes, &tmV, &tmV1, &v_full[s], j);
+        load(smem + Smem::kV + s * kKVBytes, a.pages + page0, &v_full[s], j);
       }
       // copies in flight land before the CTA leaves
       volatile int never = 0;
@@ -472,10 +471,10 @@ CUtensorMap encode(const void* base, int rank, const cuuint64_t* dims, const cuu
 
 }  // namespace
 
-void prefill_attention_pages_launch(const void* q, const void* kp, const void* vp, void* o, const int* cu_q,
-                                    const int* kv_len, const int* table, int cols, const int* tiles, int n_tiles,
-                                    int T, int nq, int nkv, int64_t pages, float scale, int splits, float* part_o,
-                                    float* part_lse, uint32_t* err, cudaStream_t s) {
+void prefill_attention_pages_launch(const void* q, const void* kv, void* o, const int* cu_q, const int* kv_len,
+                                    const int* table, int cols, const int* tiles, int n_tiles, int T, int nq, int nkv,
+                                    int pages, float scale, int splits, float* part_o, float* part_lse, uint32_t* err,
+                                    cudaStream_t s) {
   if (n_tiles == 0 || T == 0) return;
   if (nq % nkv != 0) throw std::runtime_error("fmha: nq must be a multiple of nkv");
   if (splits > 1 && (!part_o || !part_lse)) throw std::runtime_error("fmha: split-KV needs scratch buffers");
@@ -484,20 +483,19 @@ void prefill_attention_pages_launch(const void* q, const void* kp, const void* v
   cuuint64_t qs[2] = {(cuuint64_t)D * 2, (cuuint64_t)nq * D * 2};
   const cuuint32_t qb[3] = {64, 1, BQ};
   const CUtensorMap tq = encode(q, 3, qd, qs, qb);
-  // pages: [pages, nkv, PAGE, D] -> dims {D, PAGE, nkv, pages}, boxes of a tile's pages and of one
-  auto page_map = [&](const void* base, cuuint32_t n) {
-    cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)PAGE, (cuuint64_t)nkv, (cuuint64_t)pages};
+  // K's pages, then V's: [2 pages, nkv, PAGE, D] -> dims {D, PAGE, nkv, 2 pages}, boxes of a tile's pages and of one
+  auto page_map = [&](cuuint32_t n) {
+    cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)PAGE, (cuuint64_t)nkv, 2 * (cuuint64_t)pages};
     cuuint64_t str[3] = {(cuuint64_t)D * 2, (cuuint64_t)PAGE * D * 2, (cuuint64_t)nkv * PAGE * D * 2};
     const cuuint32_t box[4] = {64, PAGE, 1, n};
-    return encode(base, 4, dims, str, box);
+    return encode(kv, 4, dims, str, box);
   };
-  const CUtensorMap tk = page_map(kp, kTilePages), tv = page_map(vp, kTilePages);
-  const CUtensorMap tk1 = page_map(kp, 1), tv1 = page_map(vp, 1);
+  const CUtensorMap tkv = page_map(kTilePages), tkv1 = page_map(1);
   PagesArgs a{static_cast<__nv_bfloat16*>(o), cu_q, kv_len, table, reinterpret_cast<const int2*>(tiles), part_o,
-              part_lse, std::max(1, splits), cols, nq, nkv, scale * 1.4426950408889634f, err, 2000000000ull};
+              part_lse, std::max(1, splits), cols, nq, nkv, pages, scale * 1.4426950408889634f, err, 2000000000ull};
   static SmemLimit limit;
   limit.ensure((const void*)fmha_pages_kernel, Smem::kTotal);
-  launch_k(fmha_pages_kernel, dim3(n_tiles, nq, a.splits), dim3(kThreads), Smem::kTotal, s, tq, tk, tv, tk1, tv1, a);
+  launch_k(fmha_pages_kernel, dim3(n_tiles, nq, a.splits), dim3(kThreads), Smem::kTotal, s, tq, tkv, tkv1, a);
   MBX_CUDA_CHECK(cudaGetLastError());
   if (a.splits > 1) attn_combine_launch(part_o, part_lse, (int64_t)T * nq, a.splits, o, s);
 }

@@ -660,38 +660,53 @@ void read_pages_kv8(const torch::Tensor& kv, const torch::Tensor& ke, const torc
                         cur_stream());
 }
 
-// Causal attention of a prefill batch over the pages that read_pages_kv8 wrote
-// (k, v [pages, nkv, 16, 128], placed by a packed `table`); its split-KV
+// Causal attention of a prefill batch over an 8-bit cache: its pages read back
+// to scratch, placed by `table` (packed, `pages` in all; without one every
+// request gets a page per column), then the tensor-core kernel over them. The
 // scratch comes from the caching allocator, so that calls on other streams and
 // in other graphs have their own.
-torch::Tensor prefill_attention_pages(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
-                                      const torch::Tensor& out, const torch::Tensor& cu_q, const torch::Tensor& kv_len,
-                                      const torch::Tensor& table, const torch::Tensor& tiles, double scale,
-                                      const torch::Tensor& err, int64_t splits) {
+torch::Tensor prefill_attention_kv8(const torch::Tensor& q, const torch::Tensor& kv, const torch::Tensor& ke,
+                                    const torch::Tensor& vv, const torch::Tensor& ve,
+                                    const c10::optional<torch::Tensor>& out_opt, const torch::Tensor& cu_q,
+                                    const torch::Tensor& kv_len, const torch::Tensor& block_table,
+                                    const torch::Tensor& table, int64_t pages, const torch::Tensor& tiles,
+                                    double scale, const c10::optional<torch::Tensor>& err, int64_t splits) {
   check_dense(q, "q", torch::kBFloat16);
   TORCH_CHECK(q.dim() == 3 && q.size(2) == 128, "q must be [T, nq, 128]");
-  check_dense(out, "out", torch::kBFloat16);
-  TORCH_CHECK(out.sizes() == q.sizes(), "out must have q's shape");
-  check_dense(k, "k", torch::kBFloat16);
-  check_dense(v, "v", torch::kBFloat16);
-  TORCH_CHECK(k.dim() == 4 && k.size(2) == 16 && k.size(3) == 128 && v.sizes() == k.sizes() && k.size(0) > 0 &&
-                  k.size(0) < (int64_t)1 << 31,
-              "k and v must be [pages, nkv, 16, 128]");
-  const int64_t T = q.size(0), nq = q.size(1), nkv = k.size(1);
-  TORCH_CHECK(nkv > 0 && nq > 0 && nq % nkv == 0, "q heads must be a multiple of the kv heads");
+  if (out_opt.has_value()) {
+    check_dense(*out_opt, "out", torch::kBFloat16);
+    TORCH_CHECK(out_opt->sizes() == q.sizes(), "out must have q's shape");
+  }
+  TORCH_CHECK(kv.dim() == 4, "k_cache values must be float8_e4m3fn [blocks, nkv, 16, 128] with at least one block");
+  const int64_t T = q.size(0), nq = q.size(1), nkv = kv.size(1);
+  const Kv8Cache c = kv8_cache(kv, ke, vv, ve, nkv);
+  TORCH_CHECK(nq > 0 && nq % nkv == 0, "q heads must be a multiple of the kv heads");
   check_lens(kv_len);
   const int64_t R = kv_len.numel();
   TORCH_CHECK(cu_q.scalar_type() == torch::kInt32 && cu_q.is_contiguous() && cu_q.numel() == R + 1,
               "cu_q must be contiguous int32 [requests + 1]");
+  check_table(block_table, "block_table", R);
+  const int64_t cols = block_table.size(1);
   check_table(table, "plan table", R);
-  TORCH_CHECK(table.is_contiguous(), "plan table must be contiguous");
+  TORCH_CHECK(table.is_contiguous() && table.size(1) == cols, "plan table must be contiguous, as wide as block_table");
+  TORCH_CHECK(R * cols * nkv < (int64_t)1 << 31 && pages >= 0 && pages < (int64_t)1 << 30,
+              "prefill: too many pages, or fewer than none");
   TORCH_CHECK(tiles.scalar_type() == torch::kInt32 && tiles.is_contiguous() && tiles.dim() == 2 && tiles.size(1) == 2,
               "tiles must be contiguous int32 [n, 2]");
   TORCH_CHECK(scale > 0, "prefill attention needs a positive scale");
   TORCH_CHECK(splits >= 1 && splits < 65536 && nq < 65536, "splits and q heads must lie in 1 to 65535");
-  check_devices({{"q", &q}, {"k", &k}, {"v", &v}, {"out", &out}, {"cu_q", &cu_q}, {"kv_len", &kv_len},
-                 {"plan table", &table}, {"tiles", &tiles}, {"err", &err}});
+  check_devices({{"q", &q}, {"k_cache", &kv}, {"k_cache exps", &ke}, {"v_cache", &vv}, {"v_cache exps", &ve},
+                 {"out", out_opt ? &*out_opt : nullptr}, {"cu_q", &cu_q}, {"kv_len", &kv_len},
+                 {"block_table", &block_table}, {"plan table", &table}, {"tiles", &tiles},
+                 {"err", err ? &*err : nullptr}});
   const at::cuda::CUDAGuard guard(q.device());
+  const torch::Tensor out = out_opt ? *out_opt : torch::empty_like(q);
+  const int64_t n = std::max<int64_t>(1, pages);
+  const torch::Tensor scratch = torch::empty({2, n, nkv, 16, 128}, q.options());
+  char* const k = static_cast<char*>(scratch.data_ptr());
+  const cudaStream_t stream = cur_stream();
+  read_pages_kv8_launch(c, (int)nkv, block_table.data_ptr<int>(), block_table.stride(0), table.data_ptr<int>(), cols,
+                        kv_len.data_ptr<int>(), (int)R, (int)cols, k, k + n * nkv * 16 * 128 * 2, pages, stream);
   torch::Tensor part;
   float *po = nullptr, *pl = nullptr;
   if (splits > 1) {
@@ -699,11 +714,10 @@ torch::Tensor prefill_attention_pages(const torch::Tensor& q, const torch::Tenso
     po = part.data_ptr<float>();
     pl = po + T * nq * splits * 128;
   }
-  prefill_attention_pages_launch(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_q.data_ptr<int>(),
-                                 kv_len.data_ptr<int>(), table.data_ptr<int>(), (int)table.size(1),
-                                 tiles.data_ptr<int>(), (int)tiles.size(0), (int)T, (int)nq, (int)nkv, k.size(0),
-                                 (float)scale, (int)splits, po, pl,
-                                 reinterpret_cast<uint32_t*>(err.data_ptr<int>()), cur_stream());
+  prefill_attention_pages_launch(q.data_ptr(), k, out.data_ptr(), cu_q.data_ptr<int>(), kv_len.data_ptr<int>(),
+                                 table.data_ptr<int>(), (int)cols, tiles.data_ptr<int>(), (int)tiles.size(0), (int)T,
+                                 (int)nq, (int)nkv, (int)n, (float)scale, (int)splits, po, pl,
+                                 err ? reinterpret_cast<uint32_t*>(err->data_ptr<int>()) : nullptr, stream);
   return out;
 }
 
@@ -912,6 +926,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("scale"), py::arg("counters") = c10::nullopt);
   m.def("rope_and_cache_kv8", &rope_and_cache_kv8);
   m.def("read_pages_kv8", &read_pages_kv8);
-  m.def("prefill_attention_pages", &prefill_attention_pages);
+  m.def("prefill_attention_kv8", &prefill_attention_kv8);
   m.def("decode_attention_kv8", &decode_attention_kv8);
 }

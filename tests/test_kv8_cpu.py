@@ -223,21 +223,27 @@ def test_refusals_of_head_counts_and_outputs():
 
 @needs_ext
 def test_refusals_of_prefill_attention():
-    """The binding behind prefill_attention over an 8-bit cache."""
-    C = sub("_ext").cuda_ext()
+    ops = sub("ops")
+    k, v = ops.fp8_cache(3, 2, "cpu")
     i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
     bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
-    good = dict(q=bf(5, 4, D), k=bf(6, 2, PAGE, D), v=bf(6, 2, PAGE, D), out=bf(5, 4, D), cu_q=i32(3), kv_len=i32(2),
-                table=i32(2, 3), tiles=i32(2, 2), scale=0.1, err=i32(1), splits=1)
+    good = dict(q=bf(5, 4, D), k_cache=k, v_cache=v, cu_q=i32(3), kv_len=i32(2), block_table=i32(2, 3),
+                tiles=i32(2, 2))
+    plan = ops.PagePlan
     for change, message in ((dict(q=bf(5, 4, 64)), "q must be"), (dict(out=bf(4, 4, D)), "out must have"),
-                            (dict(q=bf(5, 3, D), out=bf(5, 3, D)), "multiple of the kv heads"),
-                            (dict(k=bf(6, 2, 8, D)), "k and v must be"), (dict(v=bf(7, 2, PAGE, D)), "k and v must be"),
+                            (dict(q=bf(5, 3, D)), "multiple of the kv heads"),
+                            (dict(k_cache=ops.Fp8Pages(k.values[:2], k.exps)), "exps must be"),
                             (dict(cu_q=i32(2)), "cu_q must be"), (dict(kv_len=i32(2).long()), "kv_len must be"),
-                            (dict(table=i32(3, 3)), "plan table must be"), (dict(tiles=i32(2, 3)), "tiles must be"),
+                            (dict(block_table=i32(3, 3)), "block_table must be"),
+                            (dict(plan=plan(i32(3, 3), 4)), "plan table must be"),
+                            (dict(plan=plan(i32(2, 2), 4)), "plan table must be"),
+                            (dict(plan=plan(i32(2, 3), -1)), "pages"), (dict(tiles=i32(2, 3)), "tiles must be"),
                             (dict(scale=-1.0), "positive scale"), (dict(scale=float("nan")), "positive scale"),
                             (dict(splits=0), "splits"), ({}, "must be a CUDA tensor")):
         with pytest.raises(RuntimeError, match=message):
-            C.prefill_attention_pages(*{**good, **change}.values())
+            ops.prefill_attention(**{**good, **change})
+    with pytest.raises(TypeError, match="both be Fp8Pages"):
+        ops.prefill_attention(**{**good, "v_cache": bf(3, 2, PAGE, D)})
 
 
 # ---------------------------------------------------------------- the engine on an 8-bit cache
