@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
       int before = 0, b0 = 0;  // pages of the requests in front; first of the 1024 looked at
       int end = scan(sums);
 #pragma unroll 1
-      while (__shfl_sync(0xffffffffu, end, 31) * a.nkv <= u0) {
+      while (__shfl_sync(0xffffffffu, end, 31) * a.nkv <= u0 && b0 < a.B) {
         before = __shfl_sync(0xffffffffu, end, 31);
         b0 += 1024;
         sums = 0;
@@ -804,6 +804,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
       at.y = quotient(off, len);
       at.z = off - at.y * len;
       at.w = len - pad;
+      if (at.x >= a.B) left = 0;
     }
   } else {
     const int pair = plan.cut == kCta ? blockIdx.x : blockIdx.x * kW + warp;
@@ -832,7 +833,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
       ++c.b;
       c.pages = pages_in(next_keys);
 #pragma unroll 1
-      while (c.pages == 0) c.pages = pages_of(++c.b);
+      while (c.pages == 0 && ++c.b < a.B) c.pages = pages_of(c.b);
+      if (c.b >= a.B) c.left = 0;  // only where another stream shortened a length meanwhile
       return true;
     };
     if (use.p >= use.pages) {  // the run starts in the room behind a pair
@@ -950,7 +952,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
       if (!ends && use.left > 0) continue;
       // ---- the segment is done
       st.end();
-      const float vs = pow2(max(st.vr, -118) - 8);
+      // rows are divided by their sum here, partial ones too, and the weights' 2^8
+      // goes with the inverse: nothing on the way leaves fp32's normal range
+      // where the result does not
+      const float vs = pow2(max(st.vr, -126));
       if (seg_p0 == 0 && ends) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -958,12 +963,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
           for (int c = 0; c < 2; ++c) {
             const int head = n * 8 + 2 * t + c;
             if (head >= G) continue;
-            const float inv = vs * inverse(st.l[n][c]);
+            const float inv = inverse(st.l[n][c]) * 0x1p-8f;
             float f[16];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              f[2 * j] = st.o[n][j][c] * inv;
-              f[2 * j + 1] = st.o[n][j][2 + c] * inv;
+              f[2 * j] = st.o[n][j][c] * inv * vs;
+              f[2 * j + 1] = st.o[n][j][2 + c] * inv * vs;
             }
             __nv_bfloat16* dst = a.o + ((int64_t)use.b * a.nq + use.kvh * G + head) * D + g * 16;
             *reinterpret_cast<uint4*>(dst) = pack_from<__nv_bfloat16>(f);
@@ -982,10 +987,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
           for (int c = 0; c < 2; ++c) {
             const int head = n * 8 + 2 * t + c;
             if (head >= G) continue;
+            const float inv = inverse(st.l[n][c]) * 0x1p-8f;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               *reinterpret_cast<float2*>(po + head * kRow + g * 16 + 2 * j) =
-                  make_float2(st.o[n][j][c] * vs, st.o[n][j][2 + c] * vs);
+                  make_float2(st.o[n][j][c] * inv * vs, st.o[n][j][2 + c] * inv * vs);
             if (g == 0) ml[head] = make_float2(st.m[n][c], st.l[n][c]);
           }
         if (lane == 0) {
@@ -1003,7 +1009,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
         keys = use.b == b + 1 ? use_next_keys : keys_of(use.b);
         use_next_keys = keys_of(use.b + 1);
       }
-      if (NT > 1 || use.b > b + 1) load_query(use.b, use.kvh);
+      if (use.left > 0 && (NT > 1 || use.b > b + 1)) load_query(use.b, use.kvh);
     }
   }
   // requests without keys: zeros, by the CTAs in turn
@@ -1022,7 +1028,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
   // arrive: the CTAs' partials of a pair that reaches over CTAs. One code for
   // both (what runs once a launch waits for its instructions, too): partial 0
   // lies by itself, the others a stride apart. A warp per (chain, head): lane i
-  // has partial i's (m, l), so that the weights 2^(m_i - M) come at once and the
+  // has partial i's (m, l), so that the weights 2^(m_i - M) l_i come at once and the
   // rows (lane l: dims 4l..4l+3) are independent loads.
   const int f0 = lane < kW ? flags[0][lane] : 0, f1 = lane < kW ? flags[1][lane] : 0;
   const uint32_t held = __ballot_sync(0xffffffffu, f0 != 0), ended = __ballot_sync(0xffffffffu, f0 & kEnds),
@@ -1089,18 +1095,19 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
           }
           const float nm = fmaxf(M, warp_max(x.x));
           const float keep = merge_weight(M, nm);
-          const float w = has ? merge_weight(x.x, nm) : 0.f;
+          const float part = has ? merge_weight(x.x, nm) * x.y : 0.f;
+          const float sum = l * keep + warp_sum(part), inv = inverse(sum);
+          const float w = part * inv, old = l * keep * inv;
           M = nm;
-          l = l * keep + warp_sum(has ? w * x.y : 0.f);
-          o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+          l = sum;
+          o = make_float4(o.x * old, o.y * old, o.z * old, o.w * old);
 #pragma unroll
           for (int j = 0; j < kBlock; ++j)  // behind the last partial: its row again, weight 0
             add_scaled(o, __shfl_sync(0xffffffffu, w, j), y[j]);
         }
         if (whole) {
-          const float inv = inverse(l);
-          const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x * inv, o.y * inv);
-          const __nv_bfloat162 hi = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+          const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x, o.y);
+          const __nv_bfloat162 hi = __floats2bfloat162_rn(o.z, o.w);
           uint2 y;
           y.x = *reinterpret_cast<const uint32_t*>(&lo);
           y.y = *reinterpret_cast<const uint32_t*>(&hi);

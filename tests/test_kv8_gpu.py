@@ -360,6 +360,46 @@ def test_decode_magnitudes(spread, qscale, scale):
     _check_decode(out, q, k8, v8, table, lens, scale if scale is not None else D ** -0.5)
 
 
+@pytest.mark.parametrize("byte", [1, 5, 9, 10, 254 - 8])
+def test_decode_extreme_value_exponents(byte):
+    """Value exponents at the ends of what Fp8Pages holds. The tolerance is
+    _attention's without its absolute part; bf16's smallest step is 2^-133."""
+    ops = sub("ops")
+    lens = [7, 40, 3000]
+    k8, v8, kvl, table = _cache(lens, 2, seed=byte)
+    v8.exps.copy_(torch.where(v8.exps == 255, v8.exps, torch.full_like(v8.exps, byte)))
+    q = torch.randn(3, 8, D, device="cuda", generator=_gen(byte)).to(torch.bfloat16)
+    out = ops.decode_attention(q, k8, v8, kvl, table)
+    for b, n in enumerate(lens):
+        v = sub("ops.fp8_pages").dequantize_rows(*_live_rows(v8, table[b], n)).double()
+        want, tol = _attention(q[b:b + 1], _row(k8, table[b], n), v, D ** -0.5)
+        assert ((out[b:b + 1].double() - want).abs() <= tol - 1e-30 + 2.0 ** -133).all(), (byte, n)
+
+
+def _live_rows(pages, table_row, n):
+    """(values [n, nkv, 128], exps [n, nkv]) of a request."""
+    blocks = table_row[:-(-n // PAGE)].long()
+    values = _bytes_of(pages)[blocks].transpose(1, 2).flatten(0, 1)[:n]
+    return values.view(torch.float8_e4m3fn), pages.exps[blocks].transpose(1, 2).flatten(0, 1)[:n]
+
+
+def test_decode_long_sums_of_the_smallest_values():
+    """Rows of one value at the smallest exponent, equal weights: the mean is
+    that value, however long the row (2^-117 over 130056 keys leaves fp32's
+    normal range on the way)."""
+    ops = sub("ops")
+    n, B = 130056, 1200
+    k8, v8 = ops.fp8_cache(1, 1, "cuda")
+    _bytes_of(v8).fill_(0x3E)  # 1.75
+    v8.exps.fill_(10)
+    table = torch.zeros(1, -(-n // PAGE), dtype=torch.int32, device="cuda").expand(B, -1)
+    kvl = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    q = torch.zeros(B, 1, D, dtype=torch.bfloat16, device="cuda")
+    out = ops.decode_attention(q, k8, v8, kvl, table).double()
+    # a rounding to bf16 of a value next to 1.75, weights and sums in fp32
+    assert ((out * 2.0 ** 117 - 1.75).abs() <= 2.0 ** -8 + 1.75 * 2.0 ** -11).all()
+
+
 def test_decode_scores_that_rise_along_the_cache():
     """The running maximum moves on every page; an early key of weight zero."""
     ops, f8 = sub("ops"), sub("ops.fp8_pages")
