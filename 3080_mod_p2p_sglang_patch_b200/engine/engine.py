@@ -369,7 +369,7 @@ class LLMEngine:
         def attn(li, q, kc, vc):
             return ops.prefill_attention(q, kc, vc, cu_d, kvl_d, bt, tiles, scale, splits=splits, **kw)
 
-        halves = self._attn_halves(q_lens, kv_lens, bt, T)
+        halves = self._attn_halves(q_lens, kv_lens, bt, T, self._page_plan)
         return self.model.forward(ids_d, pos_d, slots_d, self.kv.caches, attn, last_d, return_hidden=return_hidden,
                                   attn_halves=halves)
 
@@ -381,7 +381,7 @@ class LLMEngine:
         plan = ops.page_plan(kv_lens, self.max_blocks_per_seq)
         return {"plan": ops.PagePlan(self._h2d(plan.table), plan.pages)}
 
-    def _attn_halves(self, q_lens, kv_lens, bt, T):
+    def _attn_halves(self, q_lens, kv_lens, bt, T, page_plan=None):
         """Attention of each micro-batch of an overlapped prefill batch
         (model.overlap_split), or None. A piece that straddles the split is
         cut in two: its first rows end the first micro-batch with a kv length
@@ -419,11 +419,14 @@ class LLMEngine:
             bt_h = bt.index_select(0, sel.long())
             tiles_h = self._h2d(ops.prefill_tiles(ql))
             splits_h = ops.prefill_splits(tiles_h.shape[0], nq, max(kl))
-            kw = self._page_plan(kl)
+            plan = (page_plan(kl) if page_plan else {}).get("plan")
 
-            def f(li, q, kc, vc, cu_h=cu_h, kvl_h=kvl_h, bt_h=bt_h, tiles_h=tiles_h, splits_h=splits_h, kw=kw):
-                return ops.prefill_attention(q, kc, vc, cu_h, kvl_h, bt_h, tiles_h, scale, splits=splits_h, **kw)
-            fns.append(f)
+            def make(plan, cu=cu_h, kvl=kvl_h, bt=bt_h, tiles=tiles_h, splits=splits_h):
+                def f(li, q, kc, vc, cu_h=cu, kvl_h=kvl, bt_h=bt, tiles_h=tiles, splits_h=splits):
+                    return ops.prefill_attention(q, kc, vc, cu_h, kvl_h, bt_h, tiles_h, scale, splits=splits_h,
+                                                 plan=plan)
+                return f
+            fns.append(make(plan))
         return (T1, fns[0], fns[1])
 
     def decode_inputs(self, reqs):
