@@ -354,11 +354,17 @@ __global__ void __launch_bounds__(kReadWarps * 32) read_pages_kernel(ReadArgs a,
 //    and pairs them with byte permutes.
 //  * q is scaled per head by a power of two to [2^14, 2^15) before it becomes
 //    f16: elements down to 2^-28 of the head's largest keep all their bits.
-//  * softmax in base 2 with a running maximum m. The value exponents join the
-//    weights: w = 2^(s - m) * 2^(ve - vr + 8) in f16 with vr a running maximum
-//    of ve, so weights down to 2^-22 of the largest keep 11 bits (bf16 would
-//    keep 8). m and vr only move when a page exceeds them by more than 2^4 and
-//    2^3: then w <= 2^15 stays inside f16. The row sum uses the fp32 weights.
+//  * softmax in base 2 with a running maximum m per head; the row sum takes the
+//    weights 2^(s - m) in fp32. The value exponents join the weights of the
+//    product: w = 2^(s - m) * 2^(ve + d) in f16, the integer d per head such that
+//    the largest w lies between 2^10 and 2^15. d follows mv, the running maximum
+//    of s + ve: what a key contributes to this head, not how large its value row
+//    is. So keys that contribute down to 2^-24 of the largest keep 11 bits (bf16
+//    would keep 8), and a row that the head ignores costs the others nothing,
+//    whatever its exponent. The maxima only move when a page exceeds one by more
+//    than 2^4. Weights below 2^-126 of the largest are zero, as fp32 has none, and
+//    stay out of mv. (2^(s - m + ve + d) as an exponential of its own: 64 requests
+//    of 4096 keys 101 -> 102 us, with 16 heads per kv head 131 -> 138.)
 MBX_DEVICE float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -398,7 +404,8 @@ struct Kv8DecodeArgs {
   float scale_log2;
 };
 
-constexpr int kNoExp = -1000;  // value exponent of a masked key, and vr before the first page
+constexpr float kTopWeight = 11.f;  // log2 of the largest weight w when the maxima move, rounded down
+constexpr float kSlack = 4.f;       // log2 of what may exceed a maximum before it moves: w <= 2^15, inside f16
 
 // Where a fetched page's 16-byte chunks lie in shared memory. The reader of a
 // K chunk (row r, chunk c) is lane (g, t) = (r % 8, c % 4), of a V chunk lane
@@ -423,7 +430,8 @@ struct HeadState {
   float qs[NT][2];  // softmax scale * log2(e) * the power of two taken out of q
   float o[NT][8][4];
   float m[NT][2], l[NT][2];  // l: this lane's keys only
-  int vr;
+  float mv[NT][2];
+  int d23[NT][2];  // d, at the place of an fp32 number's exponent
 
   // This lane's elements of q [G, D] (heads behind G: zeros), in two steps, so
   // that the loads can be issued ahead of their use.
@@ -441,7 +449,6 @@ struct HeadState {
   };
   MBX_DEVICE void begin(const Query& q, float scale_log2, int lane) {
     const int t = lane & 3;
-    vr = kNoExp;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float x[2][16];
@@ -469,8 +476,9 @@ struct HeadState {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         qs[n][c] = scale_log2 * pow2(__shfl_sync(0xffffffffu, e, (2 * t + c) * 4) - 14);
-        m[n][c] = -INFINITY;
+        m[n][c] = mv[n][c] = -INFINITY;
         l[n][c] = 0.f;
+        d23[n][c] = 0;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
@@ -516,8 +524,8 @@ struct HeadState {
       for (int r = 0; r < 2; ++r) {
         const uint8_t* e = src[p] + 4096 + g + 8 * r;
         const bool on = g + 8 * r < live[p];
-        vx[p][r] = on ? (int)e[16] - 127 : kNoExp;
-        grow |= vx[p][r] > vr + 3;
+        vx[p][r] = ((int)e[16] - 127) << 23;
+        const float ve = (float)(vx[p][r] >> 23);
         const float kf = __uint_as_float((uint32_t)e[0] << 23);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -525,20 +533,13 @@ struct HeadState {
           for (int c = 0; c < 2; ++c) {
             const float x = on ? (s[p][n][2 * r + c] + s2[p][n][2 * r + c]) * (kf * qs[n][c]) : -INFINITY;
             s[p][n][2 * r + c] = x;
-            grow |= x > m[n][c] + 4.f;
+            grow |= x > m[n][c] + kSlack || x + ve > mv[n][c] + kSlack;
           }
       }
     if (__any_sync(0xffffffffu, grow)) {
-      int nv = vr;
-#pragma unroll
-      for (int p = 0; p < P; ++p) nv = max(nv, max(vx[p][0], vx[p][1]));
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) nv = max(nv, __shfl_xor_sync(0xffffffffu, nv, off));
-      const float vc = ex2((float)(vr - nv));
-      vr = nv;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float corr[2];
+        float corr[2], vc[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float nm = m[n][c];
@@ -546,16 +547,34 @@ struct HeadState {
           for (int p = 0; p < P; ++p) nm = fmaxf(nm, fmaxf(s[p][n][c], s[p][n][2 + c]));
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, off));
-          corr[c] = nm == -INFINITY ? 1.f : ex2(m[n][c] - nm);
-          m[n][c] = nm;
+          float nv = mv[n][c];
+#pragma unroll
+          for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float x = s[p][n][2 * r + c];
+              nv = x - nm >= -126.f ? fmaxf(nv, x + (float)(vx[p][r] >> 23)) : nv;
+            }
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) nv = fmaxf(nv, __shfl_xor_sync(0xffffffffu, nv, off));
+          corr[c] = vc[c] = 1.f;
+          if (nm != -INFINITY) {
+            const int old = d23[n][c] >> 23, nd = __float2int_rd(nm - nv + kTopWeight);
+            const float down = m[n][c] - nm;
+            corr[c] = ex2(down);
+            vc[c] = m[n][c] == -INFINITY ? 0.f : ex2(down + (float)(nd - old));
+            m[n][c] = nm;
+            mv[n][c] = nv;
+            d23[n][c] = nd << 23;
+          }
           l[n][c] *= corr[c];
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          o[n][i][0] *= corr[0] * vc;
-          o[n][i][1] *= corr[1] * vc;
-          o[n][i][2] *= corr[0] * vc;
-          o[n][i][3] *= corr[1] * vc;
+          o[n][i][0] *= vc[0];
+          o[n][i][1] *= vc[1];
+          o[n][i][2] *= vc[0];
+          o[n][i][3] *= vc[1];
         }
       }
     }
@@ -564,7 +583,6 @@ struct HeadState {
     for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float vf = pow2(max(vx[p][r] - vr + 8, -126));
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float w[2];
@@ -572,7 +590,9 @@ struct HeadState {
           for (int c = 0; c < 2; ++c) {
             const float x = ex2(s[p][n][2 * r + c] - (m[n][c] == -INFINITY ? 0.f : m[n][c]));
             l[n][c] += x;
-            w[c] = x * vf;
+            // x 2^(ve + d) by its exponent; below the smallest normal number: zero, or close to it
+            const int y = max(__float_as_int(x) + vx[p][r] + d23[n][c], 0);
+            w[c] = x > 0.f ? __int_as_float(y) : 0.f;
           }
           pf[p][n][r] = transpose8x8(pack_f16(w[0], w[1]));
         }
@@ -952,10 +972,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
       if (!ends && use.left > 0) continue;
       // ---- the segment is done
       st.end();
-      // rows are divided by their sum here, partial ones too, and the weights' 2^8
-      // goes with the inverse: nothing on the way leaves fp32's normal range
-      // where the result does not
-      const float vs = pow2(max(st.vr, -126));
+      // Rows are divided by their sum here, partial ones too, and the weights' 2^d
+      // is taken out in two halves: nothing on the way leaves fp32's normal range
+      // where the result does not.
       if (seg_p0 == 0 && ends) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -963,7 +982,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
           for (int c = 0; c < 2; ++c) {
             const int head = n * 8 + 2 * t + c;
             if (head >= G) continue;
-            const float inv = inverse(st.l[n][c]) * 0x1p-8f;
+            const int d = st.d23[n][c] >> 23;
+            const float vs = pow2(-(d >> 1)), inv = inverse(st.l[n][c]) * pow2((d >> 1) - d);
             float f[16];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -987,7 +1007,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kv8_kernel(Kv8DecodeArg
           for (int c = 0; c < 2; ++c) {
             const int head = n * 8 + 2 * t + c;
             if (head >= G) continue;
-            const float inv = inverse(st.l[n][c]) * 0x1p-8f;
+            const int d = st.d23[n][c] >> 23;
+            const float vs = pow2(-(d >> 1)), inv = inverse(st.l[n][c]) * pow2((d >> 1) - d);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               *reinterpret_cast<float2*>(po + head * kRow + g * 16 + 2 * j) =

@@ -376,6 +376,66 @@ def test_decode_extreme_value_exponents(byte):
         assert ((out[b:b + 1].double() - want).abs() <= tol - 1e-30 + 2.0 ** -133).all(), (byte, n)
 
 
+def _spread_tol(p, v, n):
+    """What the weights' f16 grid may cost a row of probabilities p [nq, n] over
+    v [n, nq, 128]: the key that contributes most has a weight of 2^10 at least,
+    the others are off by half of f16's smallest step, 2^-25, times their
+    e4m3 number, of which a row's largest is in (224, 448]."""
+    top = v.abs().amax(-1).T  # [nq, n]
+    return n * 2.0 ** -34 * (p * top).amax(-1, keepdim=True)
+
+
+@pytest.mark.parametrize("nq,nkv", [(8, 2), (16, 1), (3, 1)])
+@pytest.mark.parametrize("gap", [20, 24, 28, 31, 33, 40, 60, 100])
+@pytest.mark.parametrize("n", [40, 3000])
+def test_decode_loud_value_rows_that_no_head_attends_to(n, gap, nq, nkv):
+    """Rows of value 2^gap times the others' whose weight is 2^-(gap + 40) of
+    theirs at most: they count for nothing, the quiet ones for all. Loud rows
+    come first, last and in between."""
+    _check_loud(n, nq, nkv, gap, -30, gap + 60.0)
+
+
+@pytest.mark.parametrize("nq,nkv", [(8, 2), (16, 1)])
+@pytest.mark.parametrize("n", [40, 3000])
+def test_decode_weights_below_fp32_count_as_zero(n, nq, nkv):
+    """Rows 2^200 times the others, of a weight (2^-150) that fp32 does not have."""
+    _check_loud(n, nq, nkv, 200, -100, 160.0, counted=False)
+
+
+def _check_loud(n, nq, nkv, gap, low, away, counted=True):
+    """Loud rows of value 2^(low + gap) among quiet ones of 2^low, their scores
+    0.7 away ln-units lower."""
+    ops, f8 = sub("ops"), sub("ops.fp8_pages")
+    k8, v8, kvl, table = _cache([n], nkv, seed=gap)
+    g = _gen(gap + n)
+    loud = torch.zeros(table.shape[1] * PAGE, dtype=torch.bool, device="cuda")
+    loud[[0, 1, n // 2, n - 1]] = True
+    x = torch.randn(loud.numel(), nkv, D, device="cuda", generator=g)
+    v = torch.where(loud[:, None, None], x * 2.0 ** (low + gap), x * 2.0 ** low)
+    k = 0.1 * torch.randn(loud.numel(), nkv, D, device="cuda", generator=g)
+    k[..., 0] = torch.where(loud, -away, 0.0)[:, None]
+    for pages, rows in ((k8, k), (v8, v)):
+        values, exps = f8.quantize_rows(rows.view(-1, PAGE, nkv, D).transpose(1, 2))
+        _bytes_of(pages)[table[0].long()] = values.view(torch.uint8)
+        pages.exps[table[0].long()] = exps
+    q = torch.randn(1, nq, D, device="cuda", generator=g).to(torch.bfloat16)
+    q[..., 0] = 0.7
+    out = ops.decode_attention(q, k8, v8, kvl, table, scale=1.0).double()
+    G = nq // nkv
+    kk, vv = (_row(c, table[0], n).repeat_interleave(G, 1) for c in (k8, v8))
+    p = torch.softmax(torch.einsum("hd,khd->hk", q[0].double(), kk), -1)
+    if not counted:
+        p = torch.where(loud[:n], 0.0, p)
+    want = torch.einsum("hk,khd->hd", p, vv)
+    # _attention's bound with _spread_tol in the place of its absolute part
+    A = torch.einsum("hk,khd->hd", p, vv.abs())
+    mag = torch.einsum("hd,khd->hk", q[0].double().abs(), kk.abs()).amax(-1, keepdim=True)
+    tol = want.abs() * 2.0 ** -8 + A * (2.0 ** -11 + 2 * (mag * 1.4427 * 2.0 ** -17 + 2.0 ** -21)) * 1.01
+    tol = tol + _spread_tol(p, vv, n)
+    err = (out[0] - want).abs()
+    assert (err <= tol).all(), f"off by {(err / tol).max().item():.2f} of the tolerance"
+
+
 def _live_rows(pages, table_row, n):
     """(values [n, nkv, 128], exps [n, nkv]) of a request."""
     blocks = table_row[:-(-n // PAGE)].long()
