@@ -7,10 +7,10 @@
 //   values_i = round_to_nearest_even_e4m3(x_i / 2^e),  exps = e + 127
 // and stands for values_i * 2^e. e4m3 is a floating format, so a scale finer
 // than a power of two would buy at most one exponent of range and no
-// accuracy, while a power of two makes every scaling exact: a stored row is
-// exact in bf16 and in fp32 products, and which e4m3 number a value rounds to
-// does not depend on a division. Elements that are not finite are stored as
-// NaN and do not take part in the maximum.
+// accuracy, while a power of two makes every scaling exact: a stored number
+// below 2^128 is exact in bf16 and in fp32 products, and which e4m3 number a
+// value rounds to does not depend on a division. Elements that are not finite
+// are stored as NaN and do not take part in the maximum.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -27,23 +27,30 @@ constexpr int D = 128;
 constexpr int PAGE = 16;
 constexpr int kMinExp = -117;  // 2^-9 * 2^-117 = 2^-126: every stored number is a normal fp32 / bf16 number or zero
 
-// A row's exponent from the largest magnitude of its finite elements (fp32):
-// 448 = 1.75 * 2^8.
+// Rows on their way into the cache are held 2^8 smaller: a normalised and
+// rotated k of finite inputs may lie beyond fp32 (below 16 * 2^128, though).
+constexpr int kDown = 8;
+constexpr float kSmaller = 1.f / (1 << kDown);
+
+// A row's exponent from the largest magnitude of its finite elements, held
+// 2^kDown smaller: 448 = 1.75 * 2^8.
 MBX_DEVICE int row_exp(float top) {
   const uint32_t b = __float_as_uint(top);
-  const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  const int e = (int)(b >> 23) - 127 - 8 + kDown + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
   return max(e, kMinExp);
 }
 
 // 2^e for e in [-126, 127].
 MBX_DEVICE float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
+MBX_DEVICE bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
 // Two e4m3 numbers from lo and hi (lo in the low byte); what is not finite becomes NaN.
 MBX_DEVICE uint32_t e4m3x2(float lo, float hi) {
   uint16_t r;
   const float nan = __uint_as_float(0x7fffffffu);
-  lo = fabsf(lo) <= 3.4e38f ? lo : nan;
-  hi = fabsf(hi) <= 3.4e38f ? hi : nan;
+  lo = finite(lo) ? lo : nan;
+  hi = finite(hi) ? hi : nan;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
@@ -57,16 +64,15 @@ MBX_DEVICE uint32_t f16x2_of(uint32_t w, int half) {
 }
 
 // The fp32 number whose further rounding to fewer bits (22 or less) equals
-// rounding x itself: x cut to 24 bits, the last one set if anything was cut.
+// rounding x itself: x cut to 24 bits (fewer below fp32's normal range, whose
+// last, 2^-149, is still far below what is kept of a row), the last one set if
+// anything was cut.
 MBX_DEVICE float round_to_odd(double x) {
   const float f = __double2float_rz(x);
   return (double)f != x ? __uint_as_float(__float_as_uint(f) | 1u) : f;
 }
 
-MBX_DEVICE float finite_abs(float x) {
-  const float a = fabsf(x);
-  return a <= 3.4e38f ? a : 0.f;
-}
+MBX_DEVICE float finite_abs(float x) { return finite(x) ? fabsf(x) : 0.f; }
 
 // ---------------------------------------------------------------- append
 struct AppendArgs {
@@ -113,7 +119,7 @@ MBX_DEVICE F eighth_sum(F v) {  // over a row's eight lanes
   return v;
 }
 
-// A row rounded into the cache, at dst and *exp.
+// A row, held 2^kDown smaller, rounded into the cache at dst and *exp.
 MBX_DEVICE void store_e4m3(const float (&x)[8], const float (&y)[8], uint8_t* dst, uint8_t* exp, int i, bool keep) {
   float top = 0.f;
 #pragma unroll
@@ -121,7 +127,7 @@ MBX_DEVICE void store_e4m3(const float (&x)[8], const float (&y)[8], uint8_t* ds
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const int e = row_exp(top);
-  const float inv = pow2(-e);
+  const float inv = pow2(kDown - e);
   uint2 lo, hi;
   lo.x = e4m3x2(x[0] * inv, x[1] * inv) | e4m3x2(x[2] * inv, x[3] * inv) << 16;
   lo.y = e4m3x2(x[4] * inv, x[5] * inv) | e4m3x2(x[6] * inv, x[7] * inv) << 16;
@@ -259,10 +265,14 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(AppendArgs a,
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const double p = kNorm ? rs * w[k] * x[k] : (double)x[k], q = kNorm ? rs * v[k] * y[k] : (double)y[k];
-        const float px = round_to_odd(p * g.c[k] - q * g.s[k]), py = round_to_odd(q * g.c[k] + p * g.s[k]);
-        x[k] = is_k ? px : x[k];
-        y[k] = is_k ? py : y[k];
+        const float px = round_to_odd((p * g.c[k] - q * g.s[k]) * kSmaller);
+        const float py = round_to_odd((q * g.c[k] + p * g.s[k]) * kSmaller);
+        x[k] = is_k ? px : x[k] * kSmaller;
+        y[k] = is_k ? py : y[k] * kSmaller;
       }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] *= kSmaller, y[k] *= kSmaller;  // exact: bf16 keeps 16 exponents less than fp32
     }
     const int64_t blk = slot / PAGE;
     const int off = (int)(slot % PAGE);

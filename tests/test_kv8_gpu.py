@@ -172,6 +172,34 @@ def test_append_extreme_magnitudes(scale):
         assert torch.equal(_bytes_of(pages)[blk, :, off].view(torch.float8_e4m3fn).float(), v.float())
 
 
+@pytest.mark.parametrize("case", ["edge", "beyond", "norm", "small"])
+def test_append_rows_at_the_ends_of_the_range(case):
+    """k rows that are finite in the definition but near or beyond fp32's
+    largest number after the rotation or the norm, and rows whose elements reach
+    below bf16's normal range."""
+    ops = sub("ops")
+    T, nq, nkv = 19, 4, 2
+    qkv, pos, cs, slots, blocks, kw = _append_case(T, nq, nkv, case == "norm", 5, 1e-39 if case == "small" else 1.0)
+    big = torch.finfo(torch.bfloat16).max
+    if case == "edge":  # the rotation keeps a pair's length: these stay within (3.39e38, 3.41e38)
+        qkv[:] = 0.0
+        qkv.view(T, -1, D)[:, nq:, ::3] = big
+    elif case == "beyond":
+        qkv = torch.where(qkv < 0, -big, big).to(torch.bfloat16)
+    elif case == "norm":
+        kw["k_norm"] = torch.where(kw["k_norm"] > 1, big, -big / 4).to(torch.bfloat16)
+        qkv.view(T, -1, D)[:, nq:, 5:] *= 0.01  # few dims carry the row: normalised elements up to sqrt(128 / 5)
+    k8, v8 = ops.fp8_cache(blocks, nkv, "cuda")
+    ops.rope_and_cache(qkv, pos, cs, nq, nkv, slots, k8, v8, **kw)
+    _, (kv, ke), (vv, ve) = _append_want(qkv, pos, cs, nq, nkv, kw)
+    blk, off = slots // PAGE, slots % PAGE
+    for pages, v, e in ((k8, kv, ke), (v8, vv, ve)):
+        assert not torch.isnan(v.float()).any()
+        assert torch.equal(pages.exps[blk, :, off], e)
+        assert torch.equal(_bytes_of(pages)[blk, :, off].view(torch.float8_e4m3fn).float(), v.float())
+    assert (ke > 246).any() == (case != "small")
+
+
 def test_append_borders_and_elements_that_are_not_finite():
     """Rows on and next to rounding borders (position 0: no rotation), and
     rows with NaN and infinities."""
