@@ -409,8 +409,8 @@ def page_plan(kv_lens, columns: int) -> PagePlan:
 
 
 def read_pages(k_cache, v_cache, block_table, kv_len, out_table=None, k_out=None, v_out=None):
-    """Pages of an 8-bit cache back to bf16 (exact): (k, v) [pages, kv heads,
-    16, 128]. Page i of request r (block ``block_table[r, i]``) goes to page
+    """Pages of an 8-bit cache back to bf16 (exact below 2^128): (k, v) [pages,
+    kv heads, 16, 128]. Page i of request r (block ``block_table[r, i]``) goes to page
     ``out_table[r, i]`` of the outputs, by default ``r * columns + i``; the
     entries used must differ. Pages behind ``kv_len[r]`` tokens, and entries
     outside the outputs, are left as they were; rows behind the length in a

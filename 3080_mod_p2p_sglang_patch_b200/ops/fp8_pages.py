@@ -5,7 +5,9 @@ A cached row (one token, one kv head, 128 dims) is held as e4m3 numbers with
 one power-of-two scale: ``row = values * 2^(exps - 127)``. The exponent is the
 smallest at which the row's largest magnitude is at most 448 (never below
 2^-117), the values are the nearest e4m3 numbers (ties to even). A power of two
-only moves exponents, so a stored row is exact in bf16. Elements that are not
+only moves exponents, so what is stored is exact in bf16 while it is below 2^128
+(a row that reaches into bf16's last eighth of a binade may round up to it, a
+rotated k may lie above it: infinity in bf16 and fp32). Elements that are not
 finite are stored as NaN and do not take part in the maximum. A row takes 129
 bytes instead of bf16's 256.
 """
@@ -21,8 +23,11 @@ MIN_EXP = -117
 class Fp8Pages:
     """The keys or the values of one layer: ``values`` float8_e4m3fn [blocks,
     kv heads, 16, 128] (contiguous), ``exps`` uint8 [blocks, kv heads, 16]
-    (unit stride in a page, 16-byte multiples between pages), each byte in
-    1..254. Stands wherever ``ops`` takes a bf16 ``k_cache`` / ``v_cache``."""
+    (unit stride in a page, 16-byte multiples between pages). Written rows
+    have bytes from 10 on; bytes 1..254 are read, exactly from 3 to 246 (1 and 2:
+    some numbers lie between bf16's smallest steps; above 246: where the number
+    is below 2^128). Stands wherever ``ops`` takes a bf16 ``k_cache`` /
+    ``v_cache``."""
     values: torch.Tensor
     exps: torch.Tensor
 
@@ -35,7 +40,8 @@ class Fp8Pages:
         return self.values.device
 
     def dequantize(self) -> torch.Tensor:
-        """bf16 [blocks, kv heads, 16, 128], exact (plain PyTorch)."""
+        """bf16 [blocks, kv heads, 16, 128] (plain PyTorch), as exact as the
+        rows are in bf16."""
         return dequantize_rows(self.values, self.exps).to(torch.bfloat16)
 
 
@@ -64,5 +70,6 @@ def quantize_rows(x: torch.Tensor):
 
 
 def dequantize_rows(values: torch.Tensor, exps: torch.Tensor) -> torch.Tensor:
-    """fp32 rows of e4m3 ``values`` [..., 128] and ``exps`` [...] (exact)."""
+    """fp32 rows of e4m3 ``values`` [..., 128] and ``exps`` [...], exact below
+    2^128."""
     return torch.ldexp(values.float(), exps.to(torch.int32).unsqueeze(-1) - 127)

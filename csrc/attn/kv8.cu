@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(AppendArgs a,
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] *= kSmaller, y[k] *= kSmaller;  // exact: bf16 keeps 16 exponents less than fp32
+      for (int k = 0; k < 8; ++k) x[k] *= kSmaller, y[k] *= kSmaller;  // exact: bf16's smallest step is 2^-133, fp32's 2^-149
     }
     const int64_t blk = slot / PAGE;
     const int off = (int)(slot % PAGE);

@@ -71,6 +71,33 @@ def test_elements_that_are_not_finite_become_nan_and_leave_the_rest_alone():
     assert torch.isnan(b[bad]).all() and torch.equal(b[~bad], a[~bad])
 
 
+def test_stored_numbers_are_exact_in_bf16_below_2_to_the_128():
+    """Every e4m3 number at every exponent byte of the stated range."""
+    f8 = sub("ops.fp8_pages")
+    v = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    v = v[~torch.isnan(v.float())]
+    for byte in range(1, 255):
+        real = v.double() * 2.0 ** (byte - 127)
+        wide = f8.dequantize_rows(v[None], torch.tensor([byte], dtype=torch.uint8))[0]
+        inside = real.abs() < 2.0 ** 128
+        assert inside.all() or byte > 246
+        assert torch.equal(wide.double()[inside], real[inside])
+        assert torch.isinf(wide[~inside]).all()
+        half = wide.to(torch.bfloat16).double()
+        if byte >= 3:
+            assert torch.equal(half[inside], real[inside])
+        else:
+            assert ((half - real).abs() <= 2.0 ** -134).all()
+
+
+def test_a_row_at_bf16s_maximum_rounds_up_to_infinity():
+    f8 = sub("ops.fp8_pages")
+    x = torch.full((1, D), torch.finfo(torch.bfloat16).max)
+    values, exps = f8.quantize_rows(x)
+    assert int(exps) == 247 and (values.float() == 256).all()
+    assert torch.isinf(f8.dequantize_rows(values, exps)).all()
+
+
 def test_cache_constructor_layout():
     ops = sub("ops")
     k, v = ops.fp8_cache(3, 2, "cpu")

@@ -335,6 +335,19 @@ def test_read_pages_by_plan_strided_tables_and_bad_pages():
     assert ops.read_pages(k8, v8, table[:, :0], kvl)[0].shape[0] == 0
 
 
+def test_read_pages_of_every_exponent_and_number():
+    ops = sub("ops")
+    cache = ops.fp8_cache(32, 1, "cuda")
+    for i, c in enumerate(cache):
+        _bytes_of(c).view(-1, D)[:] = (torch.arange(D, device="cuda") + 128 * i).to(torch.uint8)
+        c.exps[:, 0] = torch.arange(1, 513, device="cuda").remainder(254).add(1).to(torch.uint8).view(32, PAGE)
+    table = torch.arange(32, dtype=torch.int32, device="cuda")[None]
+    got = ops.read_pages(*cache, table, torch.tensor([512], dtype=torch.int32, device="cuda"))
+    for c, x in zip(cache, got):
+        want = torch.nan_to_num(c.dequantize().float(), nan=7.0)
+        assert torch.equal(torch.nan_to_num(x.float(), nan=7.0), want) and want.isfinite().any()
+
+
 # ---------------------------------------------------------------- decode
 LENS = [1, 0, 2, 15, 16, 17, 31, 33, 100, 500, 777, 2049]
 
