@@ -58,7 +58,9 @@ def rope_and_cache(qkv, positions, cos_sin, nq, nkv, slots=None, k_cache=None, v
     store k/v at the paged ``slots`` (block * page + offset); returns q.
     ``q_norm`` / ``k_norm``: per-head RMSNorm of q and k first (Qwen3), kept
     in fp32 into the rotation. ``Fp8Pages`` caches take rows rounded once, k's
-    from fp64."""
+    from fp64; as in the kernel, slots outside the cache are not written, of
+    equal slots the last token's row stays and positions are clamped to the
+    table."""
     T = qkv.shape[0]
     D = cos_sin.shape[1]
     q = qkv[:, :nq * D].view(T, nq, D)
@@ -66,12 +68,17 @@ def rope_and_cache(qkv, positions, cos_sin, nq, nkv, slots=None, k_cache=None, v
     fp8 = isinstance(k_cache, Fp8Pages)
     if fp8:
         k = k.double()
+        positions = positions.clamp(0, cos_sin.shape[0] - 1)
     if q_norm is not None:
         q, k = ref.rmsnorm(q, q_norm, eps), ref.rmsnorm(k, k_norm, eps)
     v = qkv[:, (nq + nkv) * D:(nq + 2 * nkv) * D].view(T, nkv, D)
     qr = ref.rope(q, positions, cos_sin).to(qkv.dtype)
     if slots is not None:
         s = slots.long()
+        if fp8:
+            last = {x: t for t, x in enumerate(s.tolist()) if 0 <= x < k_cache.shape[0] * page}
+            keep = torch.tensor(list(last.values()), dtype=torch.long, device=s.device)
+            s, k, v, positions = s[keep], k[keep], v[keep], positions[keep]
         blk, off = s // page, s % page
         if fp8:
             for c, rows in ((k_cache, ref.rope(k, positions, cos_sin)), (v_cache, v.float())):

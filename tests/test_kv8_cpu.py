@@ -143,6 +143,33 @@ def test_oracle_writes_and_reads_the_format():
         assert torch.equal(out, ref.attention(q, kk, vv, causal_offset=0).to(q.dtype))
 
 
+def test_oracle_writes_as_the_kernel_does_outside_the_cache_and_the_table():
+    """Slots that are negative or past the cache are not written, the last of
+    equal slots stays, positions outside the table take its ends."""
+    ops, oracle, f8 = sub("ops"), sub("ops.oracle"), sub("ops.fp8_pages")
+    T, nq, nkv, blocks = 40, 2, 2, 3
+    g = torch.Generator().manual_seed(0)
+    cs = ops.rope_cos_sin(16, D, 10000.0, "cpu")
+    qkv = torch.randn(T, (nq + 2 * nkv) * D, generator=g).to(torch.bfloat16)
+    pos = torch.randint(-5, 30, (T,), generator=g, dtype=torch.int32)
+    slots = torch.randint(0, 12, (T,), generator=g)
+    slots[3], slots[4], slots[T - 1] = -1, blocks * PAGE, -17
+    k8, v8 = ops.fp8_cache(blocks, nkv, "cpu")
+    q = oracle.rope_and_cache(qkv, pos, cs, nq, nkv, slots, k8, v8)
+    inside = oracle.rope_and_cache(qkv, pos.clamp(0, 15), cs, nq, nkv)
+    assert torch.equal(q, inside)
+    last = {s: t for t, s in enumerate(slots.tolist()) if 0 <= s < blocks * PAGE}
+    v = qkv[:, (nq + nkv) * D:].view(T, nkv, D).float()
+    values, exps = f8.quantize_rows(v)
+    rows = v8.values.view(torch.uint8).transpose(1, 2).reshape(-1, nkv, D)
+    for s in range(blocks * PAGE):
+        if s in last:
+            assert torch.equal(rows[s], values[last[s]].view(torch.uint8)), s
+            assert torch.equal(v8.exps[s // PAGE, :, s % PAGE], exps[last[s]])
+        else:
+            assert (rows[s] == 0).all() and (v8.exps[s // PAGE, :, s % PAGE] == 127).all()
+
+
 def _args(ops, T=3, nq=4, nkv=2, blocks=3):
     k, v = ops.fp8_cache(blocks, nkv, "cpu")
     i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
