@@ -283,9 +283,10 @@ def rope_and_cache(qkv, positions, cos_sin, nq, nkv, slots=None, k_cache=None, v
     if _is_fp8(k_cache, v_cache) and slots is not None:
         if page != 16:
             raise ValueError("8-bit caches have pages of 16 tokens")
+        q_out = cuda_ext().rope_and_cache_kv8(qkv, positions, cos_sin, slots, q_out, k_cache.values, k_cache.exps,
+                                              v_cache.values, v_cache.exps, nq, nkv, q_norm, k_norm, eps)
         launches.add(1)
-        return cuda_ext().rope_and_cache_kv8(qkv, positions, cos_sin, slots, q_out, k_cache.values, k_cache.exps,
-                                             v_cache.values, v_cache.exps, nq, nkv, q_norm, k_norm, eps)
+        return q_out
     T = qkv.shape[0]
     if q_out is None:
         q_out = torch.empty((T, nq, 128), dtype=qkv.dtype, device=qkv.device)
@@ -480,10 +481,11 @@ def _prefill_fp8(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, scale, o
         table = _page_ids(pages, q.device).view(R, cols)
     else:
         table, pages = plan.table, plan.pages
-    launches.add(3 if splits > 1 else 2)
     err = workspace(q.device).err if q.is_cuda else None
-    return cuda_ext().prefill_attention_kv8(q, k_cache.values, k_cache.exps, v_cache.values, v_cache.exps, out, cu_q,
-                                            kv_len, block_table, table, pages, tiles, scale, err, splits)
+    out = cuda_ext().prefill_attention_kv8(q, k_cache.values, k_cache.exps, v_cache.values, v_cache.exps, out, cu_q,
+                                           kv_len, block_table, table, pages, tiles, scale, err, splits)
+    launches.add(3 if splits > 1 else 2)
+    return out
 
 
 def prefill_attention_mma(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles64, scale=None, out=None):
@@ -516,9 +518,10 @@ def decode_attention(q, k_cache, v_cache, kv_len, block_table, scale=None, split
     keys of blocks outside the cache do not count."""
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     if _is_fp8(k_cache, v_cache):
+        out = cuda_ext().decode_attention_kv8(q, k_cache.values, k_cache.exps, v_cache.values, v_cache.exps, out,
+                                              kv_len, block_table, scale)
         launches.add(1)
-        return cuda_ext().decode_attention_kv8(q, k_cache.values, k_cache.exps, v_cache.values, v_cache.exps, out,
-                                               kv_len, block_table, scale)
+        return out
     if out is None:
         out = torch.empty_like(q)
     B, nq, _ = q.shape

@@ -260,6 +260,22 @@ def test_refusals_of_the_cache(which):
 
 
 @needs_ext
+def test_refused_calls_count_no_launches():
+    ops, launches = sub("ops"), sub("utils.launches")
+    k, v = ops.fp8_cache(3, 2, "cpu")
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    before = launches.get()
+    for which in ("rope", "read", "decode"):
+        with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+            _call(ops, which, _args(ops)[which])
+    for splits in (1, 2):
+        with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+            ops.prefill_attention(torch.zeros(5, 4, D, dtype=torch.bfloat16), k, v, i32(3), i32(2), i32(2, 3), i32(2, 2),
+                                  splits=splits)
+    assert launches.get() == before
+
+
+@needs_ext
 def test_refusals_of_head_counts_and_outputs():
     ops = sub("ops")
     a = _args(ops)["rope"]
