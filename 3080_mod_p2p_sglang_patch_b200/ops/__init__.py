@@ -440,12 +440,15 @@ _PAGE_IDS = {}  # device -> [0, 1, 2, ...] in growing lengths: the block table o
 def _page_ids(n, device):
     if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
         return torch.arange(n, dtype=torch.int32, device=device)
-    ids = _PAGE_IDS.setdefault(device, [])
-    if not ids or ids[-1].numel() < n:
+    made = _PAGE_IDS.setdefault(device, [])
+    ids = made[-1] if made else None
+    if ids is None or ids.numel() < n:
         # copied from the host before this returns, so any stream may read it;
-        # shorter ones stay alive for the launches that have them
-        ids.append(torch.arange(max(n, 4096, 2 * ids[-1].numel() if ids else 0), dtype=torch.int32).to(device))
-    return ids[-1][:n]
+        # shorter ones stay alive for the launches that have them (and another
+        # thread may append one meanwhile: this call keeps its own)
+        ids = torch.arange(max(n, 4096, 2 * ids.numel() if ids is not None else 0), dtype=torch.int32).to(device)
+        made.append(ids)
+    return ids[:n]
 
 
 def prefill_attention(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, scale=None, out=None, splits=1,

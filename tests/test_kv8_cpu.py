@@ -170,6 +170,24 @@ def test_oracle_writes_as_the_kernel_does_outside_the_cache_and_the_table():
             assert (rows[s] == 0).all() and (v8.exps[s // PAGE, :, s % PAGE] == 127).all()
 
 
+def test_page_ids_of_two_threads(monkeypatch):
+    """A thread that needs fewer pages appends its list while another makes a
+    longer one: each gets as many as it asked for."""
+    ops = sub("ops")
+    dev = torch.device("cpu")
+    monkeypatch.setattr(ops, "_PAGE_IDS", {})
+
+    class Made(list):
+        def append(self, t):  # the other thread appends right behind
+            super().append(t)
+            super().append(torch.arange(5, dtype=torch.int32))
+
+    ops._PAGE_IDS[dev] = Made()
+    assert ops._page_ids(9000, dev).tolist() == list(range(9000))
+    assert ops._page_ids(20000, dev).tolist() == list(range(20000))
+    assert ops._page_ids(3, dev).tolist() == [0, 1, 2]
+
+
 def _args(ops, T=3, nq=4, nkv=2, blocks=3):
     k, v = ops.fp8_cache(blocks, nkv, "cpu")
     i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
