@@ -571,11 +571,13 @@ Kv8Cache kv8_cache(const torch::Tensor& kv, const torch::Tensor& ke, const torch
   return c;
 }
 
-// int32 [requests, pages] whose rows are contiguous (the row stride is free).
+// int32 [requests, pages] whose rows are contiguous (the row stride is free),
+// short enough that a request's keys fit an int32.
 void check_table(const torch::Tensor& t, const char* name, int64_t rows) {
   TORCH_CHECK(t.scalar_type() == torch::kInt32 && t.dim() == 2 && t.size(0) == rows &&
                   (t.size(1) <= 1 || t.stride(1) == 1),
               name, " must be int32 [requests, pages] with contiguous rows");
+  TORCH_CHECK(t.size(1) < (int64_t)1 << 27, name, " must have fewer than 2^27 pages a row");
 }
 void check_lens(const torch::Tensor& t) {
   TORCH_CHECK(t.scalar_type() == torch::kInt32 && t.dim() == 1 && t.is_contiguous(),

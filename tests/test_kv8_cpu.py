@@ -334,6 +334,24 @@ def test_refusals_of_prefill_attention():
         ops.prefill_attention(**{**good, "v_cache": bf(3, 2, PAGE, D)})
 
 
+@needs_ext
+def test_tables_whose_keys_pass_an_int32_are_refused():
+    """2^27 columns are 2^31 keys; the largest table below is accepted (up to
+    the device check). Untouched pages of the tables take no memory."""
+    ops = sub("ops")
+    k, v = ops.fp8_cache(3, 1, "cpu")
+    i32 = lambda *s: torch.empty(*s, dtype=torch.int32)  # noqa: E731
+    bf = lambda *s: torch.empty(*s, dtype=torch.bfloat16)  # noqa: E731
+    for cols, message in ((1 << 27, "2\\^27 pages"), ((1 << 27) - 1, "must be a CUDA tensor")):
+        bt, q, lens = i32(1, cols), bf(1, 4, D), i32(1)
+        with pytest.raises(RuntimeError, match=message):
+            ops.decode_attention(q, k, v, lens, bt)
+        with pytest.raises(RuntimeError, match=message):
+            ops.read_pages(k, v, bt, lens, out_table=bt, k_out=bf(2, 1, PAGE, D), v_out=bf(2, 1, PAGE, D))
+        with pytest.raises(RuntimeError, match=message):
+            ops.prefill_attention(q, k, v, i32(2), lens, bt, i32(1, 2), plan=ops.PagePlan(bt, 2))
+
+
 # ---------------------------------------------------------------- the engine on an 8-bit cache
 def dense_fp8(cfg, w, tokens):
     """``test_engine_cpu._dense`` (fp32, no cache, no pages) with the rotated k
