@@ -107,7 +107,8 @@ def reserve(device, gemm_elems=0, decode_o=0, decode_lse=0, awq_ws=0, awq_w=0):
 
 def gemm_error(device=None) -> int:
     """Non-zero if a tcgen05 kernel's bounded wait gave up (GEMM or prefill
-    attention; sticky until cleared)."""
+    attention), or prefill attention over an 8-bit cache needed a page that its
+    plan does not place (24); sticky until cleared."""
     return int(workspace(device or torch.cuda.current_device()).err.item())
 
 
@@ -400,8 +401,9 @@ class PagePlan:
 def page_plan(kv_lens, columns: int) -> PagePlan:
     """The plan (on the CPU) that packs the pages of requests of ``kv_lens``
     tokens one after another; ``columns`` is the block table's width. Without a
-    plan every request gets ``columns`` pages of scratch (prefill attention
-    counts on a request's pages being consecutive)."""
+    plan every request gets ``columns`` pages of scratch. (Any plan whose used
+    entries differ will do; prefill attention loads four pages of a request at
+    once where they are consecutive, as here.)"""
     counts = torch.tensor([max(0, min(columns, -(-int(n) // 16))) for n in kv_lens], dtype=torch.int32)
     i = torch.arange(columns, dtype=torch.int32)[None, :]
     start = (counts.cumsum(0, dtype=torch.int32) - counts)[:, None]
@@ -459,9 +461,11 @@ def prefill_attention(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, sca
     ``prefill_splits``); the partials are merged by a combine kernel.
 
     ``Fp8Pages`` caches are read back to bf16 scratch pages first
-    (``read_pages``; placed by ``plan``, a ``page_plan`` of the same lengths,
-    its table on the device). There ``scale`` has to be positive and rows that
-    see no key are zeros."""
+    (``read_pages``; placed by ``plan``, a ``page_plan`` of the same lengths
+    or longer ones, its table on the device). There ``scale`` has to be positive
+    and rows that see no key are zeros. Keys and values of pages that the plan
+    does not place, or whose block is not in the cache, count as zeros; the
+    former also set ``gemm_error``."""
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     if _is_fp8(k_cache, v_cache):
         return _prefill_fp8(q, k_cache, v_cache, cu_q, kv_len, block_table, tiles, scale, out, splits, plan)

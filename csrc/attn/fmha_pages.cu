@@ -1,8 +1,9 @@
 // Prefill attention over a batch's own bf16 pages (the 8-bit cache, read back),
 // on the Blackwell tensor cores (tcgen05 + TMEM + TMA).
 //
-// The scratch pages of a request lie one after another, so a tile of keys is one
-// TMA box per 64 dims. One CTA = two 128-row query tiles of one head, each with
+// Where the scratch pages of a request lie one after another, as page_plan puts
+// them, a tile of keys is one TMA box per 64 dims, elsewhere a box per page. One
+// CTA = two 128-row query tiles of one head, each with
 // its own softmax warpgroup. Per query tile and tile of 64 keys:
 //   S  = Q K^T    tcgen05.mma 128 x 64, fp32 in TMEM
 //   P  = exp2(S * scale - m) by 4 warps, one thread per row, stored as bf16 in
@@ -59,11 +60,12 @@ struct PagesArgs {
   __nv_bfloat16* o;      // [T, nq, D]
   const int* cu_q;       // [R + 1]
   const int* kv_len;     // [R]
-  const int* table;      // [R, cols]: scratch pages, consecutive in a row
+  const int* table;      // [R, cols]: scratch pages
   const int2* tiles;     // (request, q offset): 256-row query-tile pairs
   float* part_o;         // splits > 1: [T, nq, splits, D]
   float* part_lse;       //             [T, nq, splits]
   int splits, cols, nq, nkv, pages;  // pages: of K, behind which V's lie
+  int placed;            // table entries outside [0, placed) name no page
   float scale_log2;
   uint32_t* err;
   uint64_t timeout_ns;
@@ -142,7 +144,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int q_begin = a.cu_q[r], q_len = a.cu_q[r + 1] - q_begin;
   const int L = min(max(a.kv_len[r], 0), a.cols * PAGE);
   const int pos0 = L - q_len;  // position of the request's first query
-  const int page0 = a.cols > 0 ? a.table[(int64_t)r * a.cols] : 0;
+  // the scratch pages of four pages in a row (the producer's), from page p on
+  auto ids_of = [&](int p) {
+    const int* row = a.table + (int64_t)r * a.cols;
+    const int last = a.cols - 1;
+    return last < 0 ? make_int4(-1, -1, -1, -1)
+                    : make_int4(row[min(p, last)], row[min(p + 1, last)], row[min(p + 2, last)], row[min(p + 3, last)]);
+  };
+  int4 next_ids = make_int4(-1, -1, -1, -1);
+  if (warp == 0) next_ids = ids_of(0);  // where the CTA's keys begin at 0: ahead of what follows
   int rows_t[QT], kvend_t[QT], n_t[QT];  // per query tile: rows, keys it sees, key tiles
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -201,30 +211,42 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::tma_load_3d(smem + Smem::kQ + t * kQBytes + c * kQChunk, &tmQ, q_full, c * 64, head,
                             q_begin + qoff + t * BQ);
       }
-      // A tile whose pages all hold keys is one box per 64 dims; in the last one
-      // the pages behind the last are that page again (masked keys have to be
-      // finite, and what follows in the scratch is another request's).
-      auto load = [&](uint8_t* dst, int first, uint64_t* bar, int j) {
-        const int p = (tb + j) * kTilePages;
+      // A tile whose pages all hold keys and lie in a row is one box per 64 dims;
+      // in the last one the pages behind the last are that page again (masked keys
+      // have to be finite, and what follows in the scratch is another request's).
+      // A page that the table does not place reads as zeros (a coordinate behind
+      // the scratch), and the error word says so.
+      auto load = [&](uint8_t* dst, const int4& id, int first, uint64_t* bar, int p) {
+        const bool row = p + kTilePages - 1 <= last_page && id.x >= 0 && id.w < a.placed && id.y == id.x + 1 &&
+                         id.z == id.x + 2 && id.w == id.x + 3;
         for (int c = 0; c < 2; ++c) {
-          if (p + kTilePages - 1 <= last_page) {
-            tc::tma_load_4d(dst + c * kKVChunk, &tmKV, bar, c * 64, 0, kvh, first + p);
+          if (row) {
+            tc::tma_load_4d(dst + c * kKVChunk, &tmKV, bar, c * 64, 0, kvh, first + id.x);
           } else {
-            for (int i = 0; i < kTilePages; ++i)
+            for (int i = 0; i < kTilePages; ++i) {
+              const int k = min(i, last_page - p);
+              const int page = k == 0 ? id.x : k == 1 ? id.y : k == 2 ? id.z : id.w;
+              const bool there = page >= 0 && page < a.placed;
+              if (!there && a.err) atomicCAS(a.err, 0u, 24u);
               tc::tma_load_4d(dst + c * kKVChunk + i * (PAGE * 128), &tmKV1, bar, c * 64, 0, kvh,
-                              first + min(p + i, last_page));
+                              there ? first + page : 2 * a.pages);
+            }
           }
         }
       };
+      if (tb > 0) next_ids = ids_of(tb * kTilePages);
       for (int j = 0; j < n_cta && !*abort; ++j, ++issued) {
         const int s = j % NS;
+        const int p = (tb + j) * kTilePages;
+        const int4 ids = next_ids;
+        next_ids = ids_of(p + kTilePages);
         const uint32_t parity = ((j / NS) & 1) ^ 1;
         if (!mbar_wait_long(&k_empty[s], parity, abort, a.timeout_ns)) {
           set_err(a.err, 21, abort);
           break;
         }
         tc::mbar_arrive_expect_tx(&k_full[s], kKVBytes);
-        load(smem + Smem::kK + s * kKVBytes, page0, &k_full[s], j);
+        load(smem + Smem::kK + s * kKVBytes, ids, 0, &k_full[s], p);
         if (!mbar_wait_long(&v_empty[s], parity, abort, a.timeout_ns)) {
           set_err(a.err, 21, abort);
           volatile int never = 0;
@@ -232,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         tc::mbar_arrive_expect_tx(&v_full[s], kKVBytes);
-        load(smem + Smem::kV + s * kKVBytes, a.pages + page0, &v_full[s], j);
+        load(smem + Smem::kV + s * kKVBytes, ids, a.pages, &v_full[s], p);
       }
       // copies in flight land before the CTA leaves
       volatile int never = 0;
@@ -473,8 +495,8 @@ CUtensorMap encode(const void* base, int rank, const cuuint64_t* dims, const cuu
 
 void prefill_attention_pages_launch(const void* q, const void* kv, void* o, const int* cu_q, const int* kv_len,
                                     const int* table, int cols, const int* tiles, int n_tiles, int T, int nq, int nkv,
-                                    int pages, float scale, int splits, float* part_o, float* part_lse, uint32_t* err,
-                                    cudaStream_t s) {
+                                    int pages, int placed, float scale, int splits, float* part_o, float* part_lse,
+                                    uint32_t* err, cudaStream_t s) {
   if (n_tiles == 0 || T == 0) return;
   if (nq % nkv != 0) throw std::runtime_error("fmha: nq must be a multiple of nkv");
   if (splits > 1 && (!part_o || !part_lse)) throw std::runtime_error("fmha: split-KV needs scratch buffers");
@@ -492,7 +514,7 @@ void prefill_attention_pages_launch(const void* q, const void* kv, void* o, cons
   };
   const CUtensorMap tkv = page_map(kTilePages), tkv1 = page_map(1);
   PagesArgs a{static_cast<__nv_bfloat16*>(o), cu_q, kv_len, table, reinterpret_cast<const int2*>(tiles), part_o,
-              part_lse, std::max(1, splits), cols, nq, nkv, pages, scale * 1.4426950408889634f, err, 2000000000ull};
+              part_lse, std::max(1, splits), cols, nq, nkv, pages, placed, scale * 1.4426950408889634f, err, 2000000000ull};
   static SmemLimit limit;
   limit.ensure((const void*)fmha_pages_kernel, Smem::kTotal);
   launch_k(fmha_pages_kernel, dim3(n_tiles, nq, a.splits), dim3(kThreads), Smem::kTotal, s, tq, tkv, tkv1, a);

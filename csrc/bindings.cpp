@@ -718,7 +718,7 @@ torch::Tensor prefill_attention_kv8(const torch::Tensor& q, const torch::Tensor&
   }
   prefill_attention_pages_launch(q.data_ptr(), k, out.data_ptr(), cu_q.data_ptr<int>(), kv_len.data_ptr<int>(),
                                  table.data_ptr<int>(), (int)cols, tiles.data_ptr<int>(), (int)tiles.size(0), (int)T,
-                                 (int)nq, (int)nkv, (int)n, (float)scale, (int)splits, po, pl,
+                                 (int)nq, (int)nkv, (int)n, (int)pages, (float)scale, (int)splits, po, pl,
                                  err ? reinterpret_cast<uint32_t*>(err->data_ptr<int>()) : nullptr, stream);
   return out;
 }

@@ -208,13 +208,14 @@ void read_pages_kv8_launch(const Kv8Cache& c, int nkv, const int* block_table, i
                            int64_t ot_stride, const int* kv_len, int R, int max_blocks, void* k_out, void* v_out,
                            int64_t out_pages, cudaStream_t s);
 // prefill_attention_tc_launch over pages that read_pages_kv8_launch wrote: kv
-// [2, pages, nkv, 16, 128], each request's pages consecutive from table[r, 0] on
-// (row stride cols; lengths are clamped to cols pages). scale > 0. Rows that
-// see no key are zeros.
+// [2, pages, nkv, 16, 128], page i of request r at table[r, i] (row stride cols;
+// lengths are clamped to cols pages; consecutive pages load faster). A page that
+// a request needs and whose entry is not in [0, placed) counts as zeros and sets
+// *err. scale > 0. Rows that see no key are zeros.
 void prefill_attention_pages_launch(const void* q, const void* kv, void* o, const int* cu_q, const int* kv_len,
                                     const int* table, int cols, const int* tiles, int n_tiles, int T, int nq, int nkv,
-                                    int pages, float scale, int splits, float* part_o, float* part_lse, uint32_t* err,
-                                    cudaStream_t s);
+                                    int pages, int placed, float scale, int splits, float* part_o, float* part_lse,
+                                    uint32_t* err, cudaStream_t s);
 // decode_attention_launch over the 8-bit cache; lengths are clamped to
 // max_blocks pages, keys of blocks outside the cache do not count. `grid` from
 // decode_kv8_grid (for the current device); part holds

@@ -705,6 +705,62 @@ def test_prefill_rows_without_keys_and_neighbours_with_nan():
         _prefill(ops, q, k8, v8, q_lens, kvl, table, scale=0.0)
 
 
+@pytest.mark.parametrize("splits", [1, 2])
+def test_prefill_by_plans_in_any_order(splits):
+    """Plans that scatter a request's pages, leave room between them, serve
+    longer lengths, or run backwards: the same bits as the packed one."""
+    ops = sub("ops")
+    kv_lens, q_lens, nq, nkv = [333, 70, 1029, 64], [100, 70, 300, 1], 4, 2
+    k8, v8, kvl, table = _cache(kv_lens, nkv, seed=6, columns=70)
+    q = torch.randn(sum(q_lens), nq, D, device="cuda", generator=_gen(2)).to(torch.bfloat16)
+    packed = ops.page_plan(kv_lens, 70)
+    want = _prefill(ops, q, k8, v8, q_lens, kvl, table, splits=splits, plan=ops.PagePlan(packed.table.cuda(), packed.pages))
+    _check_prefill(want, q, k8, v8, table, q_lens, kv_lens)
+    n = packed.pages
+    perm = torch.randperm(n, generator=torch.Generator().manual_seed(0)).to(torch.int32)
+    backwards = torch.arange(n - 1, -1, -1, dtype=torch.int32)
+    room = 3 * torch.arange(n, dtype=torch.int32)
+    for order, pages in ((perm, n), (backwards, n), (room, 3 * n)):
+        t = torch.where(packed.table >= 0, order[packed.table.clamp_min(0).long()], packed.table)
+        got = _prefill(ops, q, k8, v8, q_lens, kvl, table, splits=splits, plan=ops.PagePlan(t.cuda(), pages))
+        assert torch.equal(got, want)
+    longer = ops.page_plan([n + 100 for n in kv_lens], 70)
+    got = _prefill(ops, q, k8, v8, q_lens, kvl, table, splits=splits, plan=ops.PagePlan(longer.table.cuda(), longer.pages))
+    assert torch.equal(got, want)
+    torch.cuda.synchronize()
+    assert ops.gemm_error() == 0
+
+
+def test_prefill_by_a_plan_that_lacks_pages():
+    """Pages that the plan does not place count as zeros, and the error word
+    says so; the requests that it places are right."""
+    ops = sub("ops")
+    kv_lens, q_lens, nq, nkv = [333, 70, 200], [33, 70, 5], 4, 2
+    k8, v8, kvl, table = _cache(kv_lens, nkv, seed=6)
+    q = torch.randn(sum(q_lens), nq, D, device="cuda", generator=_gen(2)).to(torch.bfloat16)
+    short = ops.page_plan([160, 70, 200], table.shape[1])
+    t = short.table.cuda()
+    t[2, 1], t[2, 5] = short.pages, -2 ** 31
+    err = ops.workspace("cuda").err
+    try:
+        out = _prefill(ops, q, k8, v8, q_lens, kvl, table, plan=ops.PagePlan(t, short.pages))
+        none = _prefill(ops, q, k8, v8, q_lens, kvl, table, plan=ops.PagePlan(torch.full_like(t, -1), 0))
+        torch.cuda.synchronize()
+        assert ops.gemm_error() == 24
+    finally:
+        err.zero_()
+    _check_prefill(out[33:103], q[33:103], k8, v8, table[1:2], [70], [70])
+    for r, a, b, lost in ((0, 0, 33, slice(160, 333)), (2, 103, 108, [*range(16, 32), *range(80, 96)])):
+        n = kv_lens[r]
+        k, v = _row(k8, table[r], n).clone(), _row(v8, table[r], n).clone()
+        k[lost], v[lost] = 0.0, 0.0
+        last = torch.arange(n - (b - a), n, device="cuda")
+        want, tol = _attention(q[a:b], k, v, D ** -0.5, last)
+        A, _ = _attention(q[a:b], k, v.abs(), D ** -0.5, last)
+        assert ((out[a:b].double() - want).abs() <= tol + A * 2.0 ** -8 * 1.01).all()
+    assert (none == 0).all()
+
+
 @pytest.mark.parametrize("seed", range(10))
 def test_decode_drawn_batches(seed):
     """Batches of mixed lengths, so that runs of the work list begin and end
