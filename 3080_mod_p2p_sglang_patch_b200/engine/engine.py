@@ -88,6 +88,9 @@ class LLMEngine:
             self.overlap = self.model.overlap_min_rows is not None
         nkv = cfg.kv_heads // self.tp_size
         self.max_blocks_per_seq = (max_seq + PAGE - 1) // PAGE
+        # bf16 pages that one prefill attention call over an 8-bit cache may
+        # read back: 1 GiB, or the longest request (see _prefill_groups)
+        self.scratch_pages = max(self.max_blocks_per_seq, (1 << 30) // PagedKVCache.scratch_bytes(1, nkv, cfg.head_dim))
         if kv_blocks is None:
             kv_blocks = max_batch * self.max_blocks_per_seq + 1
             if mem_fraction is not None and self.device.type == "cuda":
@@ -96,7 +99,8 @@ class LLMEngine:
                 free, total = torch.cuda.mem_get_info(self.device)
                 block_bytes = PagedKVCache.bytes_per_token(cfg.layers, nkv, cfg.head_dim,
                                                            self.kv_cache_dtype.itemsize) * PAGE
-                fit = PagedKVCache.blocks_for_memory(total, free, mem_fraction, block_bytes)
+                fit = PagedKVCache.blocks_for_memory(total, free, mem_fraction, block_bytes,
+                                                     self._scratch_reserve(prefill_graph))
                 if fit < self.max_blocks_per_seq:
                     raise ValueError(f"mem_fraction {mem_fraction}: the KV cache would hold {fit * PAGE} tokens, "
                                      f"fewer than max_seq {max_seq}")
@@ -191,6 +195,20 @@ class LLMEngine:
         if self.device.type != "cuda":
             return host.to(self.device)
         return host.pin_memory().to(self.device, non_blocking=True)
+
+    def _scratch_reserve(self, prefill_graph: bool) -> int:
+        """Bytes that prefill attention over an 8-bit cache may hold at a time:
+        one call's pages (one per lane where micro-batches overlap), and those of
+        the prefill graph, whose memory is its own."""
+        if self.kv_cache_dtype != torch.float8_e4m3fn:
+            return 0
+        # a request cut in two between the lanes is read back by both
+        batch = (self.max_batch + self.overlap) * self.max_blocks_per_seq
+        lanes = 2 if self.overlap else 1
+        pages = min(batch, lanes * self.scratch_pages)
+        if prefill_graph:
+            pages += lanes * self.max_blocks_per_seq
+        return PagedKVCache.scratch_bytes(pages, self.cfg.kv_heads // self.tp_size, self.cfg.head_dim)
 
     def _reserve_scratch(self):
         if self.impl == "oracle" or self.device.type != "cuda":
@@ -358,36 +376,74 @@ class LLMEngine:
 
             return self.model.forward(ids_d, pos_d, slots_d, self.kv.caches, attn, last_d,
                                       return_hidden=return_hidden)
+        if self.kv_cache_dtype == torch.float8_e4m3fn:
+            attn = self._attn_over_fp8(q_lens, kv_lens, bt)
+            halves = self._attn_halves(q_lens, kv_lens, bt, T, self._attn_over_fp8)
+            return self.model.forward(ids_d, pos_d, slots_d, self.kv.caches, attn, last_d,
+                                      return_hidden=return_hidden, attn_halves=halves)
         cu = torch.zeros(R + 1, dtype=torch.int32)
         cu[1:] = torch.tensor(q_lens, dtype=torch.int32).cumsum(0)
         cu_d = self._h2d(cu)
         tiles = self._h2d(ops.prefill_tiles(q_lens))
         scale = self.model.scale
         splits = ops.prefill_splits(tiles.shape[0], self.cfg.heads // self.tp_size, max(kv_lens))
-        kw = self._page_plan(kv_lens)
 
         def attn(li, q, kc, vc):
-            return ops.prefill_attention(q, kc, vc, cu_d, kvl_d, bt, tiles, scale, splits=splits, **kw)
+            return ops.prefill_attention(q, kc, vc, cu_d, kvl_d, bt, tiles, scale, splits=splits)
 
-        halves = self._attn_halves(q_lens, kv_lens, bt, T, self._page_plan)
+        halves = self._attn_halves(q_lens, kv_lens, bt, T)
         return self.model.forward(ids_d, pos_d, slots_d, self.kv.caches, attn, last_d, return_hidden=return_hidden,
                                   attn_halves=halves)
 
-    def _page_plan(self, kv_lens) -> dict:
-        """Prefill attention's scratch pages over an 8-bit cache, packed by the
-        requests' lengths (nothing for bf16, which is read in place)."""
-        if self.kv_cache_dtype != torch.float8_e4m3fn:
-            return {}
-        plan = ops.page_plan(kv_lens, self.max_blocks_per_seq)
-        return {"plan": ops.PagePlan(self._h2d(plan.table), plan.pages)}
+    def _prefill_groups(self, kv_lens):
+        """A prefill batch over an 8-bit cache in runs [(first, end), ...] of
+        requests whose pages, read back to bf16, stay within ``scratch_pages``:
+        requests that share a long prefix each read it back, so a batch's pages
+        may be many times the cache's."""
+        groups, first, pages = [], 0, 0
+        for i, n in enumerate(kv_lens):
+            mine = PagedKVCache.blocks_for(n)
+            if i > first and pages + mine > self.scratch_pages:
+                groups.append((first, i))
+                first, pages = i, 0
+            pages += mine
+        return groups + [(first, len(kv_lens))]
 
-    def _attn_halves(self, q_lens, kv_lens, bt, T, page_plan=None):
+    def _attn_over_fp8(self, q_lens, kv_lens, bt):
+        """Prefill attention (layer, q, k_cache, v_cache) -> o of a ragged batch
+        over an 8-bit cache: one call per group of ``_prefill_groups``, its
+        scratch pages packed by the requests' lengths."""
+        nq = self.cfg.heads // self.tp_size
+        scale = self.model.scale
+        calls, row = [], 0
+        for a, b in self._prefill_groups(kv_lens):
+            ql, kl = q_lens[a:b], kv_lens[a:b]
+            cu = torch.zeros(b - a + 1, dtype=torch.int32)
+            cu[1:] = torch.tensor(ql, dtype=torch.int32).cumsum(0)
+            meta = self._h2d(torch.cat([cu, torch.tensor(kl, dtype=torch.int32)]))
+            tiles = self._h2d(ops.prefill_tiles(ql))
+            plan = ops.page_plan(kl, self.max_blocks_per_seq)
+            calls.append((slice(row, row + sum(ql)), meta[:b - a + 1], meta[b - a + 1:], bt[a:b], tiles,
+                          ops.prefill_splits(tiles.shape[0], nq, max(kl)),
+                          ops.PagePlan(self._h2d(plan.table), plan.pages)))
+            row += sum(ql)
+
+        def attn(li, q, kc, vc):
+            out = torch.empty_like(q)
+            for rows, cu, kvl, table, tiles, splits, plan in calls:
+                ops.prefill_attention(q[rows], kc, vc, cu, kvl, table, tiles, scale, out=out[rows], splits=splits,
+                                      plan=plan)
+            return out
+        return attn
+
+    def _attn_halves(self, q_lens, kv_lens, bt, T, attn_of=None):
         """Attention of each micro-batch of an overlapped prefill batch
         (model.overlap_split), or None. A piece that straddles the split is
         cut in two: its first rows end the first micro-batch with a kv length
         shortened by the rows that follow; the rest start the second, whose
         keys include the first part (written to the cache earlier in the same
-        layer)."""
+        layer). ``attn_of(q_lens, kv_lens, block_table)``: the attention of a
+        micro-batch, by default over a bf16 cache."""
         T1 = self.model.overlap_split(T)
         if T1 is None:
             return None
@@ -410,6 +466,10 @@ class LLMEngine:
         for pl in parts:
             ql = [p[0] for p in pl]
             kl = [p[1] for p in pl]
+            if attn_of is not None:
+                sel = self._h2d(torch.tensor([p[2] for p in pl], dtype=torch.int64))
+                fns.append(attn_of(ql, kl, bt.index_select(0, sel)))
+                continue
             cu = torch.zeros(len(ql) + 1, dtype=torch.int32)
             cu[1:] = torch.tensor(ql, dtype=torch.int32).cumsum(0)
             meta = self._h2d(torch.cat([cu, torch.tensor(kl, dtype=torch.int32),
@@ -419,14 +479,10 @@ class LLMEngine:
             bt_h = bt.index_select(0, sel.long())
             tiles_h = self._h2d(ops.prefill_tiles(ql))
             splits_h = ops.prefill_splits(tiles_h.shape[0], nq, max(kl))
-            plan = (page_plan(kl) if page_plan else {}).get("plan")
 
-            def make(plan, cu=cu_h, kvl=kvl_h, bt=bt_h, tiles=tiles_h, splits=splits_h):
-                def f(li, q, kc, vc, cu_h=cu, kvl_h=kvl, bt_h=bt, tiles_h=tiles, splits_h=splits):
-                    return ops.prefill_attention(q, kc, vc, cu_h, kvl_h, bt_h, tiles_h, scale, splits=splits_h,
-                                                 plan=plan)
-                return f
-            fns.append(make(plan))
+            def f(li, q, kc, vc, cu_h=cu_h, kvl_h=kvl_h, bt_h=bt_h, tiles_h=tiles_h, splits_h=splits_h):
+                return ops.prefill_attention(q, kc, vc, cu_h, kvl_h, bt_h, tiles_h, scale, splits=splits_h)
+            fns.append(f)
         return (T1, fns[0], fns[1])
 
     def decode_inputs(self, reqs):

@@ -179,11 +179,18 @@ class PagedKVCache:
         return layers * 2 * kv_heads * (head_dim * dtype_bytes + (dtype_bytes == 1))
 
     @staticmethod
-    def blocks_for_memory(total_bytes: int, free_bytes: int, fraction: float, block_bytes: int) -> int:
+    def scratch_bytes(pages, kv_heads, head_dim):
+        """bf16 keys and values of ``pages`` pages of one layer, as prefill
+        attention over an 8-bit cache reads them back."""
+        return pages * 2 * kv_heads * PAGE * head_dim * 2
+
+    @staticmethod
+    def blocks_for_memory(total_bytes: int, free_bytes: int, fraction: float, block_bytes: int,
+                          reserved_bytes: int = 0) -> int:
         """Blocks that fit when weights plus KV cache may use ``fraction`` of
         the device's memory (sglang's ``--mem-fraction-static``): the budget
-        is fraction x total minus what is already in use."""
-        budget = fraction * total_bytes - (total_bytes - free_bytes)
+        is fraction x total minus what is already in use and ``reserved_bytes``."""
+        budget = fraction * total_bytes - (total_bytes - free_bytes) - reserved_bytes
         return max(0, int(budget // block_bytes))
 
     def slots(self, blocks, start: int, n: int):

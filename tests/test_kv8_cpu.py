@@ -443,3 +443,41 @@ def test_cache_dtype_names_and_sizes():
         kv.PagedKVCache(1, 2, 64, 5, "cpu", torch.float8_e4m3fn)
     p = sub("server.cli").build_parser()
     assert p.parse_args(["--kv-cache-dtype", "fp8_e4m3"]).kv_cache_dtype == "fp8_e4m3"
+
+
+def _bare_engine(**kw):
+    """An engine's sizes without weights or a cache."""
+    eng_mod, models = sub("engine"), sub("models")
+    e = object.__new__(eng_mod.LLMEngine)
+    e.cfg = models.LlamaConfig(**{**models.LlamaConfig.tiny().__dict__, "heads": 32, "kv_heads": 8})
+    e.kv_cache_dtype, e.tp_size, e.overlap = torch.float8_e4m3fn, 1, False
+    e.max_batch, e.max_blocks_per_seq, e.scratch_pages = 64, 512, 16384
+    e.__dict__.update(kw)
+    return e
+
+
+def test_prefill_scratch_is_bounded_and_counted_in_the_memory_fraction():
+    """However many requests share a prefix, a call reads back no more than its
+    bound, and the cache leaves that much of the memory fraction free."""
+    kv = sub("engine.kv_cache")
+    e = _bare_engine(scratch_pages=20)
+    assert e._prefill_groups([1]) == [(0, 1)]
+    assert e._prefill_groups([160, 160, 16]) == [(0, 2), (2, 3)]
+    assert e._prefill_groups([16] * 20) == [(0, 20)] and e._prefill_groups([17] * 20) == [(0, 10), (10, 20)]
+    assert e._prefill_groups([9999, 5, 9999]) == [(0, 1), (1, 2), (2, 3)]
+    for lens in ([3, 400, 20, 20, 300, 1, 17], [320] * 5):
+        groups = e._prefill_groups(lens)
+        assert [i for a, b in groups for i in range(a, b)] == list(range(len(lens)))
+        assert all(b - a == 1 or sum(-(-n // PAGE) for n in lens[a:b]) <= 20 for a, b in groups)
+    # 8 kv heads: 64 KB a page of one layer's keys and values in bf16
+    page = kv.PagedKVCache.scratch_bytes(1, 8, 128)
+    assert page == 2 * 8 * 16 * 128 * 2
+    assert _bare_engine(kv_cache_dtype=torch.bfloat16)._scratch_reserve(True) == 0
+    assert _bare_engine()._scratch_reserve(False) == 16384 * page                  # the bound: 64 x 512 pages are more
+    assert _bare_engine(max_batch=2)._scratch_reserve(False) == 2 * 512 * page     # all that a batch can need
+    assert _bare_engine()._scratch_reserve(True) == (16384 + 512) * page
+    assert _bare_engine(overlap=True)._scratch_reserve(True) == 2 * (16384 + 512) * page
+    assert _bare_engine(overlap=True, max_batch=2)._scratch_reserve(False) == 3 * 512 * page
+    GB = 1 << 30
+    assert kv.PagedKVCache.blocks_for_memory(180 * GB, 164 * GB, 0.9, 1 << 20, GB) == \
+        kv.PagedKVCache.blocks_for_memory(180 * GB, 164 * GB, 0.9, 1 << 20) - 1024

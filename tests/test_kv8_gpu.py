@@ -923,6 +923,32 @@ def test_native_and_oracle_score_text_alike_over_an_8_bit_cache():
     assert (scores[0] - scores[1]).abs().mean().item() < 0.05
 
 
+def _attention_inputs(eng, kv_lens, q_lens, seed):
+    cfg = eng.cfg
+    k8, v8, kvl, table = _cache(kv_lens, cfg.kv_heads, seed=seed, columns=eng.max_blocks_per_seq)
+    q = torch.randn(sum(q_lens), cfg.heads, D, device="cuda", generator=_gen(seed)).to(torch.bfloat16)
+    return k8, v8, kvl, table, q
+
+
+@pytest.mark.parametrize("scratch", [1, 30, 10 ** 6])
+def test_engine_prefill_attention_in_groups_of_bounded_scratch(scratch):
+    """A batch's attention in as many calls as its scratch bound asks for."""
+    from test_engine_gpu import CFG
+
+    ops, launches = sub("ops"), sub("utils.launches")
+    eng = _native(CFG, use_graphs=False, max_seq=1024)
+    eng.scratch_pages = scratch
+    kv_lens, q_lens = [100, 264, 1, 777, 16, 300], [100, 64, 1, 257, 3, 17]
+    k8, v8, kvl, table, q = _attention_inputs(eng, kv_lens, q_lens, 4)
+    attn = eng._attn_over_fp8(q_lens, kv_lens, table)
+    before = launches.get()
+    out = attn(0, q, k8, v8)
+    calls = {1: 6, 30: 3, 10 ** 6: 1}[scratch]  # pages 7 + 17 + 1, 49, 1 + 19
+    assert 2 * calls <= launches.get() - before <= 3 * calls
+    _check_prefill(out, q, k8, v8, table, q_lens, kv_lens)
+    assert ops.gemm_error() == 0
+
+
 @pytest.mark.skipif(not torch.cuda.is_available() or torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_second_device_while_the_first_is_current():
     ops = sub("ops")
