@@ -481,3 +481,17 @@ def test_prefill_scratch_is_bounded_and_counted_in_the_memory_fraction():
     GB = 1 << 30
     assert kv.PagedKVCache.blocks_for_memory(180 * GB, 164 * GB, 0.9, 1 << 20, GB) == \
         kv.PagedKVCache.blocks_for_memory(180 * GB, 164 * GB, 0.9, 1 << 20) - 1024
+
+
+def test_overlapped_halves_over_an_8_bit_cache_cut_as_over_bf16():
+    """The micro-batches' requests, lengths and table rows, as given to the
+    8-bit cache's attention."""
+    import types
+
+    e = _bare_engine(model=types.SimpleNamespace(overlap_split=lambda T: 256, scale=0.1), device=torch.device("cpu"))
+    bt = torch.arange(3 * 8, dtype=torch.int32).view(3, 8)
+    got = []
+    T1, a, b = e._attn_halves([100, 300, 50], [100, 700, 1050], bt, 450, lambda *args: got.append(args) or len(got))
+    assert (T1, a, b) == (256, 1, 2)
+    assert got[0][:2] == ([100, 156], [100, 700 - 144]) and torch.equal(got[0][2], bt[[0, 1]])
+    assert got[1][:2] == ([144, 50], [700, 1050]) and torch.equal(got[1][2], bt[[1, 2]])

@@ -949,6 +949,69 @@ def test_engine_prefill_attention_in_groups_of_bounded_scratch(scratch):
     assert ops.gemm_error() == 0
 
 
+@pytest.mark.parametrize("scratch", [10, 10 ** 6])
+def test_overlapped_halves_of_a_prefill_batch(scratch):
+    """The two micro-batches' attention, each on a stream of its own, the
+    straddling request cut between them."""
+    from test_engine_gpu import CFG
+
+    ops = sub("ops")
+    eng = _native(CFG, use_graphs=False, max_seq=1024)
+    eng.scratch_pages = scratch
+    kv_lens, q_lens = [100, 700, 450], [100, 300, 50]
+    k8, v8, kvl, table, q = _attention_inputs(eng, kv_lens, q_lens, 5)
+    eng.model.overlap_split = lambda T: 256
+    T1, first, second = eng._attn_halves(q_lens, kv_lens, table, 450, eng._attn_over_fp8)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        a = first(0, q[:T1], k8, v8)
+        with torch.cuda.stream(side), ops.workspace_lane(1):
+            b = second(0, q[T1:], k8, v8)
+        torch.cuda.synchronize()
+        _check_prefill(torch.cat([a, b]), q, k8, v8, table, q_lens, kv_lens)
+    assert ops.gemm_error() == 0
+
+
+def test_prefill_graph_halves_over_an_8_bit_cache():
+    """PrefillGraphRunner's two micro-batches, captured on two streams of one
+    graph and replayed for chunks of growing context."""
+    from test_engine_gpu import CFG
+
+    ops, gr = sub("ops"), sub("engine.graph_runner")
+    eng = _native(CFG, use_graphs=False, max_seq=1024)
+    T, T1 = 300, 128
+    eng.model.overlap_split = lambda n: T1
+    runner = gr.PrefillGraphRunner(eng, T)
+    seen = {}
+    eng.model.forward = lambda *args, attn_halves=None, **kw: seen.update(halves=attn_halves, whole=args[4])
+    runner._forward()
+    split, first, second = seen["halves"]
+    assert split == T1
+    k8, v8, _, table, q = _attention_inputs(eng, [500], [T], 6)
+    side, lane = torch.cuda.Stream(), torch.cuda.Stream()
+    for h in (first, second, seen["whole"]):  # workspaces before the capture
+        h(0, q[:T1] if h is first else q[T1:] if h is second else q, k8, v8)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        lane.wait_stream(side)
+        a = first(0, q[:T1], k8, v8)
+        with torch.cuda.stream(lane), ops.workspace_lane(1):
+            b = second(0, q[T1:], k8, v8)
+        side.wait_stream(lane)
+        whole = seen["whole"](0, q, k8, v8)
+    runner.bt.copy_(table[:1])
+    for n in (300, 417, 500):
+        runner.kvl.fill_(n)
+        runner.halves[0]["kvl"].fill_(n - (T - T1))
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_prefill(torch.cat([a, b]), q, k8, v8, table, [T], [n])
+        _check_prefill(whole, q, k8, v8, table, [T], [n])
+    assert ops.gemm_error() == 0
+
+
 @pytest.mark.skipif(not torch.cuda.is_available() or torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_second_device_while_the_first_is_current():
     ops = sub("ops")
