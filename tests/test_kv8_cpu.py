@@ -495,3 +495,29 @@ def test_overlapped_halves_over_an_8_bit_cache_cut_as_over_bf16():
     assert (T1, a, b) == (256, 1, 2)
     assert got[0][:2] == ([100, 156], [100, 700 - 144]) and torch.equal(got[0][2], bt[[0, 1]])
     assert got[1][:2] == ([144, 50], [700, 1050]) and torch.equal(got[1][2], bt[[1, 2]])
+
+
+def _tp_worker(rank, world):
+    from test_engine_cpu import CFG
+
+    eng_mod, par = sub("engine"), sub("parallel")
+    tp = par.TPGroup(None, "cpu", use_mailbox=False)
+    eng = eng_mod.LLMEngine(CFG, tp=tp, impl="oracle", device="cpu", full_init=True, seed=0, max_batch=4, max_seq=512,
+                            chunk=32, kv_cache_dtype="fp8_e4m3", mixed_chunk=True)
+    assert eng.kv.caches[0][0].shape[1] == CFG.kv_heads // world
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, CFG.vocab, (n,), generator=g).tolist() for n in (70, 9, 33)]
+    return {"prompts": prompts, "out": eng.generate(prompts, max_new_tokens=4)}
+
+
+def test_two_tensor_parallel_ranks_over_an_8_bit_cache():
+    from _mp import run_ranks
+    from test_engine_cpu import CFG, LOGIT_TOL
+
+    models = sub("models")
+    res = run_ranks(_tp_worker, 2)
+    assert res[0] == res[1]
+    w = models.LlamaWeights(CFG, 0, 1, "cpu", seed=0, full_init=True)  # the same model, unsharded
+    for p, o in zip(res[0]["prompts"], res[0]["out"]):
+        assert len(o) == 4
+        _near_argmax(CFG, w, p, o, LOGIT_TOL)

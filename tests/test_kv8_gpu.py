@@ -780,6 +780,22 @@ def test_decode_drawn_batches(seed):
     _check_decode(out, q, k8, v8, table, lens)
 
 
+def test_decode_among_other_requests():
+    """A request among others of changing lengths: the runs' borders move, and
+    with them the last bits; each result is within the tolerance, and the same
+    batch gives the same bits again."""
+    ops = sub("ops")
+    nq, nkv, n = 8, 2, 777
+    k8, v8, _, table = _cache([n] + [3000] * 15, nkv, seed=1)
+    q = torch.randn(16, nq, D, device="cuda", generator=_gen(1)).to(torch.bfloat16)
+    want, tol = _attention(q[:1], _row(k8, table[0], n), _row(v8, table[0], n), D ** -0.5)
+    for others in ([3000] * 15, [0] * 15, [1] * 15, [100, 2000] * 7 + [5], list(range(0, 3000, 200))):
+        kvl = torch.tensor([n] + others, dtype=torch.int32, device="cuda")
+        out = ops.decode_attention(q, k8, v8, kvl, table)
+        assert ((out[:1].double() - want).abs() <= tol).all()
+        assert torch.equal(ops.decode_attention(q, k8, v8, kvl, table), out)
+
+
 # ---------------------------------------------------------------- together
 def test_append_then_attend():
     """A prompt in two chunks, then tokens one by one, as a model's layer
