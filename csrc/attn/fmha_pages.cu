@@ -18,12 +18,16 @@
 // half the time. Here S of the next tile is issued as soon as the softmax warps
 // have the present one in registers, and PV runs under the next tile's softmax.
 // Measured, 1024 queries over 8192 keys of 32 heads, read-back (7.5 us) included:
-// 149 us, 867 TFLOP/s (53 % of the measured GEMM rate; 128 of 148 SMs have a
-// CTA); the kernel over the cache itself on the same pages 173, 128-key tiles
-// 155. A turn of 64 keys for both tiles takes 2300 cycles, 1280 of them tensor
+// 150 us on the same inputs again, 152 on changing ones (846 TFLOP/s, 51 % of the
+// measured GEMM rate; 128 of 148 SMs have a CTA); the kernel over the cache itself
+// on the same pages 173, 128-key tiles 155. A turn of 64 keys for both tiles takes 2300 cycles, 1280 of them tensor
 // work: the softmax warps of the two tiles share a scheduler and its exponential
 // unit and lengthen one another. Two threads per row (165 us), packed FMAs (150)
 // and polynomials for some of the exponentials (153 to 159) did not help.
+// P is rounded to bf16, which costs about as much again as the output's own
+// rounding (1.35 times the error of fp32 weights against 64 bits): A and B of one
+// product have the same type, and V's rows keep their exponents, for which f16 has
+// no range. The row sum takes the weights before that rounding.
 // Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer, 2-5 / 6-9 softmax and
 // epilogue of query tile 0 / 1. Every mbarrier wait is bounded; on timeout the
 // CTA records an error, drains its copies and MMAs, frees TMEM and exits.

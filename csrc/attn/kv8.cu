@@ -142,9 +142,12 @@ MBX_DEVICE void store_e4m3(const float (&x)[8], const float (&y)[8], uint8_t* ds
 constexpr int kAppendWarps = 8;
 constexpr int kMaxTokens = 32;  // of a CTA that writes k and v
 
-// Bound by the rows' stream: 328 MB in 65 us (77 % of the measured copy rate) for
-// 8005 tokens of 64 q and 2 x 8 kv heads; 8.0 us for 1024 of 32 + 2 x 8, where a
-// warp per head and 4-byte loads took 12.
+// Bound by the rows' stream: 316 MB in 64 us (76 % of the measured copy rate) for
+// 8005 tokens of 64 q and 2 x 8 kv heads; 8.3 us for 1024 of 32 + 2 x 8, where a
+// warp per head and 4-byte loads took 12. The search for later tokens of the same
+// slot is quadratic: tokens^2 / 32 slots read above 16384 tokens, and with pages
+// scattered over the cache most of them compared with a CTA's own (65536 tokens of
+// 8 + 2 x 1 heads: 209 us with pages in a row, 519 scattered, of 54 for the bytes).
 // CTAs 0 .. kv_ctas - 1 write k and v of `tokens` tokens each, the others rotate
 // q: a warp takes `passes` times four heads of one token, whose angles it loads
 // once. k is normalised and rotated in 64 bits, so that the stored byte is the
@@ -655,8 +658,9 @@ struct HeadState {
 //     last of those CTAs to arrive merges these in CTA order.
 // All orders are fixed, so results do not depend on timing. At most one pair
 // enters a CTA's run and one leaves it, hence two global partials per CTA.
-// Against a fixed split per request: 64 ragged requests 188 -> 136 us, 8 of
-// 131072 keys on one kv head 185 -> 76 us, one token 15.6 -> 6.8 us.
+// Against a fixed split per request: 64 ragged requests 188 -> 109 us, 8 of
+// 131072 keys on one kv head 185 -> 59 us, one token 15.6 -> 6.4 us (with the
+// copies' shape and the look-ahead below).
 constexpr int kWarps = 8;          // 12 and 16, with shallower rings, measured 0 to 40 % slower on few requests
 constexpr int kAlone = 8;          // pages a warp takes alone rather than share them and merge (4 and 16: the same)
 constexpr float kMergeCost = 1.f;  // see plan_work (one request of 32768 keys on one kv head: 0.5 and 2 +13 %)
