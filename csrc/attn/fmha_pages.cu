@@ -20,10 +20,11 @@
 // Measured, 1024 queries over 8192 keys of 32 heads, read-back (7.5 us) included:
 // 150 us on the same inputs again, 152 on changing ones (846 TFLOP/s, 51 % of the
 // measured GEMM rate; 128 of 148 SMs have a CTA); the kernel over the cache itself
-// on the same pages 173, 128-key tiles 155. A turn of 64 keys for both tiles takes 2300 cycles, 1280 of them tensor
-// work: the softmax warps of the two tiles share a scheduler and its exponential
-// unit and lengthen one another. Two threads per row (165 us), packed FMAs (150)
-// and polynomials for some of the exponentials (153 to 159) did not help.
+// on the same pages 173, 128-key tiles 155. A turn of 64 keys for both tiles takes
+// 2300 cycles, 1280 of them tensor work: the softmax warps of the two tiles share a
+// scheduler and its exponential unit and lengthen one another. Two threads per row
+// (165 us), packed FMAs (150) and polynomials for some of the exponentials (153 to
+// 159) did not help.
 // P is rounded to bf16, which costs about as much again as the output's own
 // rounding (1.35 times the error of fp32 weights against 64 bits): A and B of one
 // product have the same type, and V's rows keep their exponents, for which f16 has
@@ -518,7 +519,8 @@ void prefill_attention_pages_launch(const void* q, const void* kv, void* o, cons
   };
   const CUtensorMap tkv = page_map(kTilePages), tkv1 = page_map(1);
   PagesArgs a{static_cast<__nv_bfloat16*>(o), cu_q, kv_len, table, reinterpret_cast<const int2*>(tiles), part_o,
-              part_lse, std::max(1, splits), cols, nq, nkv, pages, placed, scale * 1.4426950408889634f, err, 2000000000ull};
+              part_lse, std::max(1, splits), cols, nq, nkv, pages, placed, scale * 1.4426950408889634f, err,
+              2000000000ull};
   static SmemLimit limit;
   limit.ensure((const void*)fmha_pages_kernel, Smem::kTotal);
   launch_k(fmha_pages_kernel, dim3(n_tiles, nq, a.splits), dim3(kThreads), Smem::kTotal, s, tq, tkv, tkv1, a);

@@ -375,8 +375,8 @@ __global__ void __launch_bounds__(kReadWarps * 32) read_pages_kernel(ReadArgs a,
 //    is. So keys that contribute down to 2^-24 of the largest keep 11 bits (bf16
 //    would keep 8), and a row that the head ignores costs the others nothing,
 //    whatever its exponent. The maxima only move when a page exceeds one by more
-//    than 2^4. Weights below 2^-126 of the largest are zero, as fp32 has none, and
-//    stay out of mv. (2^(s - m + ve + d) as an exponential of its own: 64 requests
+//    than 2^4. Weights below 2^-126 of the largest so far are zero, as fp32 has
+//    none, and stay out of mv. (2^(s - m + ve + d) as an exponential of its own: 64 requests
 //    of 4096 keys 101 -> 102 us, with 16 heads per kv head 131 -> 138.)
 MBX_DEVICE float ex2(float x) {
   float y;
